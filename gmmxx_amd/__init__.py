@@ -9,6 +9,11 @@ the same signatures and run on the same kernels; ``batch_gmm_*_hip``,
 ``fit_large_n`` and the ``*_large_n`` inference functions are this package's
 own spellings of them.  ``hip_ops`` mirrors the reference's experimental
 ``cuda_ops`` module.
+
+``layer_norm``, ``route_rows``, ``grouped_matmul`` and ``combine_rows``
+(``gmmxx_amd.experts``) make a mixture's components, or any gate's outputs, into
+a sparsely gated layer of experts with gradients; they have no reference
+counterpart.
 """
 
 from ._hip import HipBackendUnavailable, HipRuntimeError, HipRuntimeFallback, has_hip, require_hip
@@ -27,6 +32,7 @@ from .em import (batch_gmm_Diagonal, batch_gmm_Diagonal_hip, batch_gmm_Diagonal_
 from .interface import GMMXX
 from .large_n import (batch_gmm_largeN_cpu, fit_large_n, large_n_predict_cpu, large_n_predict_proba_cpu,
                       large_n_score_samples_cpu, predict_large_n, predict_proba_large_n, score_samples_large_n)
+from .experts import Routing, combine_rows, grouped_matmul, layer_norm, route_rows
 from . import hip_ops
 
 __all__ = [
@@ -46,6 +52,7 @@ __all__ = [
     "batch_gmm_largeN_cpu", "large_n_predict_cpu", "large_n_predict_proba_cpu", "large_n_score_samples_cpu",
     "batch_gmm_Spherical_hip", "batch_gmm_Diagonal_hip", "batch_gmm_Tied_hip", "batch_gmm_Full_hip",
     "fit_large_n", "predict_large_n", "predict_proba_large_n", "score_samples_large_n", "hip_ops",
+    "Routing", "combine_rows", "grouped_matmul", "layer_norm", "route_rows",
 ]
 
 __version__ = "0.1.0"

@@ -99,6 +99,21 @@ def _declare(lib):
         "gmmxx_hip_topk_workspace_bytes": (i64, [P, ctypes.c_int]),
         "gmmxx_hip_estep_stats_topk": (ctypes.c_int, [P, vp, vp, vp, vp, f64, f64, ctypes.c_int, vp, vp, vp,
                                                       vp, vp, i64, vp]),
+        "gmmxx_hip_layer_norm": (ctypes.c_int, [i32, i32, i64, i64, vp, i64, vp, vp, f64, vp, vp, vp, vp]),
+        "gmmxx_hip_layer_norm_workspace_bytes": (i64, [i64, i64]),
+        "gmmxx_hip_layer_norm_backward": (ctypes.c_int, [i32, i32, i64, i64, vp, i64, vp, i64, vp, vp, vp, vp, vp, vp,
+                                                         vp, i64, vp]),
+        "gmmxx_hip_route_workspace_bytes": (i64, [i64, i64, i64]),
+        "gmmxx_hip_route": (ctypes.c_int, [i32, i64, i64, i64, i32, vp, i64, vp, vp, vp, vp, vp, vp, vp, i64, vp]),
+        "gmmxx_hip_route_backward": (ctypes.c_int, [i32, i64, i64, i64, i32, vp, i64, vp, vp, vp, vp, vp, vp]),
+        "gmmxx_hip_grouped_matmul": (ctypes.c_int, [i32, i64, i64, i64, i64, i64, vp, i64, vp, vp, i64, i64, i64, vp,
+                                                    vp, i32, vp, i32, vp]),
+        "gmmxx_hip_grouped_workspace_bytes": (i64, [i64, i64, i64, i64]),
+        "gmmxx_hip_grouped_weight_grad": (ctypes.c_int, [i32, i64, i64, i64, i64, i64, vp, i64, vp, vp, i64, vp, i32,
+                                                         vp, vp, vp, i64, vp]),
+        "gmmxx_hip_combine": (ctypes.c_int, [i32, i64, i64, i64, i64, vp, i32, i64, vp, vp, vp, vp, vp]),
+        "gmmxx_hip_combine_backward": (ctypes.c_int, [i32, i64, i64, i64, i64, vp, i64, vp, vp, vp, vp, i64, vp, vp,
+                                                      vp]),
     }
     for name, (res, args) in sig.items():
         fn = getattr(lib, name)
@@ -115,7 +130,11 @@ def exported_symbols() -> Tuple[str, ...]:
             "gmmxx_hip_predict_proba_score",
             "gmmxx_hip_gram", "gmmxx_hip_finalize_stats", "gmmxx_hip_topk_workspace_bytes",
             "gmmxx_hip_estep_stats_topk", "gmmxx_hip_kmeans_pp_workspace_bytes", "gmmxx_hip_kmeans_pp",
-            "gmmxx_hip_lloyd_update", "gmmxx_hip_exchanges", "gmmxx_hip_workspace_init")
+            "gmmxx_hip_lloyd_update", "gmmxx_hip_exchanges", "gmmxx_hip_workspace_init",
+            "gmmxx_hip_layer_norm", "gmmxx_hip_layer_norm_workspace_bytes", "gmmxx_hip_layer_norm_backward",
+            "gmmxx_hip_route_workspace_bytes", "gmmxx_hip_route", "gmmxx_hip_route_backward",
+            "gmmxx_hip_grouped_matmul", "gmmxx_hip_grouped_workspace_bytes", "gmmxx_hip_grouped_weight_grad",
+            "gmmxx_hip_combine", "gmmxx_hip_combine_backward")
 
 
 def load_library(path: Optional[str] = None):

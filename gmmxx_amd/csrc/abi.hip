@@ -367,6 +367,33 @@ int check_hip(const char* what) {
   return GMMXX_OK;
 }
 
+}  // namespace
+
+namespace gx {
+
+// The messages are built of literals that fit a std::string's own buffer or are
+// allocated; a failing allocation leaves the status without its message.
+int set_error(int code, const char* msg) noexcept {
+  try {
+    g_last_error = msg;
+  } catch (...) {
+    g_last_error.clear();
+  }
+  return code;
+}
+
+int launch_status(const char* what) noexcept {
+  const hipError_t e = hipGetLastError();
+  if (e == hipSuccess) return GMMXX_OK;
+  char msg[256];
+  snprintf(msg, sizeof(msg), "%s: %s", what, hipGetErrorString(e));
+  return set_error(GMMXX_ERR_HIP, msg);
+}
+
+}  // namespace gx
+
+namespace {
+
 // em: the EM iteration's passes, whose tied logits leave out the per-row xᵀPx
 // (a row constant: responsibilities and labels do not depend on it, and the
 // log-likelihood takes it back as -½ tr(P XᵀX) in the combine phase).

@@ -208,4 +208,9 @@ void launch_kpp(const KppArgs& a, hipStream_t s);
 void launch_lloyd_update(const float* nk, const float* sum_x, float* means, int64_t M, int D, float* shift,
                          hipStream_t s);
 
+// Records the calling thread's error message and returns `code`; the status of the
+// launches just made (abi.hip).
+int set_error(int code, const char* msg) noexcept;
+int launch_status(const char* what) noexcept;
+
 }  // namespace gx

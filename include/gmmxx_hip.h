@@ -294,6 +294,86 @@ int gmmxx_hip_kmeans_pp(const float* sample, int64_t B, int64_t S, int64_t D, in
 int gmmxx_hip_lloyd_update(int64_t B, int64_t D, int64_t K, const float* nk, const float* sum_x, float* means,
                            float* shift, void* stream);
 
+/* ---------------------------------------------------------------------------
+ * The sparsely gated layer: rows normalised, sent to their best experts (a
+ * mixture's components or a gate's outputs), multiplied by the experts' own
+ * matrices and added up again.  No reference counterpart.  Elements are fp32,
+ * bf16 or fp16 (enum gmmxx_dtype `elem`); sums, statistics and gates are fp32 and
+ * results are rounded once.  Rows of D elements lie `ld` elements apart (>= 0) and
+ * may start at any element; outputs are contiguous.  A call with no rows returns
+ * GMMXX_OK and launches nothing.
+ * ------------------------------------------------------------------------- */
+
+/* y = (x - mean) rstd w + b for N rows of D <= 65536 elements, with rstd =
+ * 1 / sqrt(variance + eps).  weight and bias have D elements of type param_elem
+ * (elem or GMMXX_F32), NULL: ones / zeros.  mean and rstd (N floats each, for the
+ * backward pass) may both be NULL. */
+int gmmxx_hip_layer_norm(int elem, int param_elem, int64_t N, int64_t D, const void* x, int64_t ldx,
+                         const void* weight, const void* bias, double eps, void* y, float* mean, float* rstd,
+                         void* stream);
+
+/* Gradients of gmmxx_hip_layer_norm from dy: dx (N, D), dweight and dbias (D
+ * elements of param_elem; NULL: not wanted).  The workspace takes
+ * gmmxx_hip_layer_norm_workspace_bytes and is needed where dweight or dbias is. */
+int64_t gmmxx_hip_layer_norm_workspace_bytes(int64_t N, int64_t D);
+int gmmxx_hip_layer_norm_backward(int elem, int param_elem, int64_t N, int64_t D, const void* x, int64_t ldx,
+                                  const void* dy, int64_t lddy, const void* weight, const float* mean,
+                                  const float* rstd, void* dx, void* dweight, void* dbias, void* workspace,
+                                  int64_t workspace_bytes, void* stream);
+
+/* The k best of each row's E scores (E <= 4096, k <= min(E, 64), N k < 2^30), the
+ * lower index first among equals.  Scores of -inf or NaN are no candidates; a choice
+ * that finds none left is expert -1 with gate 0.
+ *   experts (N, k), gates (N, k): softmax over the chosen (renormalize) or over all
+ *     candidates;
+ *   offsets (E + 1): group e holds positions offsets[e] .. offsets[e + 1] - 1, in the
+ *     order of the rows; choices of expert -1 take the positions from offsets[E] on;
+ *   rows (N k): the row at each position;  slots (N, k): the position of each choice;
+ *   norm (N, 2; NULL: not wanted): the largest candidate and 1 / sum, which the
+ *     backward pass of gates over all candidates reads. */
+int64_t gmmxx_hip_route_workspace_bytes(int64_t N, int64_t E, int64_t k);
+int gmmxx_hip_route(int elem, int64_t N, int64_t E, int64_t k, int renormalize, const void* scores, int64_t ld,
+                    int32_t* experts, float* gates, int32_t* offsets, int32_t* rows, int32_t* slots, float* norm,
+                    void* workspace, int64_t workspace_bytes, void* stream);
+
+/* dscores (N, E) from dgates (N, k); norm may be NULL when renormalize is set. */
+int gmmxx_hip_route_backward(int elem, int64_t N, int64_t E, int64_t k, int renormalize, const void* scores,
+                             int64_t ld, const int32_t* experts, const float* gates, const float* norm,
+                             const float* dgates, void* dscores, void* stream);
+
+/* Products grouped by expert: out[p] = x[rows[p]] w[e] + bias[e] for the positions p
+ * of group e, and zeros at positions past offsets[E].  x has Nx rows of K elements;
+ * rows (M; NULL: position p is row p); w's element (e, k, n) lies at
+ * e we + k wk + n wn with wk or wn 1; bias (E, N) or NULL; offsets (E + 1) of 32 or 64
+ * bits (offset_bits), ascending from 0 to at most M; out (M, N), of out_elem (elem or
+ * GMMXX_F32).  E <= 4096, M < 2^30.  Offsets and rows out of range are taken as the
+ * nearest valid ones. */
+int gmmxx_hip_grouped_matmul(int elem, int64_t M, int64_t Nx, int64_t E, int64_t K, int64_t N, const void* x,
+                             int64_t ldx, const int32_t* rows, const void* w, int64_t we, int64_t wk, int64_t wn,
+                             const void* bias, const void* offsets, int offset_bits, void* out, int out_elem,
+                             void* stream);
+
+/* The weight's gradient dw[e] = sum over group e of x[rows[p]]^T dy[p] (E, K, N) and,
+ * unless dbias is NULL, the bias's (E, N); an empty group's are zeros.  The workspace
+ * takes gmmxx_hip_grouped_workspace_bytes. */
+int64_t gmmxx_hip_grouped_workspace_bytes(int64_t M, int64_t E, int64_t K, int64_t N);
+int gmmxx_hip_grouped_weight_grad(int elem, int64_t M, int64_t Nx, int64_t E, int64_t K, int64_t N, const void* x,
+                                  int64_t ldx, const int32_t* rows, const void* dy, int64_t lddy,
+                                  const void* offsets, int offset_bits, void* dw, void* dbias, void* workspace,
+                                  int64_t workspace_bytes, void* stream);
+
+/* out[n] = sum over j of gates[n, j] y[slots[n, j]] for N rows of F elements; y has M =
+ * N k rows of y_elem (elem or GMMXX_F32); gates NULL: ones.  Positions from
+ * offsets[E] on add nothing.  k <= 64, M < 2^30. */
+int gmmxx_hip_combine(int elem, int64_t N, int64_t k, int64_t E, int64_t F, const void* y, int y_elem, int64_t ldy,
+                      const float* gates, const int32_t* slots, const int32_t* offsets, void* out, void* stream);
+
+/* Gradients of gmmxx_hip_combine from dout (N, F): dy (M, F) and dgates (N, k); slots
+ * is a permutation of the M positions. */
+int gmmxx_hip_combine_backward(int elem, int64_t N, int64_t k, int64_t E, int64_t F, const void* y, int64_t ldy,
+                               const float* gates, const int32_t* slots, const int32_t* offsets, const void* dout,
+                               int64_t lddout, void* dy, float* dgates, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
