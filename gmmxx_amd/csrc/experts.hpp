@@ -70,6 +70,11 @@ struct GroupedArgs {
 };
 void launch_grouped(const GroupedArgs& a, hipStream_t s);
 void launch_grouped_dw(const GroupedArgs& a, hipStream_t s);
+// 16-bit elements in whole, aligned 16-byte chunks (grouped_mma.hip).
+bool grouped_mma_rows_ok(const GroupedArgs& a);
+bool grouped_mma_dw_ok(const GroupedArgs& a);
+void launch_grouped_mma(const GroupedArgs& a, hipStream_t s);
+void launch_grouped_mma_dw(const GroupedArgs& a, hipStream_t s);
 
 constexpr int kCombineMaxK = 64;
 struct CombineArgs {

@@ -53,6 +53,7 @@ int check_grouped(int elem, int64_t M, int64_t Nx, int64_t E, int64_t K, int64_t
   if (offset_bits != 32 && offset_bits != 64) return invalid("offset_bits must be 32 or 64");
   if (E > kGroupedMaxE) return unsupported("E > 4096");
   if (M >= kMaxPositions) return unsupported("M >= 2^30");
+  if (Nx > INT32_MAX) return unsupported("Nx >= 2^31");
   if (K > kMaxDim || N > kMaxDim) return unsupported("K or N > 2^22");
   return GMMXX_OK;
 }

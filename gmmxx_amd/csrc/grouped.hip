@@ -10,53 +10,11 @@
 // counting tiles.  Positions past offsets[E] get rows of zeros.  Offsets and row
 // indices are clamped to their arrays, so no values of theirs lead out of bounds.
 
-#include "experts.hpp"
-#include "rows.hpp"
+#include "grouped_core.hpp"
 
 namespace gx::layer {
 
 namespace {
-
-typedef __bf16 bf16_t;
-
-__device__ __forceinline__ int64_t offset_at(const GroupedArgs& a, int e) {
-  const int64_t v = e <= 0 ? 0 : a.off64 ? static_cast<const int64_t*>(a.offsets)[e] : static_cast<const int32_t*>(a.offsets)[e];
-  return v < 0 ? 0 : (v < a.M ? v : a.M);
-}
-
-// Group and first position of row tile t (BM positions each): group E is the rows
-// past the last group.  False: there is no such tile.
-template <int BM>
-__device__ __forceinline__ bool find_tile(const GroupedArgs& a, int64_t t, int& group, int64_t& first, int64_t& end) {
-  const int lane = threadIdx.x & 63;
-  int64_t before = 0;
-  for (int base = 0; base <= a.E; base += 64) {
-    const int e = base + lane;
-    int64_t lo = 0, hi = 0;
-    if (e <= a.E) {
-      lo = offset_at(a, e);
-      hi = e < a.E ? offset_at(a, e + 1) : a.M;
-    }
-    const int64_t tiles = hi > lo ? (hi - lo + BM - 1) / BM : 0;
-    int64_t incl = tiles;
-#pragma unroll
-    for (int off = 1; off < 64; off *= 2) {
-      const int64_t v = __shfl_up(incl, off);
-      if (lane >= off) incl += v;
-    }
-    const uint64_t hit = __ballot(before + incl > t);
-    if (hit) {
-      const int src = __ffsll((unsigned long long)hit) - 1;
-      const int64_t skipped = before + __shfl(incl - tiles, src);
-      group = base + src;
-      first = __shfl(lo, src) + (t - skipped) * BM;
-      end = __shfl(hi, src);
-      return true;
-    }
-    before += __shfl(incl, 63);
-  }
-  return false;
-}
 
 // Products of one 16 x 16 tile: 32-deep for 16-bit elements, 4-deep for fp32.
 template <typename T> struct Mma;
@@ -132,12 +90,7 @@ __global__ __launch_bounds__(kThreads) void grouped_rows_kernel(GroupedArgs a) {
       for (int i = tid; i < Tl::BM * Tl::BK; i += kThreads) {
         const int r = i / Tl::BK, k = i % Tl::BK;
         T v = (T)0.f;
-        if (r < rows && k0 + k < a.K) {
-          int64_t src = first + r;
-          if (a.rows) src = a.rows[src];
-          src = src < 0 ? 0 : (src < a.Nx ? src : a.Nx - 1);
-          v = static_cast<const T*>(a.x)[src * a.ldx + k0 + k];
-        }
+        if (r < rows && k0 + k < a.K) v = static_cast<const T*>(a.x)[source_row(a, first + r) * a.ldx + k0 + k];
         t.a[r][k] = v;
       }
       for (int i = tid; i < Tl::BN * Tl::BK; i += kThreads) {
@@ -181,12 +134,7 @@ __global__ __launch_bounds__(kThreads) void grouped_dw_kernel(GroupedArgs a) {
     for (int i = tid; i < Tl::BM * Tl::BK; i += kThreads) {
       const int m = i % Tl::BM, p = i / Tl::BM;
       T v = (T)0.f;
-      if (p0 + p < hi && k0 + m < a.K) {
-        int64_t src = p0 + p;
-        if (a.rows) src = a.rows[src];
-        src = src < 0 ? 0 : (src < a.Nx ? src : a.Nx - 1);
-        v = static_cast<const T*>(a.x)[src * a.ldx + k0 + m];
-      }
+      if (p0 + p < hi && k0 + m < a.K) v = static_cast<const T*>(a.x)[source_row(a, p0 + p) * a.ldx + k0 + m];
       t.a[m][p] = v;
     }
     for (int i = tid; i < Tl::BN * Tl::BK; i += kThreads) {
@@ -235,13 +183,15 @@ void dw_typed(const GroupedArgs& a, hipStream_t s) {
 }  // namespace
 
 void launch_grouped(const GroupedArgs& a, hipStream_t s) {
-  if (a.elem == ELEM_F32) rows_typed<float>(a, s);
+  if (grouped_mma_rows_ok(a)) launch_grouped_mma(a, s);
+  else if (a.elem == ELEM_F32) rows_typed<float>(a, s);
   else if (a.elem == ELEM_BF16) rows_typed<bf16_t>(a, s);
   else rows_typed<_Float16>(a, s);
 }
 
 void launch_grouped_dw(const GroupedArgs& a, hipStream_t s) {
-  if (a.elem == ELEM_F32) dw_typed<float>(a, s);
+  if (grouped_mma_dw_ok(a)) launch_grouped_mma_dw(a, s);
+  else if (a.elem == ELEM_F32) dw_typed<float>(a, s);
   else if (a.elem == ELEM_BF16) dw_typed<bf16_t>(a, s);
   else dw_typed<_Float16>(a, s);
 }
