@@ -178,7 +178,7 @@ int gmmxx_hip_grouped_matmul(int elem, int64_t M, int64_t Nx, int64_t E, int64_t
 
 int64_t gmmxx_hip_grouped_workspace_bytes(int64_t M, int64_t E, int64_t K, int64_t N) {
   if (check_grouped(GMMXX_F32, M, 1, E, K, N, 32)) return -1;
-  return 0;
+  return grouped_workspace_bytes(M, E, K, N);
 }
 
 int gmmxx_hip_grouped_weight_grad(int elem, int64_t M, int64_t Nx, int64_t E, int64_t K, int64_t N, const void* x,
@@ -193,7 +193,7 @@ int gmmxx_hip_grouped_weight_grad(int elem, int64_t M, int64_t Nx, int64_t E, in
   if (const int64_t need = gmmxx_hip_grouped_workspace_bytes(M, E, K, N))
     if (int rc = check_workspace(workspace, workspace_bytes, need)) return rc;
   GroupedArgs a = grouped_args(elem, M, Nx, E, K, N, x, ldx, rows, offsets, offset_bits);
-  a.dy = dy; a.lddy = lddy; a.out = dw; a.dbias = dbias;
+  a.dy = dy; a.lddy = lddy; a.out = dw; a.dbias = dbias; a.part = static_cast<float*>(workspace);
   launch_grouped_dw(a, (hipStream_t)stream);
   return launch_status("grouped_weight_grad");
 }
