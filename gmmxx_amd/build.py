@@ -22,7 +22,7 @@ LIB_PATH = os.path.join(PKG_DIR, "libgmmxx_hip.so")
 SOURCES = ("em_tile.hip", "em_sph_bf16.hip", "em_fused.hip", "em_coop.hip", "em_one.hip", "em_label.hip", "em_full_wide.hip", "em_full_stats.hip", "em_full_infer.hip",
            "params.hip",
            "kmeans.hip", "abi.hip",
-           "layer_norm.hip", "route.hip", "grouped.hip", "grouped_mma.hip", "grouped_few.hip", "combine.hip", "experts_abi.hip")
+           "layer_norm.hip", "route.hip", "grouped.hip", "grouped_bf16.hip", "grouped_f16.hip", "grouped_f32.hip", "grouped_few.hip", "combine.hip", "experts_abi.hip")
 ARCH = os.environ.get("GMMXX_HIP_ARCH", "gfx950")
 
 # -packed-fp32-ops: keep the compiler from emitting packed fp32 VALU ops.

@@ -73,18 +73,11 @@ struct GroupedArgs {
 void launch_grouped(const GroupedArgs& a, hipStream_t s);
 void launch_grouped_dw(const GroupedArgs& a, hipStream_t s);
 int64_t grouped_workspace_bytes(int64_t M, int64_t E, int64_t K, int64_t N);
-// Parts that an average group's positions are cut into, given the workgroups without parts, the workgroups
-// wanted and the fewest positions of a part.
-int parts_of(int64_t M, int64_t E, int64_t groups, int64_t want, int64_t least);
-int grouped_mma_dw_splits(int64_t M, int64_t E, int64_t K, int64_t N);
-// 16-bit elements in whole, aligned 16-byte chunks (grouped_mma.hip).
-bool grouped_mma_rows_ok(const GroupedArgs& a);
-bool grouped_mma_dw_ok(const GroupedArgs& a);
+// Whole, aligned 16-byte chunks, which the tiles load straight into LDS.
+bool grouped_direct(const GroupedArgs& a);
 // Few rows for each expert (grouped_few.hip).
 bool grouped_few_better(const GroupedArgs& a);
 void launch_grouped_few(const GroupedArgs& a, hipStream_t s);
-void launch_grouped_mma(const GroupedArgs& a, hipStream_t s);
-void launch_grouped_mma_dw(const GroupedArgs& a, int splits, hipStream_t s);
 
 constexpr int kCombineMaxK = 64;
 struct CombineArgs {

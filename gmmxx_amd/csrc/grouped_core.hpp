@@ -8,6 +8,10 @@ namespace gx::layer {
 
 typedef __bf16 bf16_t;
 
+// The tiles (grouped_tiles.hpp): by direct loads or not, 256 wide (16-bit elements, direct) or 128.
+template <typename T> void launch_rows_tiles(const GroupedArgs& a, bool direct, bool larger, hipStream_t s);
+template <typename T> void launch_dw_tiles(const GroupedArgs& a, bool direct, bool larger, int splits, hipStream_t s);
+
 // offsets[e], within the positions (M < 2^30).
 __device__ __forceinline__ int offset_at(const GroupedArgs& a, int e) {
   if (e <= 0) return 0;

@@ -4,7 +4,11 @@
 // of eight waves takes up to four rows of one group and 8 vectors of columns, and reads its weights once from
 // memory, 16 bytes a lane, straight to registers; the products are fp32 multiply-adds.  Larger groups take
 // several workgroups, which find the weights in cache.  The reduction is cut over the lanes and waves of the
-// workgroup and joined in a fixed order.  Any width, stride and type.
+// workgroup and joined in a fixed order.  Any width, stride and type.  Bound by the weights' bytes and by the
+// chain of waits before them (offsets, then weights and rows together, then the join): 8 rows of 8 experts,
+// 1024 -> 2048 bf16, 34 MB from memory in 14.4 us.
+
+#include <type_traits>
 
 #include "grouped_core.hpp"
 
@@ -16,92 +20,123 @@ constexpr int kThreads = 512, kWaves = kThreads / 64;
 constexpr int kRows = 4;         // of a workgroup
 constexpr int kChunk = 1024;     // reduction elements of x staged at a time
 
-// x's rows as xs[k][row], zeros past K.
+// x's rows as xs[k][row], zeros past K (up to a multiple of 128).
 template <typename T>
 __device__ __forceinline__ void stage(const GroupedArgs& a, int first, int rows, int k0, float4* xs) {
   const int r = threadIdx.x & 3, lane = threadIdx.x >> 2;
-  const T* x = static_cast<const T*>(a.x) + source_row(a, first + (r < rows ? r : 0)) * a.ldx;
+  const T* x = static_cast<const T*>(a.x) + source_row(a, first + (r < rows ? r : 0)) * a.ldx + k0;
   const int most = min(kChunk, a.K - k0);
-  for (int k = lane; k < kChunk; k += kThreads / 4)
-    reinterpret_cast<float*>(xs)[k * 4 + r] = r < rows && k < most ? to_f32(x[k0 + k]) : 0.f;
+#pragma unroll
+  for (int i = 0; i < kChunk / (kThreads / 4); ++i) {
+    if (i * (kThreads / 4) >= most) break;
+    const int k = lane + i * (kThreads / 4);
+    reinterpret_cast<float*>(xs)[k * 4 + r] = r < rows && k < most ? to_f32(x[k]) : 0.f;
+  }
+}
+
+template <typename T>
+__device__ __forceinline__ float element(const uint4& v, int i) {
+  union { uint4 u; T t[kVec<T>]; } r;
+  r.u = v;
+  return to_f32(r.t[i]);
+}
+
+__device__ __forceinline__ void add_products(float (&acc)[kRows], const float4& x, float w) {
+  acc[0] = fmaf(x.x, w, acc[0]);
+  acc[1] = fmaf(x.y, w, acc[1]);
+  acc[2] = fmaf(x.z, w, acc[2]);
+  acc[3] = fmaf(x.w, w, acc[3]);
+}
+
+// Whole chunks without conditions (their loads are all in flight before the first is used), then the rest.
+template <typename F>
+__device__ __forceinline__ void over_chunks(int K, F&& chunk) {
+  int k0 = 0;
+  for (; k0 + kChunk <= K; k0 += kChunk) chunk(k0, std::true_type());
+  if (k0 < K) chunk(k0, std::false_type());
 }
 
 template <typename T, bool KC>
 __global__ __launch_bounds__(kThreads) void grouped_few_kernel(GroupedArgs a, int ntiles) {
-  constexpr int V = kVec<T>;
-  constexpr int Cols = KC ? 64 : 8 * V;        // columns of a workgroup
+  constexpr int V = kVec<T>, Cols = 8 * V;     // columns of a workgroup
+  constexpr int Loads = 16;                    // 16-byte loads of a thread for a chunk, all in flight at once
   __shared__ __align__(16) float4 xs[kChunk];
   __shared__ float part[kWaves][kRows][Cols];
   int group, first, end, ntile;
   if (!find_tile<kRows>(a, blockIdx.x, ntiles, group, first, end, ntile)) return;
   const int rows = min(end - first, kRows), n0 = ntile * Cols;
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   if (group < a.E) {
     const T* w = static_cast<const T*>(a.w) + (int64_t)group * a.we;
+    const int c = lane & 7;
+    uint4 v[Loads];
     if constexpr (KC) {
-      // 8 lanes share a column; a wave takes every 8th stretch of 8 V reduction elements.
+      // 8 lanes share a column and V columns a thread; a wave takes every 8th stretch of 8 V reduction elements.
       constexpr int Span = 8 * V, Parts = kChunk / (Span * kWaves);
-      const int c = lane & 7;
-      for (int i = tid; i < kWaves * kRows * Cols; i += kThreads) (&part[0][0][0])[i] = 0.f;
-      for (int k0 = 0; k0 < a.K; k0 += kChunk) {
+      static_assert(V * Parts == Loads, "");
+      float acc[V][kRows] = {};
+      auto chunk = [&](int k0, auto whole) {
+#pragma unroll
+        for (int q = 0; q < Parts; ++q)
+#pragma unroll
+          for (int b = 0; b < V; ++b) {
+            if (!whole && k0 + (q * kWaves + wave) * Span >= a.K) continue;
+            const int n = n0 + 8 * b + (lane >> 3), k = k0 + (q * kWaves + wave) * Span + c * V;
+            v[q * V + b] = load16(w + (int64_t)n * a.wn + k, n < a.Nn ? (whole ? V : a.K - k) : 0);
+          }
         __syncthreads();
         stage<T>(a, first, rows, k0, xs);
         __syncthreads();
-        for (int b = 0; b < Cols; b += 8) {
-          const int n = n0 + b + (lane >> 3);
-          float acc[kRows] = {};
 #pragma unroll
-          for (int q = 0; q < Parts; ++q) {
-            const int k = (q * kWaves + wave) * Span + c * V;
-            float v[V];
-            load_row(w + (int64_t)n * a.wn + k0 + k, n < a.Nn ? a.K - k0 - k : 0, v);
-#pragma unroll
-            for (int i = 0; i < V; ++i) {
-              const float4 xv = xs[k + i];
-              acc[0] = fmaf(xv.x, v[i], acc[0]);
-              acc[1] = fmaf(xv.y, v[i], acc[1]);
-              acc[2] = fmaf(xv.z, v[i], acc[2]);
-              acc[3] = fmaf(xv.w, v[i], acc[3]);
-            }
-          }
-#pragma unroll
-          for (int r = 0; r < kRows; ++r) {
-            acc[r] = lanes_sum<8>(acc[r]);
-            if (c == 0) part[wave][r][b + (lane >> 3)] += acc[r];
-          }
-        }
-      }
-    } else {
-      // 8 lanes share a reduction row; 64 rows at a time.
-      const int c = lane & 7, kr = tid >> 3, n = n0 + c * V;
-      float acc[kRows][V] = {};
-      for (int k0 = 0; k0 < a.K; k0 += kChunk) {
-        __syncthreads();
-        stage<T>(a, first, rows, k0, xs);
-        __syncthreads();
-        const int most = min(kChunk, a.K - k0);
-#pragma unroll 8
-        for (int k = kr; k < most; k += kThreads / 8) {
-          float v[V];
-          load_row(w + (int64_t)(k0 + k) * a.wk + n, a.Nn - n, v);
-          const float4 xv = xs[k];
+        for (int q = 0; q < Parts; ++q)
 #pragma unroll
           for (int i = 0; i < V; ++i) {
-            acc[0][i] = fmaf(xv.x, v[i], acc[0][i]);
-            acc[1][i] = fmaf(xv.y, v[i], acc[1][i]);
-            acc[2][i] = fmaf(xv.z, v[i], acc[2][i]);
-            acc[3][i] = fmaf(xv.w, v[i], acc[3][i]);
+            if (!whole && k0 + (q * kWaves + wave) * Span >= a.K) continue;
+            const float4 x = xs[(q * kWaves + wave) * Span + c * V + i];
+#pragma unroll
+            for (int b = 0; b < V; ++b) add_products(acc[b], x, element<T>(v[q * V + b], i));
           }
+      };
+      over_chunks(a.K, chunk);
+#pragma unroll
+      for (int b = 0; b < V; ++b)
+#pragma unroll
+        for (int r = 0; r < kRows; ++r) {
+          const float s = lanes_sum<8>(acc[b][r]);
+          if (c == 0) part[wave][r][8 * b + (lane >> 3)] = s;
         }
-      }
+    } else {
+      // 8 lanes share a reduction row; 64 rows at a time.
+      static_assert(Loads * kThreads / 8 == kChunk, "");
+      const int kr = tid >> 3, n = n0 + c * V;
+      float acc[V][kRows] = {};
+      auto chunk = [&](int k0, auto whole) {
+#pragma unroll
+        for (int u = 0; u < Loads; ++u) {
+          if (!whole && k0 + u * (kThreads / 8) >= a.K) continue;
+          const int k = k0 + kr + u * (kThreads / 8);
+          v[u] = load16(w + (int64_t)k * a.wk + n, whole || k < a.K ? a.Nn - n : 0);
+        }
+        __syncthreads();
+        stage<T>(a, first, rows, k0, xs);
+        __syncthreads();
+#pragma unroll
+        for (int u = 0; u < Loads; ++u) {
+          if (!whole && k0 + u * (kThreads / 8) >= a.K) continue;
+          const float4 x = xs[kr + u * (kThreads / 8)];
+#pragma unroll
+          for (int i = 0; i < V; ++i) add_products(acc[i], x, element<T>(v[u], i));
+        }
+      };
+      over_chunks(a.K, chunk);
 #pragma unroll
       for (int r = 0; r < kRows; ++r)
 #pragma unroll
         for (int i = 0; i < V; ++i) {
-          float s = acc[r][i];
-          s += __shfl_xor(s, 8);
-          s += __shfl_xor(s, 16);
-          s += __shfl_xor(s, 32);
+          // the wave's 8 reduction rows: lanes 8, 16 and 32 apart
+          const auto plus = [](float p, float q) { return p + q; };
+          float s = acc[i][r] + __shfl_xor(acc[i][r], 8);
+          s = with_other<32>(with_other<16>(s, plus), plus);
           if (lane < 8) part[wave][r][lane * V + i] = s;
         }
     }
@@ -124,7 +159,7 @@ __global__ __launch_bounds__(kThreads) void grouped_few_kernel(GroupedArgs a, in
 
 template <typename T, bool KC>
 void few_typed(const GroupedArgs& a, hipStream_t s) {
-  const int cols = KC ? 64 : 8 * kVec<T>, ntiles = (a.Nn + cols - 1) / cols;
+  const int cols = 8 * kVec<T>, ntiles = (a.Nn + cols - 1) / cols;
   // (groups with rows, and the rows past the last group: no more than there are positions)
   const int64_t tiles = a.M / kRows + (a.M < a.E + 1 ? a.M : a.E + 1);
   grouped_few_kernel<T, KC><<<(unsigned)(tiles * ntiles), kThreads, 0, s>>>(a, ntiles);
@@ -137,11 +172,13 @@ void few(const GroupedArgs& a, hipStream_t s) {
 
 }  // namespace
 
-// Up to which number of positions this beats the tiles: of 1024 x 2048 matrices, 8 positions of 16 experts
-// 11.9 and 12.6 us, 16 positions 30.6 and 15.5 us by tiles of whole chunks; the element-wise tiles are slower
-// by far (fp32, 64 experts, 128 positions: 230 and 292 us).
+// Up to which number of positions this beats the tiles.  Whole 16-bit chunks: 8 (1024 x 2048 matrices, 16
+// experts: 9.8 and 12.7 us at 8 positions, 28 and 16 us at 32).  Other 16-bit shapes: two an expert (100 x 77:
+// 7.2 and 10.5 us at 32).  fp32, whose tiles take sixteen times as long: two an expert or 32 (1024 x 2048, 16
+// experts: 39 and 71 us at 32 positions, 98 and 71 us at 128; 64 experts: 173 and 255 us at 128).
 bool grouped_few_better(const GroupedArgs& a) {
-  return a.M <= 8 || (!grouped_mma_rows_ok(a) && a.M <= 2 * (int64_t)a.E);
+  if (a.elem == ELEM_F32) return a.M <= (a.E > 16 ? 2 * a.E : 32);
+  return a.M <= 8 || (!grouped_direct(a) && a.M <= 2 * (int64_t)a.E);
 }
 
 void launch_grouped_few(const GroupedArgs& a, hipStream_t s) {

@@ -32,6 +32,30 @@ __device__ __forceinline__ void load_row(const T* p, int valid, float (&v)[kVec<
   }
 }
 
+// The same as raw bytes; elements at or past `valid` are zeros.
+template <typename T>
+__device__ __forceinline__ uint4 load16(const T* p, int valid) {
+  constexpr int V = kVec<T>;
+  union { uint4 u; T t[V]; } r;
+  if (valid >= V) return ld16_any(p);
+#pragma unroll
+  for (int i = 0; i < V; ++i) r.t[i] = i < valid ? p[i] : (T)0.f;
+  return r.u;
+}
+template <typename T>
+__device__ __forceinline__ void store16(T* p, int valid, uint4 v) {
+  constexpr int V = kVec<T>;
+  union { uint4 u; u32x4_any w; T t[V]; } r;
+  r.u = v;
+  if (valid >= V) {
+    *reinterpret_cast<u32x4_any*>(p) = r.w;
+  } else {
+#pragma unroll
+    for (int i = 0; i < V; ++i)
+      if (i < valid) p[i] = r.t[i];
+  }
+}
+
 // The reverse of load_row: rounds to T (nearest even) and stores the first `valid`.
 template <typename T>
 __device__ __forceinline__ void store_row(T* p, int valid, const float (&v)[kVec<T>]) {
@@ -48,13 +72,38 @@ __device__ __forceinline__ void store_row(T* p, int valid, const float (&v)[kVec
   }
 }
 
-// Sum over aligned groups of G consecutive lanes (G a power of two up to 64), the
-// same value and the same order of additions in every lane.
+// op(v, the value at distance D) within aligned groups of 2 D lanes whose halves each hold one value: the other
+// half's value in every lane.  D up to 8 in one instruction with the operation (mirrored lanes), 16 and 32 by
+// exchanging rows.
+template <int D, typename F>
+__device__ __forceinline__ float with_other(float v, F&& op) {
+  if constexpr (D <= 8) {
+    constexpr int kCtrl = D == 1 ? 0xB1 : D == 2 ? 0x4E : D == 4 ? 0x141 : 0x140;   // quad_perm, half mirror, mirror
+    const int o = __builtin_amdgcn_update_dpp(0, __float_as_int(v), kCtrl, 0xF, 0xF, false);
+    return op(v, __int_as_float(o));
+  } else {
+    const unsigned u = __float_as_uint(v);
+    const auto r = D == 16 ? __builtin_amdgcn_permlane16_swap(u, u, false, false)
+                           : __builtin_amdgcn_permlane32_swap(u, u, false, false);
+    return op(__uint_as_float(r[0]), __uint_as_float(r[1]));
+  }
+}
+
+// op over aligned groups of G consecutive lanes (G a power of two up to 64): the same value, by the same order
+// of operations, in every lane of the group.  All 64 lanes take part.
+template <int G, typename F>
+__device__ __forceinline__ float lanes_reduce(float v, F&& op) {
+  if constexpr (G > 1) v = with_other<1>(v, op);
+  if constexpr (G > 2) v = with_other<2>(v, op);
+  if constexpr (G > 4) v = with_other<4>(v, op);
+  if constexpr (G > 8) v = with_other<8>(v, op);
+  if constexpr (G > 16) v = with_other<16>(v, op);
+  if constexpr (G > 32) v = with_other<32>(v, op);
+  return v;
+}
 template <int G>
 __device__ __forceinline__ float lanes_sum(float v) {
-#pragma unroll
-  for (int off = G / 2; off >= 1; off /= 2) v += __shfl_xor(v, off);
-  return v;
+  return lanes_reduce<G>(v, [](float a, float b) { return a + b; });
 }
 
 // Sum over groups of G threads: lanes_sum within a wave, `red` (two slots of 16
