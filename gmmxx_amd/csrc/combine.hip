@@ -33,7 +33,7 @@ __device__ __forceinline__ int taken_total(const CombineArgs& a) {
 }
 
 // tx threads (a power of two) share a row's vectors.
-template <typename Y, typename T>
+template <typename Y, typename T, bool SHORT>
 __global__ __launch_bounds__(kThreads) void combine_kernel(CombineArgs a, int tx) {
   constexpr int V = kVec<T>;
   const int lane = threadIdx.x & (tx - 1), rpb = kThreads / tx;
@@ -46,30 +46,33 @@ __global__ __launch_bounds__(kThreads) void combine_kernel(CombineArgs a, int tx
 #pragma unroll
       for (int i = 0; i < V; ++i) acc[i] = 0.f;
       for (int j0 = 0; j0 < a.k; j0 += 4) {
-        float v[4][V], g[4];
+        constexpr int H = (int)(sizeof(Y) / sizeof(T));      // vectors of y for one of out
+        uint4 u[4][H];
+        float g[4];
+        bool there[4];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           const int slot = j0 + j < a.k ? taken(a.slots[n * a.k + j0 + j], total) : -1;
-          g[j] = slot >= 0 && a.gates ? a.gates[n * a.k + j0 + j] : 1.f;
-          const Y* p = y + (int64_t)(slot >= 0 ? slot : 0) * a.ldy + c;
-          const int valid = slot >= 0 ? a.F - c : 0;
-          if constexpr (sizeof(Y) == sizeof(T)) {
-            load_row(p, valid, v[j]);
-          } else {   // fp32 rows of a 16-bit result: two vectors
-            float lo[kVec<Y>], hi[kVec<Y>];
-            load_row(p, valid, lo);
-            load_row(p + kVec<Y>, valid - kVec<Y>, hi);
+          there[j] = slot >= 0;
+          g[j] = there[j] && a.gates ? a.gates[n * a.k + j0 + j] : 1.f;
+          const Y* p = y + (int64_t)(there[j] ? slot : 0) * a.ldy + c;
+          if (j0 + j < a.k) {
 #pragma unroll
-            for (int i = 0; i < kVec<Y>; ++i) {
-              v[j][i] = lo[i];
-              v[j][kVec<Y> + i] = hi[i];
-            }
+            for (int h = 0; h < H; ++h) u[j][h] = fetch16<SHORT>(p + h * kVec<Y>, a.F - c - h * kVec<Y>);
           }
         }
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
+        for (int j = 0; j < 4; ++j) {
+          if (j0 + j >= a.k) break;
 #pragma unroll
-          for (int i = 0; i < V; ++i) acc[i] = fmaf(g[j], v[j][i], acc[i]);
+          for (int h = 0; h < H; ++h) {
+            float v[kVec<Y>];
+            unpack16<Y>(keep16<SHORT, Y>(u[j][h], there[j] ? a.F - c - h * kVec<Y> : 0, a.F), v);
+#pragma unroll
+            for (int i = 0; i < kVec<Y>; ++i)
+              acc[h * kVec<Y> + i] = fmaf(g[j], there[j] ? v[i] : 0.f, acc[h * kVec<Y> + i]);
+          }
+        }
       }
       store_row(out + c, a.F - c, acc);
     }
@@ -77,7 +80,7 @@ __global__ __launch_bounds__(kThreads) void combine_kernel(CombineArgs a, int tx
 }
 
 // G lanes of a wave share a row; KC choices at a time (dout is read again for every KC).
-template <typename T, int G, int KC>
+template <typename T, int G, int KC, bool SHORT>
 __global__ __launch_bounds__(kThreads) void combine_bwd_kernel(CombineArgs a) {
   constexpr int V = kVec<T>;
   const int lane = threadIdx.x % G;
@@ -100,17 +103,18 @@ __global__ __launch_bounds__(kThreads) void combine_bwd_kernel(CombineArgs a) {
         dot[j] = 0.f;
       }
       for (int c = lane * V; c < a.F; c += G * V) {
-        float d[V], v[KC][V];
-        load_row(dout + c, a.F - c, d);
+        uint4 ud = fetch16<SHORT>(dout + c, a.F - c), u[KC];
 #pragma unroll
-        for (int j = 0; j < KC; ++j)
-          load_row(y + (int64_t)(slot[j] >= 0 ? slot[j] : 0) * a.ldy + c, slot[j] >= 0 ? a.F - c : 0, v[j]);
+        for (int j = 0; j < KC; ++j) u[j] = fetch16<SHORT>(y + (int64_t)(slot[j] >= 0 ? slot[j] : 0) * a.ldy + c, a.F - c);
+        float d[V];
+        unpack16<T>(keep16<SHORT, T>(ud, a.F - c, a.F), d);
 #pragma unroll
         for (int j = 0; j < KC; ++j) {
-          float o[V];
+          float o[V], v[V];
+          unpack16<T>(keep16<SHORT, T>(u[j], a.F - c, a.F), v);
 #pragma unroll
           for (int i = 0; i < V; ++i) {
-            dot[j] = fmaf(d[i], v[j][i], dot[j]);
+            dot[j] = fmaf(d[i], v[i], dot[j]);
             o[i] = slot[j] >= 0 ? g[j] * d[i] : 0.f;
           }
           store_row(dy + (int64_t)(pos[j] >= 0 ? pos[j] : 0) * a.F + c, pos[j] >= 0 ? a.F - c : 0, o);
@@ -130,23 +134,26 @@ void combine_typed(const CombineArgs& a, hipStream_t s) {
   const int nvec = (a.F + kVec<T> - 1) / kVec<T>;
   int tx = 1;
   while (tx < nvec && tx < kThreads) tx *= 2;
-  combine_kernel<Y, T><<<grid_of(a.N, kThreads / tx), kThreads, 0, s>>>(a, tx);
+  // (vectors of fp32 y are the shorter)
+  if (a.F < kVec<T>) combine_kernel<Y, T, true><<<grid_of(a.N, kThreads / tx), kThreads, 0, s>>>(a, tx);
+  else combine_kernel<Y, T, false><<<grid_of(a.N, kThreads / tx), kThreads, 0, s>>>(a, tx);
 }
 
-template <typename T, int G>
+template <typename T, int G, bool SHORT>
 void combine_bwd_group(const CombineArgs& a, hipStream_t s) {
   const unsigned grid = grid_of(a.N, kThreads / G);
-  if (a.k <= 1) combine_bwd_kernel<T, G, 1><<<grid, kThreads, 0, s>>>(a);
-  else if (a.k <= 2) combine_bwd_kernel<T, G, 2><<<grid, kThreads, 0, s>>>(a);
-  else combine_bwd_kernel<T, G, 4><<<grid, kThreads, 0, s>>>(a);
+  if (a.k <= 1) combine_bwd_kernel<T, G, 1, SHORT><<<grid, kThreads, 0, s>>>(a);
+  else if (a.k <= 2) combine_bwd_kernel<T, G, 2, SHORT><<<grid, kThreads, 0, s>>>(a);
+  else combine_bwd_kernel<T, G, 4, SHORT><<<grid, kThreads, 0, s>>>(a);
 }
 
 template <typename T>
 void combine_bwd_typed(const CombineArgs& a, hipStream_t s) {
   const int nvec = (a.F + kVec<T> - 1) / kVec<T>;
-  if (nvec <= 8) combine_bwd_group<T, 8>(a, s);
-  else if (nvec <= 32) combine_bwd_group<T, 32>(a, s);
-  else combine_bwd_group<T, 64>(a, s);
+  if (a.F < kVec<T>) combine_bwd_group<T, 8, true>(a, s);
+  else if (nvec <= 8) combine_bwd_group<T, 8, false>(a, s);
+  else if (nvec <= 32) combine_bwd_group<T, 32, false>(a, s);
+  else combine_bwd_group<T, 64, false>(a, s);
 }
 
 }  // namespace

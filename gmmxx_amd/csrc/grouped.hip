@@ -23,7 +23,7 @@ constexpr int kThreads = 256;
 
 // db[e][n] = Σ_p dy[p][n]: 16 threads of one vector of columns by 16 row lanes a workgroup.
 constexpr int kBiasLanes = 16;
-template <typename T, bool SPLIT>
+template <typename T, bool SPLIT, bool SHORT>
 __global__ __launch_bounds__(kThreads) void grouped_bias_kernel(GroupedArgs a) {
   constexpr int V = kVec<T>, Cols = 16 * V;
   __shared__ float part[kBiasLanes][Cols + 4];
@@ -32,12 +32,19 @@ __global__ __launch_bounds__(kThreads) void grouped_bias_kernel(GroupedArgs a) {
   if constexpr (SPLIT) split_part(lo, hi, blockIdx.z, gridDim.z);
   float s[V] = {};
   const T* dy = static_cast<const T*>(a.dy) + n;
-#pragma unroll 4
-  for (int p = lo + r0; p < hi; p += kBiasLanes) {
-    float v[V];
-    load_row(dy + p * a.lddy, a.Nn - n, v);
+  constexpr int B = 8;      // rows in flight
+  for (int p = lo + r0; p < hi; p += B * kBiasLanes) {
+    uint4 u[B];
 #pragma unroll
-    for (int i = 0; i < V; ++i) s[i] += v[i];
+    for (int b = 0; b < B; ++b) u[b] = fetch16<SHORT>(dy + min(p + b * kBiasLanes, hi - 1) * a.lddy, a.Nn - n);
+#pragma unroll
+    for (int b = 0; b < B; ++b) {
+      float v[V];
+      unpack16<T>(keep16<SHORT, T>(u[b], a.Nn - n, a.Nn), v);
+      const bool in = p + b * kBiasLanes < hi;
+#pragma unroll
+      for (int i = 0; i < V; ++i) s[i] += in ? v[i] : 0.f;
+    }
   }
 #pragma unroll
   for (int i = 0; i < V; ++i) part[r0][c * V + i] = s[i];
@@ -108,8 +115,11 @@ template <typename T>
 void dw_rest(const GroupedArgs& a, int splits, int bias_splits, hipStream_t s) {
   if (a.dbias) {
     const dim3 grid((unsigned)((a.Nn + 16 * kVec<T> - 1) / (16 * kVec<T>)), (unsigned)a.E, (unsigned)bias_splits);
-    if (bias_splits == 1) grouped_bias_kernel<T, false><<<grid, kThreads, 0, s>>>(a);
-    else grouped_bias_kernel<T, true><<<grid, kThreads, 0, s>>>(a);
+    const bool whole = a.Nn >= kVec<T>;
+    if (bias_splits == 1 && whole) grouped_bias_kernel<T, false, false><<<grid, kThreads, 0, s>>>(a);
+    else if (bias_splits == 1) grouped_bias_kernel<T, false, true><<<grid, kThreads, 0, s>>>(a);
+    else if (whole) grouped_bias_kernel<T, true, false><<<grid, kThreads, 0, s>>>(a);
+    else grouped_bias_kernel<T, true, true><<<grid, kThreads, 0, s>>>(a);
   }
   const int64_t all = (splits > 1 ? (int64_t)a.E * a.K * a.Nn : 0) + (bias_splits > 1 ? (int64_t)a.E * a.Nn : 0);
   const int64_t blocks = (all + kThreads - 1) / kThreads;

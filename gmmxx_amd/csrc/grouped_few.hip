@@ -56,7 +56,7 @@ __device__ __forceinline__ void over_chunks(int K, F&& chunk) {
   if (k0 < K) chunk(k0, std::false_type());
 }
 
-template <typename T, bool KC>
+template <typename T, bool KC, bool SHORT>
 __global__ __launch_bounds__(kThreads) void grouped_few_kernel(GroupedArgs a, int ntiles) {
   constexpr int V = kVec<T>, Cols = 8 * V;     // columns of a workgroup
   constexpr int Loads = 16;                    // 16-byte loads of a thread for a chunk, all in flight at once
@@ -81,12 +81,19 @@ __global__ __launch_bounds__(kThreads) void grouped_few_kernel(GroupedArgs a, in
 #pragma unroll
           for (int b = 0; b < V; ++b) {
             if (!whole && k0 + (q * kWaves + wave) * Span >= a.K) continue;
-            const int n = n0 + 8 * b + (lane >> 3), k = k0 + (q * kWaves + wave) * Span + c * V;
-            v[q * V + b] = load16(w + (int64_t)n * a.wn + k, n < a.Nn ? (whole ? V : a.K - k) : 0);
+            const int n = min(n0 + 8 * b + (lane >> 3), a.Nn - 1), k = k0 + (q * kWaves + wave) * Span + c * V;
+            v[q * V + b] = fetch16<SHORT>(w + n * a.wn + k, whole ? V : a.K - k);
           }
         __syncthreads();
         stage<T>(a, first, rows, k0, xs);
         __syncthreads();
+        if (!whole) {
+#pragma unroll
+          for (int q = 0; q < Parts; ++q)
+#pragma unroll
+            for (int b = 0; b < V; ++b)
+              v[q * V + b] = keep16<SHORT, T>(v[q * V + b], a.K - (k0 + (q * kWaves + wave) * Span + c * V), a.K);
+        }
 #pragma unroll
         for (int q = 0; q < Parts; ++q)
 #pragma unroll
@@ -115,7 +122,7 @@ __global__ __launch_bounds__(kThreads) void grouped_few_kernel(GroupedArgs a, in
         for (int u = 0; u < Loads; ++u) {
           if (!whole && k0 + u * (kThreads / 8) >= a.K) continue;
           const int k = k0 + kr + u * (kThreads / 8);
-          v[u] = load16(w + (int64_t)k * a.wk + n, whole || k < a.K ? a.Nn - n : 0);
+          v[u] = fetch16<SHORT>(w + (whole ? k : min(k, a.K - 1)) * a.wk + n, a.Nn - n);
         }
         __syncthreads();
         stage<T>(a, first, rows, k0, xs);
@@ -124,6 +131,7 @@ __global__ __launch_bounds__(kThreads) void grouped_few_kernel(GroupedArgs a, in
         for (int u = 0; u < Loads; ++u) {
           if (!whole && k0 + u * (kThreads / 8) >= a.K) continue;
           const float4 x = xs[kr + u * (kThreads / 8)];
+          v[u] = keep16<SHORT, T>(v[u], whole || k0 + kr + u * (kThreads / 8) < a.K ? a.Nn - n : 0, a.Nn);
 #pragma unroll
           for (int i = 0; i < V; ++i) add_products(acc[i], x, element<T>(v[u], i));
         }
@@ -162,7 +170,8 @@ void few_typed(const GroupedArgs& a, hipStream_t s) {
   const int cols = 8 * kVec<T>, ntiles = (a.Nn + cols - 1) / cols;
   // (groups with rows, and the rows past the last group: no more than there are positions)
   const int64_t tiles = a.M / kRows + (a.M < a.E + 1 ? a.M : a.E + 1);
-  grouped_few_kernel<T, KC><<<(unsigned)(tiles * ntiles), kThreads, 0, s>>>(a, ntiles);
+  if ((KC ? a.K : a.Nn) < kVec<T>) grouped_few_kernel<T, KC, true><<<(unsigned)(tiles * ntiles), kThreads, 0, s>>>(a, ntiles);
+  else grouped_few_kernel<T, KC, false><<<(unsigned)(tiles * ntiles), kThreads, 0, s>>>(a, ntiles);
 }
 
 template <typename T>

@@ -54,7 +54,7 @@ __device__ __forceinline__ f32x16 multiply_add(float, i32x4 a, i32x4 b, f32x16 c
 // 16 bytes a lane from base + off to the wave's 1024 bytes of LDS at `dst`, in lane order.  With a
 // 32-bit off and one base for the wave the address takes no vector arithmetic.
 template <typename O>
-__device__ __forceinline__ void fetch16(const uint8_t* base, O off, uint8_t* dst) {
+__device__ __forceinline__ void fetch_direct(const uint8_t* base, O off, uint8_t* dst) {
   __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) uint32_t*)(base + off),
                                    (__attribute__((address_space(3))) uint32_t*)dst, 16, 0, 0);
 }
@@ -294,7 +294,7 @@ __device__ __forceinline__ void store_zeros(O* out, int64_t ld, int rows, int co
 
 // out = x W + b: P is the weight (columns), Q the rows of x.  WIDE: rows of x lie 2^32 bytes or more
 // from its first.
-template <typename T, bool WKC, bool DIRECT, bool WIDE, int BP, int BQ, int WP, int WQ>
+template <typename T, bool WKC, bool DIRECT, bool WIDE, int BP, int BQ, int WP, int WQ, bool SHORT>
 __global__ __launch_bounds__(64 * WP * WQ) void grouped_rows_kernel(GroupedArgs a, int ntiles) {
   typedef Core<T, WKC, true, BP, BQ, WP, WQ> C;
   typedef typename C::P P;
@@ -359,16 +359,16 @@ __global__ __launch_bounds__(64 * WP * WQ) void grouped_rows_kernel(GroupedArgs 
       if constexpr (WKC) {
         const uint32_t k = (uint32_t)min(k0 + pc, K - V) * S;
 #pragma unroll
-        for (int i = 0; i < P::Loads; ++i) fetch16(wb, poff[i] + k, dp + i * (C::Threads * 16));
+        for (int i = 0; i < P::Loads; ++i) fetch_direct(wb, poff[i] + k, dp + i * (C::Threads * 16));
       } else {
         const uint8_t* ws = wb + k0 * ld;
 #pragma unroll
         for (int i = 0; i < P::Loads; ++i)
-          fetch16(ws, __umul24(min(P::row(i), K - 1 - k0), (uint32_t)ld) + poff[0], dp + i * (C::Threads * 16));
+          fetch_direct(ws, __umul24(min(P::row(i), K - 1 - k0), (uint32_t)ld) + poff[0], dp + i * (C::Threads * 16));
       }
       const uint32_t k = (uint32_t)min(k0 + qc, K - V) * S;
 #pragma unroll
-      for (int i = 0; i < Q::Loads; ++i) fetch16(xb, (qoff_t)(qoff[i] + k), dq + i * (C::Threads * 16));
+      for (int i = 0; i < Q::Loads; ++i) fetch_direct(xb, (qoff_t)(qoff[i] + k), dq + i * (C::Threads * 16));
     };
     C::run(K, fill, wave, lane, acc, store);
   } else {
@@ -386,18 +386,21 @@ __global__ __launch_bounds__(64 * WP * WQ) void grouped_rows_kernel(GroupedArgs 
       const int k0 = s * BK;
 #pragma unroll
       for (int i = 0; i < P::Loads; ++i) {
-        if constexpr (WKC) vp[i] = load16(pat[i] + k0, K - k0 - pc);
-        else vp[i] = load16(pat[0] + min(k0 + P::row(i), K - 1) * a.wk, a.Nn - n0 - pc);
+        if constexpr (WKC) vp[i] = fetch16<SHORT>(pat[i] + k0, K - k0 - pc);
+        else vp[i] = fetch16<SHORT>(pat[0] + min(k0 + P::row(i), K - 1) * a.wk, a.Nn - n0 - pc);
       }
 #pragma unroll
-      for (int i = 0; i < Q::Loads; ++i) vq[i] = load16(qat[i] + k0, K - k0 - qc);
+      for (int i = 0; i < Q::Loads; ++i) vq[i] = fetch16<SHORT>(qat[i] + k0, K - k0 - qc);
     };
     load(0);
     auto fill = [&](int s, uint8_t* dp, uint8_t* dq) {
 #pragma unroll
-      for (int i = 0; i < P::Loads; ++i) reinterpret_cast<uint4*>(dp)[i * C::Threads + threadIdx.x] = vp[i];
+      for (int i = 0; i < P::Loads; ++i)
+        reinterpret_cast<uint4*>(dp)[i * C::Threads + threadIdx.x] =
+            keep16<SHORT, T>(vp[i], WKC ? K - s * BK - pc : a.Nn - n0 - pc, WKC ? K : a.Nn);
 #pragma unroll
-      for (int i = 0; i < Q::Loads; ++i) reinterpret_cast<uint4*>(dq)[i * C::Threads + threadIdx.x] = vq[i];
+      for (int i = 0; i < Q::Loads; ++i)
+        reinterpret_cast<uint4*>(dq)[i * C::Threads + threadIdx.x] = keep16<SHORT, T>(vq[i], K - s * BK - qc, K);
       if ((s + 1) * BK < K) load(s + 1);
     };
     C::run(K, fill, wave, lane, acc, store);
@@ -406,7 +409,7 @@ __global__ __launch_bounds__(64 * WP * WQ) void grouped_rows_kernel(GroupedArgs 
 
 // dW[e][d][f] = Σ_p x[p][d] dy[p][f]: P is dy (columns f), Q is x (rows d).  SPLIT: a group's
 // positions are cut into gridDim.y parts, whose sums are written as fp32 and added by grouped_reduce.
-template <typename T, bool DIRECT, bool WIDE, bool SPLIT, int BP, int BQ, int WP, int WQ>
+template <typename T, bool DIRECT, bool WIDE, bool SPLIT, int BP, int BQ, int WP, int WQ, bool SHORT>
 __global__ __launch_bounds__(64 * WP * WQ) void grouped_dw_kernel(GroupedArgs a, int ptiles, int qtiles) {
   typedef Core<T, false, false, BP, BQ, WP, WQ> C;
   typedef typename C::P P;
@@ -461,9 +464,9 @@ __global__ __launch_bounds__(64 * WP * WQ) void grouped_dw_kernel(GroupedArgs a,
       const uint8_t* ds = dy + k0 * ld;
 #pragma unroll
       for (int i = 0; i < P::Loads; ++i)
-        fetch16(ds, __umul24(min(P::row(i), n - 1 - k0), (uint32_t)ld) + poff, dp + i * (C::Threads * 16));
+        fetch_direct(ds, __umul24(min(P::row(i), n - 1 - k0), (uint32_t)ld) + poff, dp + i * (C::Threads * 16));
 #pragma unroll
-      for (int i = 0; i < Q::Loads; ++i) fetch16(x, qoff[i], dq + i * (C::Threads * 16));
+      for (int i = 0; i < Q::Loads; ++i) fetch_direct(x, qoff[i], dq + i * (C::Threads * 16));
     };
     C::run(n, fill, wave, lane, acc, store);
   } else {
@@ -472,17 +475,19 @@ __global__ __launch_bounds__(64 * WP * WQ) void grouped_dw_kernel(GroupedArgs a,
     uint4 vp[P::Loads], vq[Q::Loads];
     auto load = [&](int s) {
 #pragma unroll
-      for (int i = 0; i < P::Loads; ++i) vp[i] = load16(dy + min(s * BK + P::row(i), n - 1) * a.lddy, a.Nn - fc);
+      for (int i = 0; i < P::Loads; ++i) vp[i] = fetch16<SHORT>(dy + min(s * BK + P::row(i), n - 1) * a.lddy, a.Nn - fc);
 #pragma unroll
-      for (int i = 0; i < Q::Loads; ++i) vq[i] = load16(x + src[i] * a.ldx, a.K - dc);
+      for (int i = 0; i < Q::Loads; ++i) vq[i] = fetch16<SHORT>(x + src[i] * a.ldx, a.K - dc);
       look(s + 1);
     };
     load(0);
     auto fill = [&](int s, uint8_t* dp, uint8_t* dq) {
 #pragma unroll
-      for (int i = 0; i < P::Loads; ++i) reinterpret_cast<uint4*>(dp)[i * C::Threads + threadIdx.x] = vp[i];
+      for (int i = 0; i < P::Loads; ++i)
+        reinterpret_cast<uint4*>(dp)[i * C::Threads + threadIdx.x] = keep16<SHORT, T>(vp[i], a.Nn - fc, a.Nn);
 #pragma unroll
-      for (int i = 0; i < Q::Loads; ++i) reinterpret_cast<uint4*>(dq)[i * C::Threads + threadIdx.x] = vq[i];
+      for (int i = 0; i < Q::Loads; ++i)
+        reinterpret_cast<uint4*>(dq)[i * C::Threads + threadIdx.x] = keep16<SHORT, T>(vq[i], a.K - dc, a.K);
       if ((s + 1) * BK < n) load(s + 1);
     };
     C::run(n, fill, wave, lane, acc, store);
@@ -493,11 +498,11 @@ __global__ __launch_bounds__(64 * WP * WQ) void grouped_dw_kernel(GroupedArgs a,
 template <typename T>
 bool wide(const GroupedArgs& a) { return (a.Nx * a.ldx + a.K) * (int64_t)sizeof(T) >= (int64_t(1) << 32); }
 
-template <typename T, bool WKC, bool DIRECT, bool WIDE, int B, int WP, int WQ>
+template <typename T, bool WKC, bool DIRECT, bool WIDE, int B, int WP, int WQ, bool SHORT = false>
 void rows_tiled(const GroupedArgs& a, hipStream_t s) {
   const int ntiles = (a.Nn + B - 1) / B;
   const int64_t grid = (a.M / B + a.E + 1) * ntiles;
-  grouped_rows_kernel<T, WKC, DIRECT, WIDE, B, B, WP, WQ><<<(unsigned)grid, 64 * WP * WQ, 0, s>>>(a, ntiles);
+  grouped_rows_kernel<T, WKC, DIRECT, WIDE, B, B, WP, WQ, SHORT><<<(unsigned)grid, 64 * WP * WQ, 0, s>>>(a, ntiles);
 }
 
 template <typename T, bool WKC>
@@ -506,21 +511,23 @@ void rows_by(const GroupedArgs& a, bool direct, bool larger, hipStream_t s) {
     if (direct && larger)
       return wide<T>(a) ? rows_tiled<T, WKC, true, true, 256, 4, 2>(a, s) : rows_tiled<T, WKC, true, false, 256, 4, 2>(a, s);
   }
-  if (!direct) rows_tiled<T, WKC, false, true, 128, 2, 2>(a, s);
+  if (a.K < kVec<T> || a.Nn < kVec<T>) rows_tiled<T, WKC, false, true, 128, 2, 2, true>(a, s);
+  else if (!direct) rows_tiled<T, WKC, false, true, 128, 2, 2>(a, s);
   else if (wide<T>(a)) rows_tiled<T, WKC, true, true, 128, 2, 2>(a, s);
   else rows_tiled<T, WKC, true, false, 128, 2, 2>(a, s);
 }
 
-template <typename T, bool DIRECT, bool WIDE, bool SPLIT, int B, int WP, int WQ>
+template <typename T, bool DIRECT, bool WIDE, bool SPLIT, int B, int WP, int WQ, bool SHORT = false>
 void dw_tiled(const GroupedArgs& a, int splits, hipStream_t s) {
   const int pt = (a.Nn + B - 1) / B, qt = (a.K + B - 1) / B;
-  grouped_dw_kernel<T, DIRECT, WIDE, SPLIT, B, B, WP, WQ>
+  grouped_dw_kernel<T, DIRECT, WIDE, SPLIT, B, B, WP, WQ, SHORT>
       <<<dim3((unsigned)(a.E * pt * qt), (unsigned)splits), 64 * WP * WQ, 0, s>>>(a, pt, qt);
 }
 
 template <typename T, bool SPLIT>
 void dw_by(const GroupedArgs& a, bool direct, int splits, hipStream_t s) {
-  if (!direct) dw_tiled<T, false, true, SPLIT, 128, 2, 2>(a, splits, s);
+  if (a.K < kVec<T> || a.Nn < kVec<T>) dw_tiled<T, false, true, SPLIT, 128, 2, 2, true>(a, splits, s);
+  else if (!direct) dw_tiled<T, false, true, SPLIT, 128, 2, 2>(a, splits, s);
   else if (wide<T>(a)) dw_tiled<T, true, true, SPLIT, 128, 2, 2>(a, splits, s);
   else dw_tiled<T, true, false, SPLIT, 128, 2, 2>(a, splits, s);
 }

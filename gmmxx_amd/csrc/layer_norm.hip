@@ -25,7 +25,7 @@ namespace {
 constexpr int kNormThreads = 256;
 constexpr int kFwdMaxBlocks = 2048;
 
-template <typename T, typename WT, int G, int NV>
+template <typename T, typename WT, int G, int NV, bool SHORT>
 struct Norm {
   static constexpr int V = kVec<T>;
   static constexpr int Threads = G > kNormThreads ? G : kNormThreads;
@@ -34,9 +34,13 @@ struct Norm {
   // This thread's elements of a row: vector i covers columns (i G + lane) V ...
   __device__ static __forceinline__ int col(int i, int lane) { return (i * G + lane) * V; }
 
-  __device__ static __forceinline__ void load(const T* row, int D, int lane, float (&v)[NV][V]) {
+  __device__ static __forceinline__ void fetch(const T* row, int D, int lane, uint4 (&u)[NV]) {
 #pragma unroll
-    for (int i = 0; i < NV; ++i) load_row(row + col(i, lane), D - col(i, lane), v[i]);
+    for (int i = 0; i < NV; ++i) u[i] = fetch16<SHORT>(row + col(i, lane), D - col(i, lane));
+  }
+  __device__ static __forceinline__ void unpack(const uint4 (&u)[NV], int D, int lane, float (&v)[NV][V]) {
+#pragma unroll
+    for (int i = 0; i < NV; ++i) unpack16<T>(keep16<SHORT, T>(u[i], D - col(i, lane), D), v[i]);
   }
   __device__ static __forceinline__ void load_param(const void* p, int D, int lane, float fill, float (&v)[NV][V]) {
     const WT* w = static_cast<const WT*>(p);
@@ -51,35 +55,44 @@ struct Norm {
   }
 };
 
-template <typename T, typename WT, int G, int NV>
-__global__ __launch_bounds__((Norm<T, WT, G, NV>::Threads)) void norm_fwd_kernel(NormArgs a) {
-  using L = Norm<T, WT, G, NV>;
+template <typename T, typename WT, int G, int NV, bool SHORT>
+__global__ __launch_bounds__((Norm<T, WT, G, NV, SHORT>::Threads)) void norm_fwd_kernel(NormArgs a) {
+  using L = Norm<T, WT, G, NV, SHORT>;
   constexpr int V = L::V;
-  __shared__ float red[2][16];
+  __shared__ float red[2][16][1];
   int turn = 0;
   const int lane = threadIdx.x % G, sub = threadIdx.x / G;
+  const int64_t step = (int64_t)gridDim.x * L::RPB;
+  int64_t row = (int64_t)blockIdx.x * L::RPB + sub;
+  if (row >= a.N) return;
+  const T* x0 = static_cast<const T*>(a.x);
+  uint4 next[NV];
+  L::fetch(x0 + row * a.ldx, a.D, lane, next);
   float w[NV][V], b[NV][V];
   L::load_param(a.weight, a.D, lane, 1.f, w);
   L::load_param(a.bias, a.D, lane, 0.f, b);
   const float inv = 1.f / (float)a.D;
-  for (int64_t row = (int64_t)blockIdx.x * L::RPB + sub; row < a.N; row += (int64_t)gridDim.x * L::RPB) {
+  for (; row < a.N; row += step) {
     float x[NV][V];
-    L::load(static_cast<const T*>(a.x) + row * a.ldx, a.D, lane, x);
-    float s = 0.f;
+    L::unpack(next, a.D, lane, x);
+    if (row + step < a.N) L::fetch(x0 + (row + step) * a.ldx, a.D, lane, next);
+    float s[1] = {0.f};
 #pragma unroll
     for (int i = 0; i < NV; ++i)
 #pragma unroll
-      for (int j = 0; j < V; ++j) s += x[i][j];
-    const float mean = group_sum<G>(s, red, turn) * inv;
-    float q = 0.f;
+      for (int j = 0; j < V; ++j) s[0] += x[i][j];
+    group_sums<G>(s, red, turn);
+    const float mean = s[0] * inv;
+    float q[1] = {0.f};
 #pragma unroll
     for (int i = 0; i < NV; ++i)
 #pragma unroll
       for (int j = 0; j < V; ++j) {
         x[i][j] = L::col(i, lane) + j < a.D ? x[i][j] - mean : 0.f;
-        q = fmaf(x[i][j], x[i][j], q);
+        q[0] = fmaf(x[i][j], x[i][j], q[0]);
       }
-    const float rstd = 1.f / sqrtf(group_sum<G>(q, red, turn) * inv + a.eps);
+    group_sums<G>(q, red, turn);
+    const float rstd = 1.f / sqrtf(q[0] * inv + a.eps);
     T* out = static_cast<T*>(a.y) + row * a.D;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
@@ -94,14 +107,26 @@ __global__ __launch_bounds__((Norm<T, WT, G, NV>::Threads)) void norm_fwd_kernel
   }
 }
 
-template <typename T, typename WT, int G, int NV>
-__global__ __launch_bounds__((Norm<T, WT, G, NV>::Threads)) void norm_bwd_kernel(NormArgs a) {
-  using L = Norm<T, WT, G, NV>;
+template <typename T, typename WT, int G, int NV, bool SHORT>
+__global__ __launch_bounds__((Norm<T, WT, G, NV, SHORT>::Threads)) void norm_bwd_kernel(NormArgs a) {
+  using L = Norm<T, WT, G, NV, SHORT>;
   constexpr int V = L::V;
-  __shared__ float red[2][16];
+  __shared__ float red[2][16][2];
   __shared__ float cols[L::RPB > 1 ? L::Threads * NV * V : 1];
   int turn = 0;
   const int lane = threadIdx.x % G, sub = threadIdx.x / G;
+  const int64_t step = (int64_t)gridDim.x * L::RPB;
+  int64_t row = (int64_t)blockIdx.x * L::RPB + sub;
+  const T *x0 = static_cast<const T*>(a.x), *dy0 = static_cast<const T*>(a.dy);
+  uint4 next_x[NV], next_dy[NV];
+  float next_mean = 0.f, next_rstd = 0.f;
+  auto fetch = [&](int64_t r) {
+    L::fetch(x0 + r * a.ldx, a.D, lane, next_x);
+    L::fetch(dy0 + r * a.lddy, a.D, lane, next_dy);
+    next_mean = a.mean[r];
+    next_rstd = a.rstd[r];
+  };
+  if (row < a.N) fetch(row);
   float w[NV][V], dw[NV][V], db[NV][V];
   L::load_param(a.weight, a.D, lane, 1.f, w);
 #pragma unroll
@@ -109,12 +134,13 @@ __global__ __launch_bounds__((Norm<T, WT, G, NV>::Threads)) void norm_bwd_kernel
 #pragma unroll
     for (int j = 0; j < V; ++j) dw[i][j] = db[i][j] = 0.f;
   const float inv = 1.f / (float)a.D;
-  for (int64_t row = (int64_t)blockIdx.x * L::RPB + sub; row < a.N; row += (int64_t)gridDim.x * L::RPB) {
+  for (; row < a.N; row += step) {
     float h[NV][V], g[NV][V];
-    L::load(static_cast<const T*>(a.x) + row * a.ldx, a.D, lane, h);
-    L::load(static_cast<const T*>(a.dy) + row * a.lddy, a.D, lane, g);
-    const float mean = a.mean[row], rstd = a.rstd[row];
-    float sg = 0.f, sgh = 0.f;
+    L::unpack(next_x, a.D, lane, h);
+    L::unpack(next_dy, a.D, lane, g);
+    const float mean = next_mean, rstd = next_rstd;
+    if (row + step < a.N) fetch(row + step);
+    float s[2] = {0.f, 0.f};
 #pragma unroll
     for (int i = 0; i < NV; ++i)
 #pragma unroll
@@ -123,11 +149,11 @@ __global__ __launch_bounds__((Norm<T, WT, G, NV>::Threads)) void norm_bwd_kernel
         dw[i][j] = fmaf(g[i][j], h[i][j], dw[i][j]);
         db[i][j] += g[i][j];
         g[i][j] *= w[i][j];
-        sg += g[i][j];
-        sgh = fmaf(g[i][j], h[i][j], sgh);
+        s[0] += g[i][j];
+        s[1] = fmaf(g[i][j], h[i][j], s[1]);
       }
-    const float mg = group_sum<G>(sg, red, turn) * inv;
-    const float mgh = group_sum<G>(sgh, red, turn) * inv;
+    group_sums<G>(s, red, turn);
+    const float mg = s[0] * inv, mgh = s[1] * inv;
     T* out = static_cast<T*>(a.y) + row * a.D;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
@@ -193,17 +219,18 @@ __global__ __launch_bounds__(kSumCols* kSumRows) void norm_sum_kernel(NormArgs a
   }
 }
 
-// Calls f.template operator()<G, NV>() for the smallest group that holds a row of D.
+// Calls f.template operator()<G, NV, SHORT>() for the smallest group that holds a row of D.
 template <typename T, typename F>
 void with_group(int D, F&& f) {
   constexpr int N16 = 16 / kVec<T>;    // vectors of 16 elements
-  if (D <= 8 * 16) f.template operator()<8, N16>();
-  else if (D <= 16 * 16) f.template operator()<16, N16>();
-  else if (D <= 32 * 16) f.template operator()<32, N16>();
-  else if (D <= 64 * 16) f.template operator()<64, N16>();
-  else if (D <= 256 * 16) f.template operator()<256, N16>();
-  else if (D <= 256 * 32) f.template operator()<256, 2 * N16>();
-  else f.template operator()<1024, 4 * N16>();
+  if (D < kVec<T>) f.template operator()<8, N16, true>();
+  else if (D <= 8 * 16) f.template operator()<8, N16, false>();
+  else if (D <= 16 * 16) f.template operator()<16, N16, false>();
+  else if (D <= 32 * 16) f.template operator()<32, N16, false>();
+  else if (D <= 64 * 16) f.template operator()<64, N16, false>();
+  else if (D <= 256 * 16) f.template operator()<256, N16, false>();
+  else if (D <= 256 * 32) f.template operator()<256, 2 * N16, false>();
+  else f.template operator()<1024, 4 * N16, false>();
 }
 
 template <typename F>
@@ -229,11 +256,11 @@ struct FwdOp {
   }
   template <typename T, typename WT> struct Go {
     const NormArgs& a; hipStream_t s;
-    template <int G, int NV> void operator()() {
-      using L = Norm<T, WT, G, NV>;
+    template <int G, int NV, bool SHORT> void operator()() {
+      using L = Norm<T, WT, G, NV, SHORT>;
       const int64_t need = (a.N + L::RPB - 1) / L::RPB;
       const int grid = (int)(need < kFwdMaxBlocks ? need : kFwdMaxBlocks);
-      norm_fwd_kernel<T, WT, G, NV><<<grid, L::Threads, 0, s>>>(a);
+      norm_fwd_kernel<T, WT, G, NV, SHORT><<<grid, L::Threads, 0, s>>>(a);
     }
   };
 };
@@ -247,8 +274,8 @@ struct BwdOp {
   }
   template <typename T, typename WT> struct Go {
     const NormArgs& a; hipStream_t s; int blocks;
-    template <int G, int NV> void operator()() {
-      norm_bwd_kernel<T, WT, G, NV><<<blocks, Norm<T, WT, G, NV>::Threads, 0, s>>>(a);
+    template <int G, int NV, bool SHORT> void operator()() {
+      norm_bwd_kernel<T, WT, G, NV, SHORT><<<blocks, Norm<T, WT, G, NV, SHORT>::Threads, 0, s>>>(a);
     }
   };
 };

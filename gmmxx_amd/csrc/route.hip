@@ -7,7 +7,7 @@
 // is placed after all groups.
 //
 // Grouping is stable (by expert, then by row), so it is a function of the scores
-// alone.  Three launches:
+// alone.  Three launches (one for up to 64 rows and 512 experts):
 //   top:   choices, gates and, for each block of rows, the count of every expert;
 //   scan:  the counts become exclusive prefixes over the blocks, and their totals;
 //   place: every block adds the experts' offsets to its prefixes and ranks its own
@@ -35,80 +35,132 @@ int64_t block_rows(int64_t N) {
   return r;
 }
 
-// The weight of score v beside the row's largest m.
-__device__ __forceinline__ float weight_of(float v, float m) {
-  return v == m ? 1.f : (v == -INFINITY ? 0.f : expf(v - m));
+// exp(x) for x <= 0 by the hardware's power of two, with the rounding of x log2(e) put back in first order.
+__device__ __forceinline__ float exp_below(float x) {
+  const float y = fmaxf(x * kLog2e, -150.f);      // (2^-150 is 0)
+  const float lost = fmaf(x, 1.925963033500e-8f, fmaf(x, kLog2e, -y));      // (log2(e) = kLog2e + 1.926e-8)
+  return y > -150.f ? fast_exp2(y) * fmaf(lost, kLn2, 1.f) : 0.f;
 }
 
-template <typename T, int G, int V>
-__global__ __launch_bounds__(kThreads) void route_top_kernel(RouteArgs a, int64_t rpb) {
-  __shared__ int count[kRouteMaxE + 1];
-  __shared__ int sel[kPassRows * kRouteMaxK];
-  __shared__ float wsel[kPassRows * kRouteMaxK];
+// The weight of score v beside the row's largest m (v <= m): 1 for each of several +inf.
+__device__ __forceinline__ float weight_of(float v, float m) { return v == m ? 1.f : exp_below(v - m); }
+
+// Integers in the order of the scores; -0 as 0.  kNone, the key of -inf, and below: no candidate.
+__device__ __forceinline__ int key_of(float v) {
+  const int b = __float_as_int(v + 0.f);
+  return b ^ ((b >> 31) & 0x7fffffff);
+}
+__device__ __forceinline__ float score_of(int key) { return __int_as_float(key ^ ((key >> 31) & 0x7fffffff)); }
+constexpr int kNone = (int)0x807fffffu;
+
+// op over a group's lanes for integers (see lanes_reduce).
+template <int G, typename F>
+__device__ __forceinline__ int lanes_reduce_int(int v, F&& op) {
+  return __float_as_int(lanes_reduce<G>(__int_as_float(v), [&](float a, float b) {
+    return __int_as_float(op(__float_as_int(a), __float_as_int(b)));
+  }));
+}
+
+// The choices of up to kPassRows rows, to LDS.  G lanes share a row, NV vectors of its scores each: vector i of
+// lane l holds the scores from (i G + l) kVec on, as integers in their order.  Each round takes the group's
+// largest remaining score, then the lowest index that has it.  About 5 instructions a held score and round, so
+// G is the smallest that holds the row in 32 scores a lane (64 at the most experts).
+template <typename T, int G, int NV, bool SHORT>
+__device__ __forceinline__ void choose_rows(const RouteArgs& a, int64_t base, int rows, int* sel, float* wsel) {
+  constexpr int VV = kVec<T>, R = kThreads / G;
   const int lane = threadIdx.x % G, sub = threadIdx.x / G;
-  constexpr int R = kThreads / G;
+  const auto larger = [](int p, int q) { return p > q ? p : q; };
+  const auto smaller = [](int p, int q) { return p < q ? p : q; };
+  for (int r0 = 0; r0 < rows; r0 += R) {        // (all lanes stay in the loop: groups exchange across the wave)
+    const int r = r0 + sub;
+    const bool there = r < rows;
+    const T* row = static_cast<const T*>(a.scores) + (base + (there ? r : 0)) * a.lds;
+    int v[NV][VV];
+    uint4 u[NV];
+#pragma unroll
+    for (int i = 0; i < NV; ++i) u[i] = fetch16<SHORT>(row + (i * G + lane) * VV, a.E - (i * G + lane) * VV);
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int c = (i * G + lane) * VV;
+      float s[VV];
+      unpack16<T>(keep16<SHORT, T>(u[i], a.E - c, a.E), s);
+#pragma unroll
+      for (int j = 0; j < VV; ++j) v[i][j] = s[j] == s[j] && c + j < a.E ? key_of(s[j]) : INT32_MIN;
+    }
+    int best = INT32_MIN;
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+#pragma unroll
+      for (int q = 0; q < VV; ++q) best = larger(best, v[i][q]);
+    best = lanes_reduce_int<G>(best, larger);
+    const float m = best > kNone ? score_of(best) : -INFINITY;
+    float sum = 0.f;
+    if (!a.renormalize) {
+      if (fabsf(m) < INFINITY) {
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+#pragma unroll
+          for (int q = 0; q < VV; ++q) sum += v[i][q] > kNone ? exp_below(score_of(v[i][q]) - m) : 0.f;
+      } else {      // of +inf each weighs 1
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+#pragma unroll
+          for (int q = 0; q < VV; ++q) sum += v[i][q] == best ? 1.f : 0.f;
+      }
+      sum = lanes_sum<G>(sum);
+    }
+    float chosen = 0.f;
+    for (int j = 0; j < a.k; ++j) {
+      if (j > 0) {
+        best = INT32_MIN;
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+#pragma unroll
+          for (int q = 0; q < VV; ++q) best = larger(best, v[i][q]);
+        best = lanes_reduce_int<G>(best, larger);
+      }
+      int at = INT32_MAX;
+#pragma unroll
+      for (int i = NV - 1; i >= 0; --i)
+#pragma unroll
+        for (int q = VV - 1; q >= 0; --q) at = v[i][q] == best ? i * G * VV + q : at;
+      at = lanes_reduce_int<G>(at == INT32_MAX ? at : at + lane * VV, smaller);
+      const bool none = best <= kNone;
+      const float w = none ? 0.f : weight_of(score_of(best), m);
+      chosen += w;
+      const int mine = at - lane * VV;
+#pragma unroll
+      for (int i = 0; i < NV; ++i)
+#pragma unroll
+        for (int q = 0; q < VV; ++q) v[i][q] = mine == i * G * VV + q ? INT32_MIN : v[i][q];
+      if (lane == 0 && there) {
+        sel[r * a.k + j] = none ? -1 : at;
+        wsel[r * a.k + j] = w;
+      }
+    }
+    if (a.renormalize) sum = chosen;
+    const float inv = m == -INFINITY ? 0.f : 1.f / sum;
+    // (the lanes of a group are one wave's: lane 0's LDS writes above come first)
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    if (there) {
+      for (int j = lane; j < a.k; j += G) wsel[r * a.k + j] *= inv;
+      if (lane == 0 && a.norm) a.norm[base + r] = make_float2(m, inv);
+    }
+  }
+}
+
+template <typename T, int G, int NV, bool SHORT>
+__global__ __launch_bounds__(kThreads) void route_top_kernel(RouteArgs a, int64_t rpb) {
+  extern __shared__ int lds[];           // choices, their weights, counts: top_lds()
+  int* sel = lds;
+  float* wsel = reinterpret_cast<float*>(lds + kPassRows * a.k);
+  int* count = lds + 2 * kPassRows * a.k;
   for (int e = threadIdx.x; e <= a.E; e += kThreads) count[e] = 0;
   const int64_t first = blockIdx.x * rpb, last = first + rpb < a.N ? first + rpb : a.N;
   for (int64_t base = first; base < last; base += kPassRows) {
     const int rows = (int)(last - base < kPassRows ? last - base : kPassRows);
     __syncthreads();
-    for (int r = sub; r < rows; r += R) {
-      const T* row = static_cast<const T*>(a.scores) + (base + r) * a.lds;
-      float v[V];
-      float m = -INFINITY;
-#pragma unroll
-      for (int i = 0; i < V; ++i) {
-        const int c = lane * V + i;
-        const float s = c < a.E ? to_f32(row[c]) : -INFINITY;
-        v[i] = s == s ? s : -INFINITY;
-        m = fmaxf(m, v[i]);
-      }
-#pragma unroll
-      for (int off = G / 2; off >= 1; off /= 2) m = fmaxf(m, __shfl_xor(m, off));
-      float sum = 0.f;
-      if (!a.renormalize) {
-#pragma unroll
-        for (int i = 0; i < V; ++i) sum += weight_of(v[i], m);
-        sum = lanes_sum<G>(sum);
-      }
-      float chosen = 0.f;
-      for (int j = 0; j < a.k; ++j) {
-        float best = v[0];
-        int at = 0;
-#pragma unroll
-        for (int i = 1; i < V; ++i)
-          if (v[i] > best) {
-            best = v[i];
-            at = i;
-          }
-        int idx = lane * V + at;
-#pragma unroll
-        for (int off = G / 2; off >= 1; off /= 2) {
-          const float b2 = __shfl_xor(best, off);
-          const int i2 = __shfl_xor(idx, off);
-          if (b2 > best || (b2 == best && i2 < idx)) {
-            best = b2;
-            idx = i2;
-          }
-        }
-        const bool none = best == -INFINITY;
-        const float w = none ? 0.f : weight_of(best, m);
-        chosen += w;
-#pragma unroll
-        for (int i = 0; i < V; ++i)
-          if (idx == lane * V + i) v[i] = -INFINITY;
-        if (lane == 0) {
-          sel[r * a.k + j] = none ? -1 : idx;
-          wsel[r * a.k + j] = w;
-        }
-      }
-      if (a.renormalize) sum = chosen;
-      const float inv = m == -INFINITY ? 0.f : 1.f / sum;
-      // (the lanes of a group are one wave's: lane 0's LDS writes above come first)
-      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-      for (int j = lane; j < a.k; j += G) wsel[r * a.k + j] *= inv;
-      if (lane == 0 && a.norm) a.norm[base + r] = make_float2(m, inv);
-    }
+    choose_rows<T, G, NV, SHORT>(a, base, rows, sel, wsel);
     __syncthreads();
     for (int i = threadIdx.x; i < rows * a.k; i += kThreads) {
       const int e = sel[i];
@@ -152,29 +204,29 @@ __global__ __launch_bounds__(kScanCols* kScanParts) void route_scan_kernel(Route
   }
 }
 
-template <int MAXE>
-__global__ __launch_bounds__(kThreads) void route_place_kernel(RouteArgs a, int64_t rpb) {
+// Positions of choices first .. last - 1 (expert(i): that of choice i, a.E for none), given total(e), how many
+// choices expert e has, and before(e), how many of them come before `first`.
+template <int MAXE, typename X, typename N, typename B>
+__device__ __forceinline__ void place(const RouteArgs& a, int64_t first, int64_t last, X&& expert, N&& total,
+                                      B&& before) {
   constexpr int W = kThreads / 64;
   __shared__ int next[W][MAXE + 1];      // counts of a wave's part, then the next position of each expert
   __shared__ int wave_sum[W];
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
   const int groups = a.E + 1;            // the last: choices without an expert
-  const int64_t first = blockIdx.x * rpb * a.k;
-  const int64_t all = a.N * a.k, last = first + rpb * a.k < all ? first + rpb * a.k : all;
   const int64_t per = (last - first + W * 64 - 1) / (W * 64) * 64;
   const int64_t lo = first + w * per < last ? first + w * per : last, hi = lo + per < last ? lo + per : last;
-  for (int e = threadIdx.x; e < W * groups; e += kThreads) next[e / groups][e % groups] = 0;
+  for (int e = threadIdx.x; e < groups; e += kThreads)
+#pragma unroll
+    for (int q = 0; q < W; ++q) next[q][e] = 0;
   __syncthreads();
-  for (int64_t i = lo + lane; i < hi; i += 64) {
-    const int e = a.experts[i];
-    atomicAdd(&next[w][e < 0 ? a.E : e], 1);
-  }
+  for (int64_t i = lo + lane; i < hi; i += 64) atomicAdd(&next[w][expert(i)], 1);
   // The experts' offsets: an exclusive scan of the totals, each thread a contiguous part.
   const int chunk = (groups + kThreads - 1) / kThreads;
   const int e0 = threadIdx.x * chunk < groups ? threadIdx.x * chunk : groups;
   const int e1 = e0 + chunk < groups ? e0 + chunk : groups;
   int s = 0;
-  for (int e = e0; e < e1; ++e) s += a.totals[e];
+  for (int e = e0; e < e1; ++e) s += total(e);
   int incl = s;
 #pragma unroll
   for (int off = 1; off < 64; off *= 2) {
@@ -185,17 +237,16 @@ __global__ __launch_bounds__(kThreads) void route_place_kernel(RouteArgs a, int6
   __syncthreads();
   int off0 = incl - s;
   for (int q = 0; q < w; ++q) off0 += wave_sum[q];
-  const int32_t* before = a.hist + (int64_t)blockIdx.x * groups;
   for (int e = e0; e < e1; ++e) {
     if (blockIdx.x == 0) a.offsets[e] = off0;
-    int at = off0 + before[e];
+    int at = off0 + before(e);
 #pragma unroll
     for (int q = 0; q < W; ++q) {
       const int n = next[q][e];
       next[q][e] = at;
       at += n;
     }
-    off0 += a.totals[e];
+    off0 += total(e);
   }
   __syncthreads();
   int bits = 0;
@@ -203,8 +254,7 @@ __global__ __launch_bounds__(kThreads) void route_place_kernel(RouteArgs a, int6
   for (int64_t i0 = lo; i0 < hi; i0 += 64) {
     const int64_t i = i0 + lane;
     const bool in = i < hi;
-    int e = in ? a.experts[i] : 0;
-    e = e < 0 ? a.E : e;
+    const int e = in ? expert(i) : 0;
     uint64_t same = __ballot(in);
     for (int b = 0; b < bits; ++b) {
       const uint64_t set = __ballot((e >> b) & 1);
@@ -222,14 +272,51 @@ __global__ __launch_bounds__(kThreads) void route_place_kernel(RouteArgs a, int6
   }
 }
 
+template <int MAXE>
+__global__ __launch_bounds__(kThreads) void route_place_kernel(RouteArgs a, int64_t rpb) {
+  const int64_t first = blockIdx.x * rpb * a.k, all = a.N * a.k, last = first + rpb * a.k < all ? first + rpb * a.k : all;
+  const int32_t* before = a.hist + (int64_t)blockIdx.x * (a.E + 1);
+  place<MAXE>(
+      a, first, last,
+      [&](int64_t i) {
+        const int e = a.experts[i];
+        return e < 0 ? a.E : e;
+      },
+      [&](int e) { return a.totals[e]; }, [&](int e) { return before[e]; });
+}
+
+// Few rows (one pass of one block) in one launch.
+constexpr int kOneMaxE = 512;
+template <typename T, int G, int NV, bool SHORT>
+__global__ __launch_bounds__(kThreads) void route_one_kernel(RouteArgs a) {
+  extern __shared__ int lds[];
+  int* sel = lds;
+  float* wsel = reinterpret_cast<float*>(lds + kPassRows * a.k);
+  int* count = lds + 2 * kPassRows * a.k;
+  for (int e = threadIdx.x; e <= a.E; e += kThreads) count[e] = 0;
+  choose_rows<T, G, NV, SHORT>(a, 0, (int)a.N, sel, wsel);
+  __syncthreads();
+  const int all = (int)a.N * a.k;
+  for (int i = threadIdx.x; i < all; i += kThreads) {
+    const int e = sel[i];
+    a.experts[i] = e;
+    a.gates[i] = wsel[i];
+    atomicAdd(&count[e < 0 ? a.E : e], 1);
+  }
+  __syncthreads();
+  place<kOneMaxE>(
+      a, 0, all, [&](int64_t i) { return sel[i] < 0 ? a.E : sel[i]; }, [&](int e) { return count[e]; },
+      [](int) { return 0; });
+}
+
 // Gradient of the scores: renormalised gates  ds_e = g_e (dg_e - Σ g dg) for the chosen, 0 elsewhere;
 // otherwise  ds_e = [e chosen] g_e dg_e - p_e Σ g dg,  p_e = w_e / Σ w.
-template <typename T>
+template <typename T, bool SHORT>
 __global__ __launch_bounds__(kThreads) void route_bwd_kernel(RouteArgs a, int tile) {
-  extern __shared__ float lds[];
+  extern __shared__ int lds[];
   constexpr int V = kVec<T>;
-  int* sel = reinterpret_cast<int*>(lds);             // [tile][k]
-  float* coef = lds + tile * a.k;                     // [tile][k]
+  int* sel = lds;                                                      // [tile][k]
+  float* coef = reinterpret_cast<float*>(lds + tile * a.k);            // [tile][k]
   float* mean = coef + tile * a.k;                    // [tile]
   const int64_t base = (int64_t)blockIdx.x * tile;
   const int rows = (int)(a.N - base < tile ? a.N - base : tile);
@@ -257,10 +344,10 @@ __global__ __launch_bounds__(kThreads) void route_bwd_kernel(RouteArgs a, int ti
 #pragma unroll
       for (int q = 0; q < V; ++q) o[q] = 0.f;
     } else {
-      load_row(static_cast<const T*>(a.scores) + (base + r) * a.lds + c, a.E - c, o);
+      unpack16<T>(keep16<SHORT, T>(fetch16<SHORT>(static_cast<const T*>(a.scores) + (base + r) * a.lds + c, a.E - c), a.E - c, a.E), o);
       const float2 nm = a.norm[base + r];
 #pragma unroll
-      for (int q = 0; q < V; ++q) o[q] = -mean[r] * (o[q] == o[q] && nm.y != 0.f ? weight_of(o[q], nm.x) * nm.y : 0.f);
+      for (int q = 0; q < V; ++q) o[q] = -mean[r] * (o[q] > -INFINITY ? weight_of(o[q], nm.x) * nm.y : 0.f);      // (NaN and -inf: no candidates)
     }
     for (int j = 0; j < a.k; ++j) {
       const int e = sel[r * a.k + j];
@@ -273,13 +360,34 @@ __global__ __launch_bounds__(kThreads) void route_bwd_kernel(RouteArgs a, int ti
   }
 }
 
+size_t top_lds(const RouteArgs& a) { return (size_t)(2 * kPassRows * a.k + a.E + 1) * 4; }
+
+template <typename T, int G, int NV, bool SHORT>
+void top_shaped(const RouteArgs& a, int64_t rpb, unsigned grid, hipStream_t s) {
+  if constexpr (G * NV * kVec<T> <= kOneMaxE) {
+    if (a.N <= kPassRows) return route_one_kernel<T, G, NV, SHORT><<<1, kThreads, top_lds(a), s>>>(a);
+  }
+  route_top_kernel<T, G, NV, SHORT><<<grid, kThreads, top_lds(a), s>>>(a, rpb);
+}
+
 template <typename T>
 void top_typed(const RouteArgs& a, int64_t rpb, unsigned grid, hipStream_t s) {
-  if (a.E <= 8) route_top_kernel<T, 8, 1><<<grid, kThreads, 0, s>>>(a, rpb);
-  else if (a.E <= 64) route_top_kernel<T, 16, 4><<<grid, kThreads, 0, s>>>(a, rpb);
-  else if (a.E <= 256) route_top_kernel<T, 64, 4><<<grid, kThreads, 0, s>>>(a, rpb);
-  else if (a.E <= 1024) route_top_kernel<T, 64, 16><<<grid, kThreads, 0, s>>>(a, rpb);
-  else route_top_kernel<T, 64, 64><<<grid, kThreads, 0, s>>>(a, rpb);
+  constexpr int N8 = 8 / kVec<T>;       // vectors of 8 scores
+  if (a.E < kVec<T>) top_shaped<T, 4, N8, true>(a, rpb, grid, s);
+  else if (a.E <= 32) top_shaped<T, 4, N8, false>(a, rpb, grid, s);
+  else if (a.E <= 64) top_shaped<T, 4, 2 * N8, false>(a, rpb, grid, s);
+  else if (a.E <= 128) top_shaped<T, 8, 2 * N8, false>(a, rpb, grid, s);
+  else if (a.E <= 256) top_shaped<T, 8, 4 * N8, false>(a, rpb, grid, s);
+  else if (a.E <= 512) top_shaped<T, 16, 4 * N8, false>(a, rpb, grid, s);
+  else if (a.E <= 1024) top_shaped<T, 32, 4 * N8, false>(a, rpb, grid, s);
+  else if (a.E <= 2048) top_shaped<T, 64, 4 * N8, false>(a, rpb, grid, s);
+  else top_shaped<T, 64, 8 * N8, false>(a, rpb, grid, s);
+}
+
+template <typename T>
+void bwd_typed(const RouteArgs& a, int tile, unsigned grid, size_t lds, hipStream_t s) {
+  if (a.E < kVec<T>) route_bwd_kernel<T, true><<<grid, kThreads, lds, s>>>(a, tile);
+  else route_bwd_kernel<T, false><<<grid, kThreads, lds, s>>>(a, tile);
 }
 
 size_t align256(size_t v) { return (v + 255) / 256 * 256; }
@@ -301,6 +409,7 @@ void launch_route(const RouteArgs& a, hipStream_t s) {
   if (a.elem == ELEM_F32) top_typed<float>(a, rpb, blocks, s);
   else if (a.elem == ELEM_BF16) top_typed<__bf16>(a, rpb, blocks, s);
   else top_typed<_Float16>(a, rpb, blocks, s);
+  if (a.N <= kPassRows && a.E <= kOneMaxE) return;
   route_scan_kernel<<<(a.E + 1 + kScanCols - 1) / kScanCols, kScanCols * kScanParts, 0, s>>>(a, (int)blocks);
   if (a.E <= 512) route_place_kernel<512><<<blocks, kThreads, 0, s>>>(a, rpb);
   else route_place_kernel<kRouteMaxE><<<blocks, kThreads, 0, s>>>(a, rpb);
@@ -310,9 +419,9 @@ void launch_route_bwd(const RouteArgs& a, hipStream_t s) {
   const int tile = 32;
   const unsigned grid = (unsigned)((a.N + tile - 1) / tile);
   const size_t lds = (size_t)(2 * tile * a.k + tile) * 4;
-  if (a.elem == ELEM_F32) route_bwd_kernel<float><<<grid, kThreads, lds, s>>>(a, tile);
-  else if (a.elem == ELEM_BF16) route_bwd_kernel<__bf16><<<grid, kThreads, lds, s>>>(a, tile);
-  else route_bwd_kernel<_Float16><<<grid, kThreads, lds, s>>>(a, tile);
+  if (a.elem == ELEM_F32) bwd_typed<float>(a, tile, grid, lds, s);
+  else if (a.elem == ELEM_BF16) bwd_typed<__bf16>(a, tile, grid, lds, s);
+  else bwd_typed<_Float16>(a, tile, grid, lds, s);
 }
 
 }  // namespace gx::layer

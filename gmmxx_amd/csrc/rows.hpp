@@ -15,33 +15,52 @@ __device__ __forceinline__ float to_f32(_Float16 v) { return (float)v; }
 template <typename T>
 constexpr int kVec = 16 / (int)sizeof(T);
 
-// V consecutive elements as fp32; elements at or past `valid` read as 0.  Whole
-// vectors are one 16-byte load whatever the row's alignment; the last, partial one
-// of an odd row is read element by element.
-template <typename T>
-__device__ __forceinline__ void load_row(const T* p, int valid, float (&v)[kVec<T>]) {
+// 16 bytes of a row of n elements, of which `valid` are left from p on, whatever the row's alignment: one load
+// without a branch, so that several are in flight together.  Near the row's end it takes the row's last 16
+// bytes instead, which keep16 moves to their place.  SHORT: n is less than a vector; element by element.
+template <bool SHORT, typename T>
+__device__ __forceinline__ uint4 fetch16(const T* p, int valid) {
   constexpr int V = kVec<T>;
-  if (valid >= V) {
-    union { uint4 u; T t[V]; } r;
-    r.u = ld16_any(p);
-#pragma unroll
-    for (int i = 0; i < V; ++i) v[i] = to_f32(r.t[i]);
-  } else {
-#pragma unroll
-    for (int i = 0; i < V; ++i) v[i] = i < valid ? to_f32(p[i]) : 0.f;
-  }
-}
-
-// The same as raw bytes; elements at or past `valid` are zeros.
-template <typename T>
-__device__ __forceinline__ uint4 load16(const T* p, int valid) {
-  constexpr int V = kVec<T>;
+  if constexpr (!SHORT) return ld16_any(valid >= V ? p : p + (valid - V));
   union { uint4 u; T t[V]; } r;
-  if (valid >= V) return ld16_any(p);
 #pragma unroll
   for (int i = 0; i < V; ++i) r.t[i] = i < valid ? p[i] : (T)0.f;
   return r.u;
 }
+
+// What fetch16 loaded, with zeros at elements at or past `valid`.
+template <bool SHORT, typename T>
+__device__ __forceinline__ uint4 keep16(uint4 u, int valid, int n) {
+  constexpr int V = kVec<T>;
+  if constexpr (SHORT) return valid > 0 ? u : make_uint4(0, 0, 0, 0);
+  if (n % V == 0) return valid > 0 ? u : make_uint4(0, 0, 0, 0);
+  if (valid >= V) return u;
+  const int bytes = valid > 0 ? (V - valid) * (int)sizeof(T) : 16, words = bytes >> 2;
+  const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+  uint32_t t[5];
+#pragma unroll
+  for (int i = 0; i < 5; ++i) {
+    t[i] = 0;
+#pragma unroll
+    for (int s = 0; s + i < 4; ++s) t[i] = words == s ? w[s + i] : t[i];
+  }
+  if constexpr (sizeof(T) == 2) {
+    const int bits = (bytes & 2) * 8;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) t[i] = __builtin_amdgcn_alignbit(t[i + 1], t[i], bits);
+  }
+  return make_uint4(t[0], t[1], t[2], t[3]);
+}
+
+// The elements of 16 bytes as fp32.
+template <typename T>
+__device__ __forceinline__ void unpack16(uint4 u, float (&v)[kVec<T>]) {
+  union { uint4 u; T t[kVec<T>]; } r;
+  r.u = u;
+#pragma unroll
+  for (int i = 0; i < kVec<T>; ++i) v[i] = to_f32(r.t[i]);
+}
+
 template <typename T>
 __device__ __forceinline__ void store16(T* p, int valid, uint4 v) {
   constexpr int V = kVec<T>;
@@ -56,7 +75,7 @@ __device__ __forceinline__ void store16(T* p, int valid, uint4 v) {
   }
 }
 
-// The reverse of load_row: rounds to T (nearest even) and stores the first `valid`.
+// Rounds to T (nearest even) and stores the first `valid`.
 template <typename T>
 __device__ __forceinline__ void store_row(T* p, int valid, const float (&v)[kVec<T>]) {
   constexpr int V = kVec<T>;
@@ -106,22 +125,26 @@ __device__ __forceinline__ float lanes_sum(float v) {
   return lanes_reduce<G>(v, [](float a, float b) { return a + b; });
 }
 
-// Sum over groups of G threads: lanes_sum within a wave, `red` (two slots of 16
-// floats, used in turn so that one barrier separates writers from readers) above it.
-template <int G>
-__device__ __forceinline__ float group_sum(float v, float (*red)[16], int& turn) {
-  if constexpr (G <= 64) {
-    return lanes_sum<G>(v);
-  } else {
-    v = lanes_sum<64>(v);
-    float* slot = red[turn & 1];
-    turn ^= 1;
-    if ((threadIdx.x & 63) == 0) slot[threadIdx.x >> 6] = v;
-    __syncthreads();
-    float s = 0.f;
+// Sums of N values over groups of G threads: lanes_sum within a wave, `red` (two slots of 16 waves' values, used
+// in turn so that one barrier separates writers from readers) above it.
+template <int G, int N>
+__device__ __forceinline__ void group_sums(float (&v)[N], float (*red)[16][N], int& turn) {
 #pragma unroll
-    for (int w = 0; w < G / 64; ++w) s += slot[w];
-    return s;
+  for (int i = 0; i < N; ++i) v[i] = lanes_sum<(G < 64 ? G : 64)>(v[i]);
+  if constexpr (G > 64) {
+    float(*slot)[N] = red[turn & 1];
+    turn ^= 1;
+    if ((threadIdx.x & 63) == 0) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) slot[threadIdx.x >> 6][i] = v[i];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      v[i] = 0.f;
+#pragma unroll
+      for (int w = 0; w < G / 64; ++w) v[i] += slot[w][i];
+    }
   }
 }
 
