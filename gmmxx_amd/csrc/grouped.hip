@@ -134,8 +134,12 @@ int parts_of(int64_t M, int64_t E, int64_t groups, int64_t want, int64_t least) 
   return (int)(s < 1 ? 1 : s < 65535 ? s : 65535);
 }
 
-// Parts of the weight gradient by tiles of 128, of which 512 run at once, and of db.
-int dw_parts(int64_t M, int64_t E, int64_t K, int64_t N) { return parts_of(M, E, E * tiles(K, 128) * tiles(N, 128), 512, 128); }
+// Parts of the weight gradient by tiles of 128, of which 512 run at once, and of db.  Twice as many workgroups
+// even out groups of uneven sizes: 100003 fp32 rows, 200 experts, 100 x 77 in 3 parts 111 us, in 6 parts 83 us
+// and 3 us more for their sums.
+int dw_parts(int64_t M, int64_t E, int64_t K, int64_t N, int size) {
+  return parts_of(M, E, E * tiles(K, 128) * tiles(N, 128), 1024, 256 / size);
+}
 int bias_parts(int64_t M, int64_t E, int64_t N) { return parts_of(M, E, E * tiles(N, 128), 2048, 128); }
 
 template <typename T>
@@ -148,7 +152,7 @@ void rows_typed(const GroupedArgs& a, hipStream_t s) {
 template <typename T>
 void dw_typed(GroupedArgs a, hipStream_t s) {
   const bool direct = dw_direct(a), larger = sizeof(T) == 2 && direct && dw_larger(a.E, a.K, a.Nn);
-  const int splits = larger ? 1 : dw_parts(a.M, a.E, a.K, a.Nn), bs = a.dbias ? bias_parts(a.M, a.E, a.Nn) : 1;
+  const int splits = larger ? 1 : dw_parts(a.M, a.E, a.K, a.Nn, sizeof(T)), bs = a.dbias ? bias_parts(a.M, a.E, a.Nn) : 1;
   a.bias_part = a.part + (splits > 1 ? (int64_t)splits * a.E * a.K * a.Nn : 0);
   launch_dw_tiles<T>(a, direct, larger, splits, s);
   dw_rest<T>(a, splits, bs, s);
@@ -157,7 +161,7 @@ void dw_typed(GroupedArgs a, hipStream_t s) {
 }  // namespace
 
 int64_t grouped_workspace_bytes(int64_t M, int64_t E, int64_t K, int64_t N) {
-  const int s = dw_parts(M, E, K, N), b = bias_parts(M, E, N);
+  const int s = dw_parts(M, E, K, N, 4), b = bias_parts(M, E, N);
   return ((s > 1 ? s * E * K * N : 0) + (b > 1 ? b * E * N : 0)) * (int64_t)sizeof(float);
 }
 

@@ -19,11 +19,19 @@ __device__ __forceinline__ int offset_at(const GroupedArgs& a, int e) {
   return (int)(v < 0 ? 0 : (v < a.M ? v : a.M));
 }
 
-// Row of x at position p, within x.
-__device__ __forceinline__ int64_t source_row(const GroupedArgs& a, int64_t p) {
-  int64_t src = a.rows ? a.rows[p] : p;
-  return src < 0 ? 0 : (src < a.Nx ? src : a.Nx - 1);
+// Rows of x at the positions at(0) .. at(N - 1), as read: in flight together (a wait for each would cost the
+// chain of them).  in_x() brings one into x.
+template <int N, typename F>
+__device__ __forceinline__ void source_rows(const GroupedArgs& a, int (&row)[N], F&& at) {
+  if (a.rows) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) row[i] = a.rows[at(i)];
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; ++i) row[i] = at(i);
+  }
 }
+__device__ __forceinline__ int in_x(const GroupedArgs& a, int row) { return min(max(row, 0), (int)a.Nx - 1); }
 
 template <int BM>
 __device__ __forceinline__ int tiles_of(int lo, int hi) {

@@ -24,7 +24,8 @@ constexpr int kChunk = 1024;     // reduction elements of x staged at a time
 template <typename T>
 __device__ __forceinline__ void stage(const GroupedArgs& a, int first, int rows, int k0, float4* xs) {
   const int r = threadIdx.x & 3, lane = threadIdx.x >> 2;
-  const T* x = static_cast<const T*>(a.x) + source_row(a, first + (r < rows ? r : 0)) * a.ldx + k0;
+  const int at = first + (r < rows ? r : 0);
+  const T* x = static_cast<const T*>(a.x) + in_x(a, a.rows ? a.rows[at] : at) * a.ldx + k0;
   const int most = min(kChunk, a.K - k0);
 #pragma unroll
   for (int i = 0; i < kChunk / (kThreads / 4); ++i) {

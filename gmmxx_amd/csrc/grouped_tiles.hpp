@@ -336,7 +336,8 @@ __global__ __launch_bounds__(64 * WP * WQ) void grouped_rows_kernel(GroupedArgs 
                             [&](int r) { return q0 + r < rows ? out + (int64_t)r * a.Nn : nullptr; });
     }
   };
-  auto source = [&](int i) { return source_row(a, first + min(Q::row(i), rows - 1)) * a.ldx; };
+  int src[Q::Loads];
+  source_rows(a, src, [&](int i) { return first + min(Q::row(i), rows - 1); });
   if constexpr (DIRECT) {
     const uint8_t *wb = reinterpret_cast<const uint8_t*>(w), *xb = reinterpret_cast<const uint8_t*>(x);
     const int64_t ld = a.wk * S;
@@ -344,7 +345,7 @@ __global__ __launch_bounds__(64 * WP * WQ) void grouped_rows_kernel(GroupedArgs 
     uint32_t poff[WKC ? P::Loads : 1];
     qoff_t qoff[Q::Loads];
 #pragma unroll
-    for (int i = 0; i < Q::Loads; ++i) qoff[i] = (qoff_t)(source(i) * S);
+    for (int i = 0; i < Q::Loads; ++i) qoff[i] = (qoff_t)(in_x(a, src[i]) * a.ldx * S);
     if constexpr (WKC) {
 #pragma unroll
       for (int i = 0; i < P::Loads; ++i) poff[i] = (uint32_t)min(n0 + P::row(i), a.Nn - 1) * (uint32_t)a.wn * S;
@@ -374,7 +375,7 @@ __global__ __launch_bounds__(64 * WP * WQ) void grouped_rows_kernel(GroupedArgs 
   } else {
     const T *pat[WKC ? P::Loads : 1], *qat[Q::Loads];
 #pragma unroll
-    for (int i = 0; i < Q::Loads; ++i) qat[i] = x + source(i) + qc;
+    for (int i = 0; i < Q::Loads; ++i) qat[i] = x + in_x(a, src[i]) * a.ldx + qc;
     if constexpr (WKC) {
 #pragma unroll
       for (int i = 0; i < P::Loads; ++i) pat[i] = w + min(n0 + P::row(i), a.Nn - 1) * a.wn + pc;
@@ -441,10 +442,7 @@ __global__ __launch_bounds__(64 * WP * WQ) void grouped_dw_kernel(GroupedArgs a,
                           [&](int r) { return d0 + q0 + r < a.K ? at + (int64_t)r * a.Nn : nullptr; });
   };
   int src[Q::Loads];      // rows of x, read a step ahead; past the last: the last
-  auto look = [&](int s) {
-#pragma unroll
-    for (int i = 0; i < Q::Loads; ++i) src[i] = (int)source_row(a, lo + min(s * BK + Q::row(i), n - 1));
-  };
+  auto look = [&](int s) { source_rows(a, src, [&](int i) { return lo + min(s * BK + Q::row(i), n - 1); }); };
   look(0);
   if constexpr (DIRECT) {
     const int64_t ld = a.lddy * S;
@@ -459,7 +457,7 @@ __global__ __launch_bounds__(64 * WP * WQ) void grouped_dw_kernel(GroupedArgs a,
       const int k0 = s * BK;
       qoff_t qoff[Q::Loads];
 #pragma unroll
-      for (int i = 0; i < Q::Loads; ++i) qoff[i] = ((qoff_t)src[i] * (qoff_t)a.ldx + qcol) * S;
+      for (int i = 0; i < Q::Loads; ++i) qoff[i] = ((qoff_t)in_x(a, src[i]) * (qoff_t)a.ldx + qcol) * S;
       look(s + 1);
       const uint8_t* ds = dy + k0 * ld;
 #pragma unroll
@@ -477,7 +475,7 @@ __global__ __launch_bounds__(64 * WP * WQ) void grouped_dw_kernel(GroupedArgs a,
 #pragma unroll
       for (int i = 0; i < P::Loads; ++i) vp[i] = fetch16<SHORT>(dy + min(s * BK + P::row(i), n - 1) * a.lddy, a.Nn - fc);
 #pragma unroll
-      for (int i = 0; i < Q::Loads; ++i) vq[i] = fetch16<SHORT>(x + src[i] * a.ldx, a.K - dc);
+      for (int i = 0; i < Q::Loads; ++i) vq[i] = fetch16<SHORT>(x + in_x(a, src[i]) * a.ldx, a.K - dc);
       look(s + 1);
     };
     load(0);

@@ -4,8 +4,8 @@
 // and with h = (x - μ) ρ, g = dy·w:
 //   dx = ρ (g - mean g - h mean(g h)),  dw = Σ_rows dy·h,  db = Σ_rows dy.
 //
-// A group of G threads holds a row in registers (up to 16 elements a thread, 32 and
-// 64 for the widest rows), so x is read once and the mean is taken out before the
+// A group of G threads holds a row in registers (up to 16 elements a thread, 32 above
+// 4096 columns and 64, partly spilled, above 16384), so x is read once and the mean is taken out before the
 // squares are summed: rows whose mean is large beside their spread lose nothing.
 // Everything is fp32; the one rounding is the store.  G is the smallest group that
 // holds the row, so narrow rows share a wave.  Groups stride over the rows and keep
@@ -230,6 +230,7 @@ void with_group(int D, F&& f) {
   else if (D <= 64 * 16) f.template operator()<64, N16, false>();
   else if (D <= 256 * 16) f.template operator()<256, N16, false>();
   else if (D <= 256 * 32) f.template operator()<256, 2 * N16, false>();
+  else if (D <= 512 * 32) f.template operator()<512, 2 * N16, false>();
   else f.template operator()<1024, 4 * N16, false>();
 }
 
