@@ -3,7 +3,9 @@
     python -m gmmxx_amd.build          # or: from gmmxx_amd.build import build; build()
 
 Each translation unit is compiled separately (in parallel) and linked into a
-shared library next to this file, where ``gmmxx_amd._hip`` loads it.
+shared library next to this file, where ``gmmxx_amd._hip`` loads it.  The
+autograd functions of ``gmmxx_amd.experts`` are a Python extension beside it,
+``_autograd.so``, compiled against the installed torch.
 """
 
 from __future__ import annotations
@@ -12,6 +14,7 @@ import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 from concurrent.futures import ThreadPoolExecutor
 
 PKG_DIR = os.path.dirname(os.path.abspath(__file__))
@@ -19,6 +22,7 @@ ROOT = os.path.dirname(PKG_DIR)
 CSRC = os.path.join(PKG_DIR, "csrc")
 BUILD_DIR = os.path.join(PKG_DIR, "_build")
 LIB_PATH = os.path.join(PKG_DIR, "libgmmxx_hip.so")
+AUTOGRAD_PATH = os.path.join(PKG_DIR, "_autograd.so")
 SOURCES = ("em_tile.hip", "em_sph_bf16.hip", "em_fused.hip", "em_coop.hip", "em_one.hip", "em_label.hip", "em_full_wide.hip", "em_full_stats.hip", "em_full_infer.hip",
            "params.hip",
            "kmeans.hip", "abi.hip",
@@ -57,11 +61,33 @@ def _compile(src: str) -> str:
     return obj
 
 
+def _build_autograd() -> None:
+    """Compile csrc/autograd.cpp (host code only) into _autograd.so."""
+    import torch
+    from torch.utils import cpp_extension
+
+    tmp = AUTOGRAD_PATH + ".tmp"
+    cmd = [shutil.which("g++") or "c++", "-O2", "-std=c++17", "-fPIC", "-shared", "-D__HIP_PLATFORM_AMD__=1",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", "-I", os.path.join(ROOT, "include"),
+           *(a for p in cpp_extension.include_paths() for a in ("-isystem", p)),
+           "-isystem", os.path.join(os.environ.get("ROCM_PATH", "/opt/rocm"), "include"),
+           "-isystem", sysconfig.get_paths()["include"], os.path.join(CSRC, "autograd.cpp"), "-o", tmp,
+           *("-L" + p for p in cpp_extension.library_paths()),
+           "-lc10", "-lc10_hip", "-ltorch_cpu", "-ltorch", "-ltorch_python"]
+    res = subprocess.run(cmd, capture_output=True, text=True)
+    if res.returncode != 0:
+        raise RuntimeError(f"g++ failed on autograd.cpp:\n{res.stderr}")
+    os.replace(tmp, AUTOGRAD_PATH)
+
+
 def build(verbose: bool = False) -> str:
-    """Compile every HIP translation unit and link libgmmxx_hip.so; returns its path."""
+    """Compile every HIP translation unit and link libgmmxx_hip.so, and the autograd
+    extension; returns the library's path."""
     os.makedirs(BUILD_DIR, exist_ok=True)
-    with ThreadPoolExecutor(max_workers=len(SOURCES)) as ex:
+    with ThreadPoolExecutor(max_workers=len(SOURCES) + 1) as ex:
+        extension = ex.submit(_build_autograd)
         objs = list(ex.map(_compile, SOURCES))
+        extension.result()
     tmp = LIB_PATH + ".tmp"
     cmd = [_hipcc(), f"--offload-arch={ARCH}", "-shared", "-fPIC", *objs, "-o", tmp]
     res = subprocess.run(cmd, capture_output=True, text=True)
@@ -69,7 +95,7 @@ def build(verbose: bool = False) -> str:
         raise RuntimeError(f"link failed:\n{res.stderr}")
     os.replace(tmp, LIB_PATH)
     if verbose:
-        print(f"built {LIB_PATH}")
+        print(f"built {LIB_PATH} and {AUTOGRAD_PATH}")
     return LIB_PATH
 
 
