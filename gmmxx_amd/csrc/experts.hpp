@@ -11,7 +11,7 @@ namespace gx::layer {
 enum Elem { ELEM_F32 = 0, ELEM_BF16 = 1, ELEM_F16 = 2 };   // enum gmmxx_dtype
 
 constexpr int kNormMaxD = 65536;
-constexpr int kNormMaxBlocks = 1024;     // row slices of the backward pass
+constexpr int kNormMaxBlocks = 512;     // row slices of the backward pass
 struct NormArgs {
   const void* x;  int64_t ldx;           // rows of D elements, row stride in elements
   const void* dy; int64_t lddy;

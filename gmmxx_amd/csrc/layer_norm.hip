@@ -5,7 +5,7 @@
 //   dx = ρ (g - mean g - h mean(g h)),  dw = Σ_rows dy·h,  db = Σ_rows dy.
 //
 // A group of G threads holds a row in registers (up to 16 elements a thread, 32 above
-// 4096 columns and 64, partly spilled, above 16384), so x is read once and the mean is taken out before the
+// 16384 columns and 64 above 32768, where part of it spills), so x is read once and the mean is taken out before the
 // squares are summed: rows whose mean is large beside their spread lose nothing.
 // Everything is fp32; the one rounding is the store.  G is the smallest group that
 // holds the row, so narrow rows share a wave.  Groups stride over the rows and keep
@@ -23,7 +23,7 @@ namespace gx::layer {
 namespace {
 
 constexpr int kNormThreads = 256;
-constexpr int kFwdMaxBlocks = 2048;
+constexpr int kFwdMaxBlocks = 1024;
 
 template <typename T, typename WT, int G, int NV, bool SHORT>
 struct Norm {
@@ -42,16 +42,31 @@ struct Norm {
 #pragma unroll
     for (int i = 0; i < NV; ++i) unpack16<T>(keep16<SHORT, T>(u[i], D - col(i, lane), D), v[i]);
   }
+  // This thread's columns of w or b, or `fill` where there is none.
   __device__ static __forceinline__ void load_param(const void* p, int D, int lane, float fill, float (&v)[NV][V]) {
-    const WT* w = static_cast<const WT*>(p);
+    if (!p) {
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
+      for (int i = 0; i < NV; ++i)
 #pragma unroll
-      for (int j = 0; j < V; ++j) {
-        const int c = col(i, lane) + j;
-        v[i][j] = c < D ? (w ? to_f32(w[c]) : fill) : 0.f;
-      }
+        for (int j = 0; j < V; ++j) v[i][j] = fill;
+      return;
     }
+    constexpr int H = V / kVec<WT>, W = kVec<WT>;      // vectors of w for one of x
+    const WT* w = static_cast<const WT*>(p);
+    uint4 u[NV][H];
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+#pragma unroll
+      for (int h = 0; h < H; ++h) u[i][h] = fetch16<SHORT>(w + col(i, lane) + h * W, D - col(i, lane) - h * W);
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+#pragma unroll
+      for (int h = 0; h < H; ++h) {
+        float e[W];
+        unpack16<WT>(keep16<SHORT, WT>(u[i][h], D - col(i, lane) - h * W, D), e);
+#pragma unroll
+        for (int j = 0; j < W; ++j) v[i][h * W + j] = e[j];
+      }
   }
 };
 
@@ -220,7 +235,8 @@ __global__ __launch_bounds__(kSumCols* kSumRows) void norm_sum_kernel(NormArgs a
 }
 
 // Calls f.template operator()<G, NV, SHORT>() for the smallest group that holds a row of D.
-template <typename T, typename F>
+// (the backward pass of 1024 threads would spill: 4096 x 16384 bf16 293 us by them, 202 us by 512)
+template <typename T, bool BWD, typename F>
 void with_group(int D, F&& f) {
   constexpr int N16 = 16 / kVec<T>;    // vectors of 16 elements
   if (D < kVec<T>) f.template operator()<8, N16, true>();
@@ -229,8 +245,9 @@ void with_group(int D, F&& f) {
   else if (D <= 32 * 16) f.template operator()<32, N16, false>();
   else if (D <= 64 * 16) f.template operator()<64, N16, false>();
   else if (D <= 256 * 16) f.template operator()<256, N16, false>();
-  else if (D <= 256 * 32) f.template operator()<256, 2 * N16, false>();
-  else if (D <= 512 * 32) f.template operator()<512, 2 * N16, false>();
+  else if (D <= 512 * 16) f.template operator()<512, N16, false>();
+  else if (D <= 1024 * 16) f.template operator()<BWD ? 512 : 1024, BWD ? 2 * N16 : N16, false>();
+  else if (D <= 1024 * 32) f.template operator()<1024, 2 * N16, false>();
   else f.template operator()<1024, 4 * N16, false>();
 }
 
@@ -253,7 +270,7 @@ struct FwdOp {
   const NormArgs& a; hipStream_t s;
   template <typename T, typename WT> void operator()() {
     Go<T, WT> go{a, s};
-    with_group<T>(a.D, go);
+    with_group<T, false>(a.D, go);
   }
   template <typename T, typename WT> struct Go {
     const NormArgs& a; hipStream_t s;
@@ -270,7 +287,7 @@ struct BwdOp {
   const NormArgs& a; hipStream_t s; int blocks;
   template <typename T, typename WT> void operator()() {
     Go<T, WT> go{a, s, blocks};
-    with_group<T>(a.D, go);
+    with_group<T, true>(a.D, go);
     if (a.part) norm_sum_kernel<WT><<<(2 * a.D + kSumCols - 1) / kSumCols, kSumCols * kSumRows, 0, s>>>(a, blocks);
   }
   template <typename T, typename WT> struct Go {
