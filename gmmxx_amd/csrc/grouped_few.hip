@@ -184,10 +184,10 @@ void few(const GroupedArgs& a, hipStream_t s) {
 
 // Up to which number of positions this beats the tiles.  Whole 16-bit chunks: 8 (1024 x 2048 matrices, 16
 // experts: 9.8 and 12.7 us at 8 positions, 28 and 16 us at 32).  Other 16-bit shapes: two an expert (100 x 77:
-// 7.2 and 10.5 us at 32).  fp32, whose tiles take sixteen times as long: two an expert or 32 (1024 x 2048, 16
-// experts: 39 and 71 us at 32 positions, 98 and 71 us at 128; 64 experts: 173 and 255 us at 128).
+// 7.2 and 10.5 us at 32).  fp32: one an expert or 32 (256 x 512, 16 experts: 6 and 14 us at 32 positions; 64
+// experts, two an expert: 22 and 14.5 us; 1024 x 2048 likewise: 168 and 87 us).
 bool grouped_few_better(const GroupedArgs& a) {
-  if (a.elem == ELEM_F32) return a.M <= (a.E > 16 ? 2 * a.E : 32);
+  if (a.elem == ELEM_F32) return a.M <= (a.E > 32 ? a.E : 32);
   return a.M <= 8 || (!grouped_direct(a) && a.M <= 2 * (int64_t)a.E);
 }
 

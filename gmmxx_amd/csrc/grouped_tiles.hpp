@@ -117,7 +117,7 @@ struct Share {
   static constexpr int Loads = R * 128 / (THREADS * 16);
   static constexpr int PerRow = KC ? 8 : R / V;               // chunks of a row of the tile
   static constexpr int Step = THREADS / PerRow;               // tile rows between a thread's loads
-  static_assert(Loads >= 1 && Step % 8 == 0, "a thread's rows agree modulo 8");
+  static_assert(Loads >= 1 && (Step % 8 == 0 || (!KC && sizeof(T) == 4)), "a thread's rows agree modulo 8");
   // Tile row of load i: a row of the operand (KC) or a reduction row.
   __device__ static __forceinline__ int row(int i) { return threadIdx.x / PerRow + i * Step; }
   // First element of the thread's chunk along the tile row.
@@ -182,8 +182,8 @@ struct Core {
   // One barrier a step, before the last of its products: by then every fragment of the step is in
   // registers, so its buffer takes the loads of the step after next, and the next step's first fragments
   // are read under those last products.  The last step's fragments are masked.
-  // Then store(piece) is called with 1/8 (1/4) of the stages' LDS for each of 8 (4) waves: room for the wave's
-  // part of the tile in 16 bits.
+  // Then store(piece) is called with a piece of the stages' LDS for each wave: room for the wave's part of the
+  // tile in 16 bits (256 x 32: in fp32).
   template <typename F, typename G>
   __device__ static __forceinline__ void run(int total, F&& fill, int wave, int lane, f32x16 (&acc)[TP][TQ],
                                              G&& store) {
@@ -230,8 +230,12 @@ struct Core {
       __builtin_amdgcn_sched_barrier(0);
     }
     __syncthreads();
-    static_assert(BP == BQ, "every array holds two waves' results");
-    store((wave & 4 ? (wave & 2 ? qb : pb) : (wave & 2 ? qa : pa)) + (wave & 1) * (BP * 64));
+    if constexpr (BP == BQ) {      // every array holds two waves' results
+      store((wave & 4 ? (wave & 2 ? qb : pb) : (wave & 2 ? qa : pa)) + (wave & 1) * (BP * 64));
+    } else {
+      static_assert(BP == 256 && WP == 4 && WQ == 1 && BQ == 32, "pa holds all waves' results");
+      store(pa + wave * (BP * 32));
+    }
   }
 };
 
@@ -244,7 +248,7 @@ __device__ __forceinline__ void store_tile(uint8_t* piece, const f32x16 (&acc)[2
                                            R&& row) {
   constexpr int Bytes = 64 * sizeof(O), Chunks = Bytes / 16;       // of a row
   constexpr int Rows = 64 / Chunks;                                // rows that the wave writes at a time
-  constexpr int Group = sizeof(O) == 2 ? TQ : TQ / 2;              // 32-row tiles that the piece holds
+  constexpr int Group = sizeof(O) == 2 || TQ == 1 ? TQ : TQ / 2;   // 32-row tiles that the piece holds
 #pragma unroll
   for (int j0 = 0; j0 < TQ; j0 += Group) {
 #pragma unroll
@@ -496,23 +500,37 @@ __global__ __launch_bounds__(64 * WP * WQ) void grouped_dw_kernel(GroupedArgs a,
 template <typename T>
 bool wide(const GroupedArgs& a) { return (a.Nx * a.ldx + a.K) * (int64_t)sizeof(T) >= (int64_t(1) << 32); }
 
-template <typename T, bool WKC, bool DIRECT, bool WIDE, int B, int WP, int WQ, bool SHORT = false>
+template <typename T, bool WKC, bool DIRECT, bool WIDE, int BP, int BQ, int WP, int WQ, bool SHORT = false>
 void rows_tiled(const GroupedArgs& a, hipStream_t s) {
-  const int ntiles = (a.Nn + B - 1) / B;
-  const int64_t grid = (a.M / B + a.E + 1) * ntiles;
-  grouped_rows_kernel<T, WKC, DIRECT, WIDE, B, B, WP, WQ, SHORT><<<(unsigned)grid, 64 * WP * WQ, 0, s>>>(a, ntiles);
+  const int ntiles = (a.Nn + BP - 1) / BP;
+  const int64_t grid = (a.M / BQ + a.E + 1) * ntiles;
+  grouped_rows_kernel<T, WKC, DIRECT, WIDE, BP, BQ, WP, WQ, SHORT><<<(unsigned)grid, 64 * WP * WQ, 0, s>>>(a, ntiles);
+}
+
+// fp32 tiles of 256 columns by 32 rows where the groups are small: whether they take less matrix work than tiles
+// of 128 (a group's last row tile is half full on average).  1024 x 2048 matrices, 64 experts: 95 us and 256 us
+// by tiles of 128 at 256 positions (537 MB of weights, 5.6 TB/s), 200 and 260 us at 4096; 16 experts, where both
+// leave CUs idle: 42 and 71 us at 128 positions.
+inline bool small_groups(const GroupedArgs& a) {
+  return (a.M / 32.0 + 0.5 * a.E) * ((a.Nn + 255) / 256) * 0.5 < (a.M / 128.0 + 0.5 * a.E) * ((a.Nn + 127) / 128);
 }
 
 template <typename T, bool WKC>
 void rows_by(const GroupedArgs& a, bool direct, bool larger, hipStream_t s) {
   if constexpr (sizeof(T) == 2) {
     if (direct && larger)
-      return wide<T>(a) ? rows_tiled<T, WKC, true, true, 256, 4, 2>(a, s) : rows_tiled<T, WKC, true, false, 256, 4, 2>(a, s);
+      return wide<T>(a) ? rows_tiled<T, WKC, true, true, 256, 256, 4, 2>(a, s)
+                        : rows_tiled<T, WKC, true, false, 256, 256, 4, 2>(a, s);
+  } else if (small_groups(a) && a.K >= kVec<T> && a.Nn >= kVec<T>) {
+    if (!direct) rows_tiled<T, WKC, false, true, 256, 32, 4, 1>(a, s);
+    else if (wide<T>(a)) rows_tiled<T, WKC, true, true, 256, 32, 4, 1>(a, s);
+    else rows_tiled<T, WKC, true, false, 256, 32, 4, 1>(a, s);
+    return;
   }
-  if (a.K < kVec<T> || a.Nn < kVec<T>) rows_tiled<T, WKC, false, true, 128, 2, 2, true>(a, s);
-  else if (!direct) rows_tiled<T, WKC, false, true, 128, 2, 2>(a, s);
-  else if (wide<T>(a)) rows_tiled<T, WKC, true, true, 128, 2, 2>(a, s);
-  else rows_tiled<T, WKC, true, false, 128, 2, 2>(a, s);
+  if (a.K < kVec<T> || a.Nn < kVec<T>) rows_tiled<T, WKC, false, true, 128, 128, 2, 2, true>(a, s);
+  else if (!direct) rows_tiled<T, WKC, false, true, 128, 128, 2, 2>(a, s);
+  else if (wide<T>(a)) rows_tiled<T, WKC, true, true, 128, 128, 2, 2>(a, s);
+  else rows_tiled<T, WKC, true, false, 128, 128, 2, 2>(a, s);
 }
 
 template <typename T, bool DIRECT, bool WIDE, bool SPLIT, int B, int WP, int WQ, bool SHORT = false>
