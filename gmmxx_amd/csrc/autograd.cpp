@@ -281,7 +281,7 @@ struct Grouped : torch::autograd::Function<Grouped> {
       dx = combine_forward(parts, Tensor(), slots, offsets, x.scalar_type());
     }
     if (need_w || need_b) {
-      dw = m ? at::empty({e, d, f}, x.options()) : at::zeros({e, d, f}, x.options());
+      if (need_w) dw = m ? at::empty({e, d, f}, x.options()) : at::zeros({e, d, f}, x.options());
       if (need_b) db = m ? at::empty({e, f}, x.options()) : at::zeros({e, f}, x.options());
       if (m) {
         On on(x);
@@ -292,7 +292,6 @@ struct Grouped : torch::autograd::Function<Grouped> {
                                       ptr(ws), need, on.stream()),
               "grouped_weight_grad");
       }
-      if (!need_w) dw = Tensor();
     }
     return once({dx, dw, db, Tensor(), Tensor(), Tensor()});
   }

@@ -187,7 +187,7 @@ int gmmxx_hip_grouped_weight_grad(int elem, int64_t M, int64_t Nx, int64_t E, in
                                   int64_t workspace_bytes, void* stream) {
   if (int rc = check_grouped(elem, M, Nx, E, K, N, offset_bits)) return rc;
   if (M == 0) return GMMXX_OK;
-  if (!x || !dy || !offsets || !dw) return invalid("NULL buffer");
+  if (!x || !dy || !offsets || (!dw && !dbias)) return invalid("NULL buffer");
   if (ldx < 0 || lddy < 0) return invalid("strides must be non-negative");
   if (!rows && Nx < M) return invalid("x has fewer rows than there are positions");
   if (const int64_t need = gmmxx_hip_grouped_workspace_bytes(M, E, K, N))

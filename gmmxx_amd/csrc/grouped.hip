@@ -152,9 +152,9 @@ void rows_typed(const GroupedArgs& a, hipStream_t s) {
 template <typename T>
 void dw_typed(GroupedArgs a, hipStream_t s) {
   const bool direct = dw_direct(a), larger = sizeof(T) == 2 && direct && dw_larger(a.E, a.K, a.Nn);
-  const int splits = larger ? 1 : dw_parts(a.M, a.E, a.K, a.Nn, sizeof(T)), bs = a.dbias ? bias_parts(a.M, a.E, a.Nn) : 1;
+  const int splits = larger || !a.out ? 1 : dw_parts(a.M, a.E, a.K, a.Nn, sizeof(T)), bs = a.dbias ? bias_parts(a.M, a.E, a.Nn) : 1;
   a.bias_part = a.part + (splits > 1 ? (int64_t)splits * a.E * a.K * a.Nn : 0);
-  launch_dw_tiles<T>(a, direct, larger, splits, s);
+  if (a.out) launch_dw_tiles<T>(a, direct, larger, splits, s);
   dw_rest<T>(a, splits, bs, s);
 }
 

@@ -347,14 +347,14 @@ int gmmxx_hip_route_backward(int elem, int64_t N, int64_t E, int64_t k, int reno
  * e we + k wk + n wn with wk or wn 1; bias (E, N) or NULL; offsets (E + 1) of 32 or 64
  * bits (offset_bits), ascending from 0 to at most M; out (M, N), of out_elem (elem or
  * GMMXX_F32).  E <= 4096, M < 2^30.  Offsets and rows out of range are taken as the
- * nearest valid ones. */
+ * nearest valid ones; where offsets descend, some rows of out may stay unwritten. */
 int gmmxx_hip_grouped_matmul(int elem, int64_t M, int64_t Nx, int64_t E, int64_t K, int64_t N, const void* x,
                              int64_t ldx, const int32_t* rows, const void* w, int64_t we, int64_t wk, int64_t wn,
                              const void* bias, const void* offsets, int offset_bits, void* out, int out_elem,
                              void* stream);
 
-/* The weight's gradient dw[e] = sum over group e of x[rows[p]]^T dy[p] (E, K, N) and,
- * unless dbias is NULL, the bias's (E, N); an empty group's are zeros.  The workspace
+/* The weight's gradient dw[e] = sum over group e of x[rows[p]]^T dy[p] (E, K, N) and the
+ * bias's (E, N); one of them may be NULL; an empty group's are zeros.  The workspace
  * takes gmmxx_hip_grouped_workspace_bytes. */
 int64_t gmmxx_hip_grouped_workspace_bytes(int64_t M, int64_t E, int64_t K, int64_t N);
 int gmmxx_hip_grouped_weight_grad(int elem, int64_t M, int64_t Nx, int64_t E, int64_t K, int64_t N, const void* x,
