@@ -225,8 +225,10 @@ struct Core {
     for (int kk = 0; kk < KK; ++kk) {
       if (kk + 1 < KK) f[(kk + 1) & 1].read(p, q, rp, rq, kk + 1);
       __builtin_amdgcn_sched_barrier(0);
-      f[kk & 1].mask(left - 2 * V * kk);
-      f[kk & 1].multiply(acc);
+      if (total - last * BK > 2 * V * kk) {
+        f[kk & 1].mask(left - 2 * V * kk);
+        f[kk & 1].multiply(acc);
+      }
       __builtin_amdgcn_sched_barrier(0);
     }
     __syncthreads();

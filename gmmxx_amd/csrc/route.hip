@@ -35,11 +35,13 @@ int64_t block_rows(int64_t N) {
   return r;
 }
 
-// exp(x) for x <= 0 by the hardware's power of two, with the rounding of x log2(e) put back in first order.
+// exp(x) for x <= 0, 0 for NaN: by the hardware's power of two, with the rounding of x log2(e) put back in first
+// order.
 __device__ __forceinline__ float exp_below(float x) {
-  const float y = fmaxf(x * kLog2e, -150.f);      // (2^-150 is 0)
+  x = fmaxf(x, -110.f);                   // (exp(-110) is 0; finite, so is what follows)
+  const float y = x * kLog2e;
   const float lost = fmaf(x, 1.925963033500e-8f, fmaf(x, kLog2e, -y));      // (log2(e) = kLog2e + 1.926e-8)
-  return y > -150.f ? fast_exp2(y) * fmaf(lost, kLn2, 1.f) : 0.f;
+  return fast_exp2(y) * fmaf(lost, kLn2, 1.f);
 }
 
 // The weight of score v beside the row's largest m (v <= m): 1 for each of several +inf.
@@ -100,7 +102,7 @@ __device__ __forceinline__ void choose_rows(const RouteArgs& a, int64_t base, in
 #pragma unroll
         for (int i = 0; i < NV; ++i)
 #pragma unroll
-          for (int q = 0; q < VV; ++q) sum += v[i][q] > kNone ? exp_below(score_of(v[i][q]) - m) : 0.f;
+          for (int q = 0; q < VV; ++q) sum += exp_below(score_of(v[i][q]) - m);      // (no candidate: -inf or NaN)
       } else {      // of +inf each weighs 1
 #pragma unroll
         for (int i = 0; i < NV; ++i)
