@@ -3,9 +3,11 @@
 //
 // The backward pass of a Python autograd function takes the interpreter's lock on the
 // engine's own thread; at small sizes that and the interpreter cost several times what
-// the kernels do.  Here both directions run without the interpreter.  The entry points
-// are those of the library that the package loaded: their addresses are handed over
-// once (bind), so there is one library whatever its path.
+// the kernels do: the norm of one row takes 6 us a call where it took 11, of 100003 x
+// 100 with its gradients 70 us where it took 118 (46 us of them kernels).  Here both
+// directions run without the interpreter.  The entry points are those of the library
+// that the package loaded: their addresses are handed over once (bind), so there is one
+// library whatever its path.
 //
 // Arguments have been checked by the caller (gmmxx_amd/experts.py): matrices with
 // adjacent row elements, matching shapes, types and devices.
