@@ -16,7 +16,7 @@
 // Integer counts do not depend on the order of the additions.
 //
 // The choice is bound by instructions (see choose_rows), the gradient by bytes, the
-// rest by waits.  100000 x 500 fp32, 4 of all: top 82 us (the scores at 2.4 TB/s), scan
+// rest by waits.  100000 x 500 fp32, 4 of all: top 76 us (the scores at 2.6 TB/s), scan
 // 13 us, place 10 us, gradient 79 us (5.1 TB/s).  65537 x 64, 8 of 64: 13, 7, 7 and
 // 10 us.  Three rows of 64 in one launch: 4.4 us.
 
@@ -70,13 +70,16 @@ __device__ __forceinline__ int lanes_reduce_int(int v, F&& op) {
 
 // The choices of up to kPassRows rows, to LDS.  G lanes share a row, NV vectors of its scores each: vector i of
 // lane l holds the scores from (i G + l) kVec on, as integers in their order.  Each round takes the group's
-// largest remaining score, then the lowest index that has it.  About 5 instructions a held score and round, and
-// 14 for its exponential where all candidates count: 100000 x 500 scores of 4 rounds take 37 million of a wave,
-// 60 us of what the card issues.  So G is the smallest that holds the row in 32 scores a lane (64 at the most
-// experts): what lanes exchange is the smaller part.
+// largest remaining score, then the lowest index that has it.  With few rows to a wave (G from 16 on) a round
+// passes over the vectors in which no row of the wave has its score: 134217 x 500, 4 each 93 us by it and 98 us
+// without, 16777 x 4000, 8 each 201 and 252 us, but 200000 x 64, 8 each 59 and 57 us.  About 5 instructions a
+// held score and round where nothing is passed over, and 14 for its exponential where all candidates count:
+// 100000 x 500, 4 of all take 30 million of a wave, 48 us of what the card issues.  So G is the smallest that
+// holds the row in 32 scores a lane (64 at the most experts): what lanes exchange is the smaller part.
 template <typename T, int G, int NV, bool SHORT>
 __device__ __forceinline__ void choose_rows(const RouteArgs& a, int64_t base, int rows, int* sel, float* wsel) {
   constexpr int VV = kVec<T>, R = kThreads / G;
+  constexpr bool kSkip = G >= 16;
   const int lane = threadIdx.x % G, sub = threadIdx.x / G;
   const auto larger = [](int p, int q) { return p > q ? p : q; };
   const auto smaller = [](int p, int q) { return p < q ? p : q; };
@@ -96,11 +99,14 @@ __device__ __forceinline__ void choose_rows(const RouteArgs& a, int64_t base, in
 #pragma unroll
       for (int j = 0; j < VV; ++j) v[i][j] = s[j] == s[j] && c + j < a.E ? key_of(s[j]) : INT32_MIN;
     }
-    int best = INT32_MIN;
+    int top[NV], best = INT32_MIN;              // of each vector, and of the row
 #pragma unroll
-    for (int i = 0; i < NV; ++i)
+    for (int i = 0; i < NV; ++i) {
+      top[i] = INT32_MIN;
 #pragma unroll
-      for (int q = 0; q < VV; ++q) best = larger(best, v[i][q]);
+      for (int q = 0; q < VV; ++q) top[i] = larger(top[i], v[i][q]);
+      best = larger(best, top[i]);
+    }
     best = lanes_reduce_int<G>(best, larger);
     const float m = best > kNone ? score_of(best) : -INFINITY;
     float sum = 0.f;
@@ -119,29 +125,36 @@ __device__ __forceinline__ void choose_rows(const RouteArgs& a, int64_t base, in
       sum = lanes_sum<G>(sum);
     }
     float chosen = 0.f;
+    int mine = 0;                               // the last choice, as this lane's score 0 would be 0
     for (int j = 0; j < a.k; ++j) {
       if (j > 0) {
         best = INT32_MIN;
 #pragma unroll
-        for (int i = 0; i < NV; ++i)
+        for (int i = 0; i < NV; ++i) {
+          if (!kSkip || __any((unsigned)(mine - i * G * VV) < (unsigned)VV)) {
+            top[i] = INT32_MIN;
 #pragma unroll
-          for (int q = 0; q < VV; ++q) best = larger(best, v[i][q]);
+            for (int q = 0; q < VV; ++q) {
+              v[i][q] = mine == i * G * VV + q ? INT32_MIN : v[i][q];
+              top[i] = larger(top[i], v[i][q]);
+            }
+          }
+          best = larger(best, top[i]);
+        }
         best = lanes_reduce_int<G>(best, larger);
       }
       int at = INT32_MAX;
 #pragma unroll
       for (int i = NV - 1; i >= 0; --i)
+        if (!kSkip || __any(top[i] == best)) {
 #pragma unroll
-        for (int q = VV - 1; q >= 0; --q) at = v[i][q] == best ? i * G * VV + q : at;
+          for (int q = VV - 1; q >= 0; --q) at = v[i][q] == best ? i * G * VV + q : at;
+        }
       at = lanes_reduce_int<G>(at == INT32_MAX ? at : at + lane * VV, smaller);
       const bool none = best <= kNone;
       const float w = none ? 0.f : weight_of(score_of(best), m);
       chosen += w;
-      const int mine = at - lane * VV;
-#pragma unroll
-      for (int i = 0; i < NV; ++i)
-#pragma unroll
-        for (int q = 0; q < VV; ++q) v[i][q] = mine == i * G * VV + q ? INT32_MIN : v[i][q];
+      mine = at - lane * VV;
       if (lane == 0 && there) {
         sel[r * a.k + j] = none ? -1 : at;
         wsel[r * a.k + j] = w;
