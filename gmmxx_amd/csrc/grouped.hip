@@ -16,7 +16,7 @@
 // after its last product.  One bf16 product of 8192 x 8192 x 8192: 920 us, 1.19 PFLOP/s
 // (fp32 143 TFLOP/s).  32768 positions of 32 uneven groups, 1024 x 2048 bf16: forward
 // 193 us, for x 193 us, for W 183 us (137 GFLOP each, 710 - 750 TFLOP/s: about 1150 tiles
-// are 4.5 for each CU), db 28 us.  100003 fp32 rows of 200 groups, 100 x 77: 67, 53, 85
+// are 4.5 for each CU), db 28 us.  100003 fp32 rows of 200 groups, 100 x 77: 62, 48, 83
 // and 12 us.
 
 #include <math.h>

@@ -57,58 +57,79 @@ __device__ __forceinline__ int xcd_tile(int id, int total) {
   return x * per + (x < rest ? x : rest) + id / 8;
 }
 
+// op over lanes 0 .. l in lane l, for values that are not negative (0 changes nothing): within rows of 16 lanes,
+// then across them.
+template <typename F>
+__device__ __forceinline__ int lanes_scan(int v, F&& op) {
+  v = op(v, __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, false));      // shifted by 1, 2, 4 and 8 lanes
+  v = op(v, __builtin_amdgcn_update_dpp(0, v, 0x112, 0xF, 0xF, false));
+  v = op(v, __builtin_amdgcn_update_dpp(0, v, 0x114, 0xF, 0xF, false));
+  v = op(v, __builtin_amdgcn_update_dpp(0, v, 0x118, 0xF, 0xF, false));
+  v = op(v, __builtin_amdgcn_update_dpp(0, v, 0x142, 0xA, 0xF, false));      // lane 15 to rows 1 and 3
+  return op(v, __builtin_amdgcn_update_dpp(0, v, 0x143, 0xC, 0xF, false));   // lane 31 to rows 2 and 3
+}
+
 // The tile of workgroup `id`: its group, positions (BM a tile) and column tile (of `ntiles`, innermost).
 // Group E is the rows past the last group.  False: there is no such tile; the grid holds the most that
-// ascending offsets can give.  Every wave counts the groups' tiles for itself, 64 groups at a time.
+// ascending offsets can give.  Every wave counts the groups' tiles for itself, 256 groups at a time: four a lane,
+// all their offsets in flight together, since each product waits for this (of 200 groups, 100003 fp32 rows, 32 x
+// 128: 25 us, 29 us by 64 groups at a time and sums through LDS).
 template <int BM>
 __device__ __forceinline__ bool find_tile(const GroupedArgs& a, int id, int ntiles, int& group, int& first, int& end,
                                           int& ntile) {
+  constexpr int PER = 4, Sweep = 64 * PER;
   const int lane = threadIdx.x & 63;
-  int all = 0, past = 0, lo = 0, hi = 0;
-  for (int base = 0; base < a.E; base += 64) {
-    const int e = base + lane;
-    lo = e < a.E ? offset_at(a, e) : 0;
-    hi = e < a.E ? offset_at(a, e + 1) : 0;
-    all += tiles_of<BM>(lo, hi);
-    past = max(past, hi);
-  }
+  const auto add = [](int p, int q) { return p + q; };
+  const auto larger = [](int p, int q) { return p > q ? p : q; };
+  int off[PER + 1], count = 0, incl = 0;
+  auto sweep = [&](int base) {
 #pragma unroll
-  for (int off = 32; off >= 1; off /= 2) {
-    all += __shfl_xor(all, off);
-    past = max(past, __shfl_xor(past, off));
+    for (int i = 0; i <= PER; ++i) off[i] = offset_at(a, min(base + lane * PER + i, a.E));
+    count = 0;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) count += tiles_of<BM>(off[i], off[i + 1]);
+    incl = lanes_scan(count, add);
+  };
+  int all = 0, past = 0;
+  for (int base = 0; base < a.E; base += Sweep) {
+    sweep(base);
+    all += __builtin_amdgcn_readlane(incl, 63);
+    int most = off[0];
+#pragma unroll
+    for (int i = 1; i <= PER; ++i) most = max(most, off[i]);
+    past = max(past, __builtin_amdgcn_readlane(lanes_scan(most, larger), 63));
   }
-  all = __builtin_amdgcn_readfirstlane(all + tiles_of<BM>(past, (int)a.M)) * ntiles;
-  if (id >= all) return false;
-  const int tile = xcd_tile(id, all), t = tile / ntiles;
+  const int total = (all + tiles_of<BM>(past, (int)a.M)) * ntiles;
+  if (id >= total) return false;
+  const int tile = xcd_tile(id, total), t = tile / ntiles;
   ntile = tile - t * ntiles;
+  if (t >= all) {
+    group = a.E;
+    first = past + (t - all) * BM;
+    end = (int)a.M;
+    return true;
+  }
   int before = 0;
-  for (int base = 0; base <= a.E; base += 64) {
-    const int e = base + lane;
-    if (a.E >= 64) {      // (else as they were)
-      lo = e < a.E ? offset_at(a, e) : 0;
-      hi = e < a.E ? offset_at(a, e + 1) : 0;
-    }
-    if (e == a.E) {
-      lo = past;
-      hi = (int)a.M;
-    }
-    const int tiles = tiles_of<BM>(lo, hi);
-    int incl = tiles;
-#pragma unroll
-    for (int off = 1; off < 64; off *= 2) {
-      const int v = __shfl_up(incl, off);
-      if (lane >= off) incl += v;
-    }
+  for (int base = 0; base < a.E; base += Sweep) {
+    if (a.E > Sweep) sweep(base);      // (else as they were)
     const uint64_t hit = __ballot(before + incl > t);
     if (hit) {
       const int src = __ffsll((unsigned long long)hit) - 1;
-      const int skipped = before + __shfl(incl - tiles, src);
-      group = __builtin_amdgcn_readfirstlane(base + src);
-      first = __builtin_amdgcn_readfirstlane(__shfl(lo, src) + (t - skipped) * BM);
-      end = __builtin_amdgcn_readfirstlane(__shfl(hi, src));
+      int rest = t - before - __builtin_amdgcn_readlane(incl - count, src);
+#pragma unroll
+      for (int i = 0; i < PER; ++i) {
+        const int lo = __builtin_amdgcn_readlane(off[i], src), hi = __builtin_amdgcn_readlane(off[i + 1], src);
+        const int tiles = tiles_of<BM>(lo, hi);
+        if (rest >= 0 && rest < tiles) {
+          group = base + src * PER + i;
+          first = lo + rest * BM;
+          end = hi;
+        }
+        rest -= tiles;
+      }
       return true;
     }
-    before += __shfl(incl, 63);
+    before += __builtin_amdgcn_readlane(incl, 63);
   }
   return false;
 }
