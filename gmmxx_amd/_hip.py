@@ -145,7 +145,7 @@ def load_library(path: Optional[str] = None):
     p = path or os.environ.get("GMMXX_HIP_LIBRARY", _LIB_PATH)
     try:
         lib = _declare(ctypes.CDLL(p, mode=ctypes.RTLD_LOCAL))
-    except OSError as exc:
+    except (OSError, AttributeError) as exc:      # (AttributeError: a library without some entry point)
         _load_error = exc
         raise HipBackendUnavailable(
             f"cannot load {p}: {exc}. Build it with `python -m gmmxx_amd.build`.") from exc

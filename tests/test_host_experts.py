@@ -171,3 +171,13 @@ def test_failures_are_the_packages_own():
         experts._failed(RuntimeError("gmmxx_hip_route failed (status 3): x\nException raised from check"))
     with pytest.raises(RuntimeError, match="out of memory"):
         experts._failed(RuntimeError("out of memory"))
+
+
+def test_library_without_the_entry_points(tmp_path):
+    import subprocess
+    src = tmp_path / "old.c"
+    src.write_text("int gmmxx_hip_abi_version(void) { return 2; }\n")
+    old = tmp_path / "old.so"
+    subprocess.run(["gcc", "-shared", "-fPIC", "-o", str(old), str(src)], check=True)
+    with pytest.raises(_hip.HipBackendUnavailable, match="Build it"):
+        _hip.load_library(str(old))
