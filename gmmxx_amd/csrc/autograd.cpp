@@ -12,8 +12,11 @@
 // Arguments have been checked by the caller (gmmxx_amd/experts.py): matrices with
 // adjacent row elements, matching shapes, types and devices.
 
+#include <c10/core/AutogradState.h>
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 #include <torch/extension.h>
 
 #include <string>
@@ -88,7 +91,23 @@ Tensor rows_of(const Tensor& t) { return t.stride(1) == 1 || t.size(1) == 1 ? t 
 
 Tensor bytes(int64_t n, const Tensor& like) { return at::empty({n}, like.options().dtype(at::kByte)); }
 
+// What no result would show is refused: the operators have no forward-mode derivative, and a result without a
+// tangent would pass for a constant; a trace would record the results' allocation but not the launch that writes
+// them.
+void refuse(std::initializer_list<const Tensor*> ts) {
+  using c10::impl::TorchDispatchModeTLS;
+  TORCH_CHECK_NOT_IMPLEMENTED(
+      !torch::jit::tracer::isTracing() && !(TorchDispatchModeTLS::any_modes_set() &&
+                                            TorchDispatchModeTLS::get_mode(c10::impl::TorchDispatchModeKey::PROXY)),
+      "gmmxx_amd operators cannot be traced");
+  if (!c10::AutogradState::get_tls_state().get_fw_grad_mode()) return;
+  for (const Tensor* t : ts)
+    TORCH_CHECK_NOT_IMPLEMENTED(!t->defined() || !t->_fw_grad(0).defined(),
+                                "gmmxx_amd operators have no forward-mode derivative");
+}
+
 bool wants_grad(std::initializer_list<const Tensor*> ts) {
+  refuse(ts);
   if (!at::GradMode::is_enabled()) return false;
   for (const Tensor* t : ts)
     if (t->defined() && t->requires_grad()) return true;
@@ -137,6 +156,7 @@ struct LayerNorm : torch::autograd::Function<LayerNorm> {
   }
 
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    refuse({&grads[0]});
     const auto saved = ctx->get_saved_variables();
     const Tensor &x = saved[0], &w = saved[1], &stats = saved[2];
     const int64_t n = x.size(0), d = x.size(1), bias = ctx->saved_data["bias"].toInt();
@@ -203,6 +223,7 @@ struct Route : torch::autograd::Function<Route> {
   }
 
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    refuse({&grads[1]});
     if (!grads[1].defined()) return {Tensor(), Tensor(), Tensor()};
     const auto saved = ctx->get_saved_variables();
     const Tensor &experts = saved[0], &gates = saved[1], &scores = saved[2], &norm = saved[3];
@@ -267,6 +288,7 @@ struct Grouped : torch::autograd::Function<Grouped> {
   }
 
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    refuse({&grads[0]});
     const auto saved = ctx->get_saved_variables();
     const Tensor &x = saved[0], &w = saved[1], &offsets = saved[2], &rows = saved[3], &slots = saved[4];
     const bool need_x = ctx->needs_input_grad(0), need_w = ctx->needs_input_grad(1);
@@ -316,6 +338,7 @@ struct Combine : torch::autograd::Function<Combine> {
   }
 
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    refuse({&grads[0]});
     const auto saved = ctx->get_saved_variables();
     const Tensor &y = saved[0], &gates = saved[1], &slots = saved[2], &offsets = saved[3];
     const int64_t n = slots.size(0), k = slots.size(1);

@@ -12,10 +12,11 @@ them:
 ``scores`` are a gate's outputs or a mixture's log joint densities (log
 responsibilities serve as well: a row's constant cancels).  Every function runs
 on the caller's current stream, never synchronises, and is differentiable (once)
-by torch's autograd; where no gradient is wanted, nothing is saved.  Elements are
-float32, bfloat16 or float16; sums and statistics are float32 and results are
-rounded once.  Results are the same from run to run: no sum depends on the order
-in which workgroups finish.
+by torch's autograd; where no gradient is wanted, nothing is saved.  Forward-mode
+derivatives and traces (``torch.jit.trace``, ``make_fx``) are refused with
+``NotImplementedError``.  Elements are float32, bfloat16 or float16; sums and
+statistics are float32 and results are rounded once.  Results are the same from
+run to run: no sum depends on the order in which workgroups finish.
 
 The kernels are hand-written HIP behind the C ABI (include/gmmxx_hip.h); the
 autograd functions around it are the native module ``gmmxx_amd._autograd``
