@@ -229,13 +229,12 @@ def grouped_matmul(x: torch.Tensor, weight: torch.Tensor, groups: Union[Routing,
         bias = bias.contiguous()
     if isinstance(groups, Routing):
         offsets = _int_tensor(groups.offsets, "groups.offsets", index, (e + 1,))
-        if _tensor(groups.slots, "groups.slots").ndim != 2:
-            raise ValueError(f"groups.slots must have shape (N, top_k), got {tuple(groups.slots.shape)}")
+        if _tensor(groups.slots, "groups.slots").ndim != 2 or not 1 <= groups.slots.shape[1] <= MAX_TOP_K:
+            raise ValueError(f"groups.slots must have shape (N, top_k) with 1 <= top_k <= {MAX_TOP_K}, "
+                             f"got {tuple(groups.slots.shape)}")
         slots = _int_tensor(groups.slots, "groups.slots", index, (x.shape[0], groups.slots.shape[1]))
         rows = _int_tensor(groups.rows, "groups.rows", index, (slots.numel(),))
         m = slots.numel()
-        if slots.shape[1] > MAX_TOP_K:
-            raise ValueError(f"groups: top_k must be at most {MAX_TOP_K}, got {slots.shape[1]}")
     else:
         offsets = _int_tensor(groups, "groups", index, (e + 1,), (torch.int32, torch.int64))
         rows = slots = None
