@@ -37,6 +37,7 @@ _ELEMS = (torch.float32, torch.bfloat16, torch.float16)
 MAX_EXPERTS = 4096
 MAX_TOP_K = 64
 MAX_NORM_WIDTH = 65536
+MAX_WIDTH = 1 << 22
 _MAX_POSITIONS = 1 << 30
 
 
@@ -202,7 +203,7 @@ def grouped_matmul(x: torch.Tensor, weight: torch.Tensor, groups: Union[Routing,
                    bias: Optional[torch.Tensor] = None) -> torch.Tensor:
     """``x[p] @ weight[e] + bias[e]`` for every position p of every expert e's group.
 
-    ``weight`` is (E, D, F) with E <= 4096, contiguous or a transposed view of
+    ``weight`` is (E, D, F) with E <= 4096 and D and F <= 2^22, contiguous or a transposed view of
     (E, F, D), ``bias`` (E, F), both of x's dtype.  ``groups`` is
 
     * a ``Routing``: ``x`` is (N, D), its rows are read where the routing sends them,
@@ -218,10 +219,12 @@ def grouped_matmul(x: torch.Tensor, weight: torch.Tensor, groups: Union[Routing,
     if x.ndim != 2 or x.shape[1] < 1:
         raise ValueError(f"x must have shape (rows, D) with D >= 1, got {tuple(x.shape)}")
     _like(weight, "weight", x.dtype, index)
+    if x.shape[1] > MAX_WIDTH:
+        raise ValueError(f"x must have shape (rows, D) with D <= {MAX_WIDTH}, got {tuple(x.shape)}")
     if weight.ndim != 3 or weight.shape[1] != x.shape[1] or not 1 <= weight.shape[0] <= MAX_EXPERTS \
-            or weight.shape[2] < 1:
-        raise ValueError(f"weight must have shape (E, {x.shape[1]}, F) with 1 <= E <= {MAX_EXPERTS}, "
-                         f"got {tuple(weight.shape)}")
+            or not 1 <= weight.shape[2] <= MAX_WIDTH:
+        raise ValueError(f"weight must have shape (E, {x.shape[1]}, F) with 1 <= E <= {MAX_EXPERTS} and "
+                         f"1 <= F <= {MAX_WIDTH}, got {tuple(weight.shape)}")
     e, _, f = weight.shape
     if bias is not None:
         if tuple(_like(bias, "bias", x.dtype, index).shape) != (e, f):
@@ -253,8 +256,8 @@ def combine_rows(y: torch.Tensor, routing: Routing, gates: Optional[torch.Tensor
     """``out[n] = sum over j of gates[n, j] * y[routing.slots[n, j]]``: the experts' results
     of each row, added up.
 
-    ``y`` is (N * top_k, F) in grouped order, ``gates`` (N, top_k) float32, by default
-    ``routing.gates``.  Choices without an expert add nothing.  Differentiable in y
+    ``y`` is (N * top_k, F) in grouped order, F <= 2^22, ``gates`` (N, top_k) float32,
+    by default ``routing.gates``.  Choices without an expert add nothing.  Differentiable in y
     and the gates."""
     _operand(y, "y")
     index = y.get_device()
@@ -268,8 +271,8 @@ def combine_rows(y: torch.Tensor, routing: Routing, gates: Optional[torch.Tensor
     if offsets.ndim != 1 or offsets.shape[0] < 2:
         raise ValueError(f"routing.offsets must have shape (E + 1,), got {tuple(offsets.shape)}")
     offsets = _int_tensor(offsets, "routing.offsets", index, offsets.shape)
-    if y.ndim != 2 or y.shape[0] != slots.numel() or y.shape[1] < 1:
-        raise ValueError(f"y must have shape ({slots.numel()}, F) with F >= 1, got {tuple(y.shape)}")
+    if y.ndim != 2 or y.shape[0] != slots.numel() or not 1 <= y.shape[1] <= MAX_WIDTH:
+        raise ValueError(f"y must have shape ({slots.numel()}, F) with 1 <= F <= {MAX_WIDTH}, got {tuple(y.shape)}")
     if y.shape[0] >= _MAX_POSITIONS:
         raise ValueError(f"there must be fewer than {_MAX_POSITIONS} positions, got {y.shape[0]}")
     gates = routing.gates if gates is None else gates

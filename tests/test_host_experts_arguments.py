@@ -28,3 +28,18 @@ def test_top_k_out_of_range(n, k):
         gmmxx_amd.grouped_matmul(x, torch.zeros(3, 4, 5), routing(n, k))
     with pytest.raises(ValueError, match="top_k"):
         gmmxx_amd.combine_rows(torch.zeros(n * k, 5), routing(n, k))
+
+
+WIDE = (1 << 22) + 1
+
+
+@pytest.mark.parametrize("rows", [0, 2])
+@pytest.mark.parametrize("which", ["D", "F"])
+def test_matrices_too_wide(rows, which):
+    """The library's limit, by the argument's own name."""
+    x = torch.zeros(1, 1).expand(rows, WIDE if which == "D" else 4)
+    w = torch.zeros(1, 1, 1).expand(3, x.shape[1], WIDE if which == "F" else 4)
+    with pytest.raises(ValueError, match="4194304"):
+        gmmxx_amd.grouped_matmul(x, w, torch.zeros(4, dtype=torch.int32))
+    with pytest.raises(ValueError, match="4194304"):
+        gmmxx_amd.combine_rows(torch.zeros(1, 1).expand(rows, WIDE), routing(rows, 1))
