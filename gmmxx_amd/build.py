@@ -5,7 +5,8 @@
 Each translation unit is compiled separately (in parallel) and linked into a
 shared library next to this file, where ``gmmxx_amd._hip`` loads it.  The
 autograd functions of ``gmmxx_amd.experts`` are a Python extension beside it,
-``_autograd.so``, compiled against the installed torch.
+``_autograd.so``, compiled against the installed torch; where a C++ compiler, torch
+or Python's headers are missing, the library is built without it.
 """
 
 from __future__ import annotations
@@ -15,7 +16,9 @@ import shutil
 import subprocess
 import sys
 import sysconfig
+import warnings
 from concurrent.futures import ThreadPoolExecutor
+from typing import Optional
 
 PKG_DIR = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(PKG_DIR)
@@ -61,13 +64,30 @@ def _compile(src: str) -> str:
     return obj
 
 
+def _cxx() -> Optional[str]:
+    return shutil.which("g++") or shutil.which("c++")
+
+
+def _autograd_lacks() -> Optional[str]:
+    """What the autograd extension needs and this host does not have."""
+    if _cxx() is None:
+        return "a C++ compiler"
+    if not os.path.exists(os.path.join(sysconfig.get_paths()["include"], "Python.h")):
+        return "Python's headers"
+    try:
+        import torch.utils.cpp_extension  # noqa: F401
+    except ImportError:
+        return "torch"
+    return None
+
+
 def _build_autograd() -> None:
     """Compile csrc/autograd.cpp (host code only) into _autograd.so."""
     import torch
     from torch.utils import cpp_extension
 
     tmp = AUTOGRAD_PATH + ".tmp"
-    cmd = [shutil.which("g++") or "c++", "-O2", "-std=c++17", "-fPIC", "-shared", "-D__HIP_PLATFORM_AMD__=1",
+    cmd = [_cxx(), "-O2", "-std=c++17", "-fPIC", "-shared", "-D__HIP_PLATFORM_AMD__=1",
            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", "-I", os.path.join(ROOT, "include"),
            *(a for p in cpp_extension.include_paths() for a in ("-isystem", p)),
            "-isystem", os.path.join(os.environ.get("ROCM_PATH", "/opt/rocm"), "include"),
@@ -82,20 +102,31 @@ def _build_autograd() -> None:
 
 def build(verbose: bool = False) -> str:
     """Compile every HIP translation unit and link libgmmxx_hip.so, and the autograd
-    extension; returns the library's path."""
+    extension; returns the library's path.
+
+    The library does not depend on the extension: it is in place before an error of the
+    extension's is raised, and a host that lacks what only the extension needs gets a
+    warning.  An extension of an earlier build is taken away then: it may not fit."""
     os.makedirs(BUILD_DIR, exist_ok=True)
+    lacks = _autograd_lacks()
     with ThreadPoolExecutor(max_workers=len(SOURCES) + 1) as ex:
-        extension = ex.submit(_build_autograd)
+        extension = None if lacks else ex.submit(_build_autograd)
         objs = list(ex.map(_compile, SOURCES))
-        extension.result()
     tmp = LIB_PATH + ".tmp"
     cmd = [_hipcc(), f"--offload-arch={ARCH}", "-shared", "-fPIC", *objs, "-o", tmp]
     res = subprocess.run(cmd, capture_output=True, text=True)
     if res.returncode != 0:
         raise RuntimeError(f"link failed:\n{res.stderr}")
     os.replace(tmp, LIB_PATH)
+    if (extension is None or extension.exception()) and os.path.exists(AUTOGRAD_PATH):
+        os.remove(AUTOGRAD_PATH)
+    if extension is None:
+        warnings.warn(f"{os.path.basename(AUTOGRAD_PATH)} is not built for want of {lacks}; gmmxx_amd.experts needs it",
+                      RuntimeWarning, stacklevel=2)
+    else:
+        extension.result()
     if verbose:
-        print(f"built {LIB_PATH} and {AUTOGRAD_PATH}")
+        print(f"built {LIB_PATH}" + ("" if lacks else f" and {AUTOGRAD_PATH}"))
     return LIB_PATH
 
 
