@@ -12,6 +12,15 @@ typedef __bf16 bf16_t;
 template <typename T> void launch_rows_tiles(const GroupedArgs& a, bool direct, bool larger, hipStream_t s);
 template <typename T> void launch_dw_tiles(const GroupedArgs& a, bool direct, bool larger, int splits, hipStream_t s);
 
+// A grid of `blocks` workgroups and `parts` along y.  A dimension's threads are counted in 32 bits, so what passes
+// 2^31 of them goes along z (the last layer may have workgroups to spare).
+inline dim3 grid_of(int64_t blocks, int threads, int parts = 1) {
+  const int64_t most = (int64_t(1) << 31) / threads;
+  if (blocks <= most) return dim3((unsigned)blocks, (unsigned)parts);
+  return dim3((unsigned)most, (unsigned)parts, (unsigned)((blocks + most - 1) / most));
+}
+__device__ __forceinline__ int block_id() { return (int)(blockIdx.z * gridDim.x + blockIdx.x); }
+
 // offsets[e], within the positions (M < 2^30).
 __device__ __forceinline__ int offset_at(const GroupedArgs& a, int e) {
   if (e <= 0) return 0;

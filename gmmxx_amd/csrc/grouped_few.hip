@@ -64,7 +64,7 @@ __global__ __launch_bounds__(kThreads) void grouped_few_kernel(GroupedArgs a, in
   __shared__ __align__(16) float4 xs[kChunk];
   __shared__ float part[kWaves][kRows][Cols];
   int group, first, end, ntile;
-  if (!find_tile<kRows>(a, blockIdx.x, ntiles, group, first, end, ntile)) return;
+  if (!find_tile<kRows>(a, block_id(), ntiles, group, first, end, ntile)) return;
   const int rows = min(end - first, kRows), n0 = ntile * Cols;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   if (group < a.E) {
@@ -171,8 +171,9 @@ void few_typed(const GroupedArgs& a, hipStream_t s) {
   const int cols = 8 * kVec<T>, ntiles = (a.Nn + cols - 1) / cols;
   // (groups with rows, and the rows past the last group: no more than there are positions)
   const int64_t tiles = a.M / kRows + (a.M < a.E + 1 ? a.M : a.E + 1);
-  if ((KC ? a.K : a.Nn) < kVec<T>) grouped_few_kernel<T, KC, true><<<(unsigned)(tiles * ntiles), kThreads, 0, s>>>(a, ntiles);
-  else grouped_few_kernel<T, KC, false><<<(unsigned)(tiles * ntiles), kThreads, 0, s>>>(a, ntiles);
+  const dim3 grid = grid_of(tiles * ntiles, kThreads);
+  if ((KC ? a.K : a.Nn) < kVec<T>) grouped_few_kernel<T, KC, true><<<grid, kThreads, 0, s>>>(a, ntiles);
+  else grouped_few_kernel<T, KC, false><<<grid, kThreads, 0, s>>>(a, ntiles);
 }
 
 template <typename T>

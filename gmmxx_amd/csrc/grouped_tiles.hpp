@@ -307,7 +307,7 @@ __global__ __launch_bounds__(64 * WP * WQ) void grouped_rows_kernel(GroupedArgs 
   typedef typename C::Q Q;
   constexpr int S = sizeof(T), V = C::V, BK = C::BK;
   int group, first, end, ntile;
-  if (!find_tile<BQ>(a, blockIdx.x, ntiles, group, first, end, ntile)) return;
+  if (!find_tile<BQ>(a, block_id(), ntiles, group, first, end, ntile)) return;
   const int n0 = ntile * BP;
   const int rows = end - first < BQ ? end - first : BQ;
   if (group == a.E) {
@@ -424,8 +424,9 @@ __global__ __launch_bounds__(64 * WP * WQ) void grouped_dw_kernel(GroupedArgs a,
   typedef typename Result<T, SPLIT>::type O;
   constexpr int S = sizeof(T), V = C::V, BK = C::BK;
   // (consecutive workgroups go to the 8 XCDs in turn: each XCD gets a share of every group, whatever their sizes)
-  const int id = blockIdx.x;
+  const int id = block_id();
   const int e = id / (ptiles * qtiles), tile = id % (ptiles * qtiles);
+  if (e >= a.E) return;
   const int f0 = (tile % ptiles) * BP, d0 = (tile / ptiles) * BQ;
   int lo = offset_at(a, e), hi = offset_at(a, e + 1);
   O* out = static_cast<O*>(a.out) + (int64_t)e * a.K * a.Nn;
@@ -505,8 +506,8 @@ bool wide(const GroupedArgs& a) { return (a.Nx * a.ldx + a.K) * (int64_t)sizeof(
 template <typename T, bool WKC, bool DIRECT, bool WIDE, int BP, int BQ, int WP, int WQ, bool SHORT = false>
 void rows_tiled(const GroupedArgs& a, hipStream_t s) {
   const int ntiles = (a.Nn + BP - 1) / BP;
-  const int64_t grid = (a.M / BQ + a.E + 1) * ntiles;
-  grouped_rows_kernel<T, WKC, DIRECT, WIDE, BP, BQ, WP, WQ, SHORT><<<(unsigned)grid, 64 * WP * WQ, 0, s>>>(a, ntiles);
+  grouped_rows_kernel<T, WKC, DIRECT, WIDE, BP, BQ, WP, WQ, SHORT>
+      <<<grid_of((a.M / BQ + a.E + 1) * ntiles, 64 * WP * WQ), 64 * WP * WQ, 0, s>>>(a, ntiles);
 }
 
 // fp32 tiles of 256 columns by 32 rows where the groups are small: whether they take less matrix work than tiles
@@ -539,7 +540,7 @@ template <typename T, bool DIRECT, bool WIDE, bool SPLIT, int B, int WP, int WQ,
 void dw_tiled(const GroupedArgs& a, int splits, hipStream_t s) {
   const int pt = (a.Nn + B - 1) / B, qt = (a.K + B - 1) / B;
   grouped_dw_kernel<T, DIRECT, WIDE, SPLIT, B, B, WP, WQ, SHORT>
-      <<<dim3((unsigned)(a.E * pt * qt), (unsigned)splits), 64 * WP * WQ, 0, s>>>(a, pt, qt);
+      <<<grid_of((int64_t)a.E * pt * qt, 64 * WP * WQ, splits), 64 * WP * WQ, 0, s>>>(a, pt, qt);
 }
 
 template <typename T, bool SPLIT>

@@ -438,7 +438,8 @@ void launch_route(const RouteArgs& a, hipStream_t s) {
 }
 
 void launch_route_bwd(const RouteArgs& a, hipStream_t s) {
-  const int tile = 32;
+  int tile = 32;            // rows of a block; more where the grid's threads would pass 2^31 (k is small there)
+  while ((a.N + tile - 1) / tile > (int64_t(1) << 31) / kThreads) tile *= 2;
   const unsigned grid = (unsigned)((a.N + tile - 1) / tile);
   const size_t lds = (size_t)(2 * tile * a.k + tile) * 4;
   if (a.elem == ELEM_F32) bwd_typed<float>(a, tile, grid, lds, s);
