@@ -86,8 +86,12 @@ void* ptr(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
 float* floats(const Tensor& t) { return static_cast<float*>(ptr(t)); }
 int32_t* ints(const Tensor& t) { return static_cast<int32_t*>(ptr(t)); }
 
+// A tensor whose memory holds its values: a view may stand for the negatives of them (the imaginary part of a
+// conjugate), which data_ptr() does not tell.
+Tensor plain(const Tensor& t) { return t.defined() && t.is_neg() ? t.resolve_neg() : t; }
+
 // A matrix whose rows' elements are adjacent.
-Tensor rows_of(const Tensor& t) { return t.stride(1) == 1 || t.size(1) == 1 ? t : t.contiguous(); }
+Tensor rows_of(const Tensor& t) { return t.stride(1) == 1 || t.size(1) == 1 ? plain(t) : plain(t).contiguous(); }
 
 Tensor bytes(int64_t n, const Tensor& like) { return at::empty({n}, like.options().dtype(at::kByte)); }
 
@@ -130,6 +134,7 @@ variable_list once(variable_list grads) {
 }
 
 Tensor or_none(const std::optional<Tensor>& t) { return t.has_value() ? *t : Tensor(); }
+std::optional<Tensor> plain(const std::optional<Tensor>& t) { return t.has_value() ? std::optional(plain(*t)) : t; }
 
 // --- layer norm ---------------------------------------------------------------
 
@@ -182,7 +187,10 @@ struct LayerNorm : torch::autograd::Function<LayerNorm> {
   }
 };
 
-Tensor layer_norm(const Tensor& x, const std::optional<Tensor>& weight, const std::optional<Tensor>& bias, double eps) {
+Tensor layer_norm(const Tensor& x0, const std::optional<Tensor>& weight0, const std::optional<Tensor>& bias0,
+                  double eps) {
+  const Tensor x = plain(x0);
+  const std::optional<Tensor> weight = plain(weight0), bias = plain(bias0);
   const Tensor w = or_none(weight), b = or_none(bias);
   if (wants_grad({&x, &w, &b})) return LayerNorm::apply(x, weight, bias, eps);
   return norm_forward(x, w, b, eps, nullptr);
@@ -232,7 +240,7 @@ struct Route : torch::autograd::Function<Route> {
     const auto type = (at::ScalarType)ctx->saved_data["type"].toInt();
     Tensor ds = at::empty({n, e}, gates.options().dtype(type));
     if (n) {
-      const Tensor dg = grads[1].contiguous();
+      const Tensor dg = plain(grads[1]).contiguous();
       On on(gates);
       check(lib.route_backward(elem(type), n, e, k, renormalize, ptr(scores), scores.defined() ? scores.stride(0) : 0,
                                ints(experts), floats(gates), floats(norm), floats(dg), ptr(ds), on.stream()),
@@ -242,7 +250,8 @@ struct Route : torch::autograd::Function<Route> {
   }
 };
 
-std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor> route(const Tensor& scores, int64_t k, bool renormalize) {
+std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor> route(const Tensor& scores0, int64_t k, bool renormalize) {
+  const Tensor scores = plain(scores0);
   const variable_list r =
       wants_grad({&scores}) ? Route::apply(scores, k, renormalize) : route_forward(scores, k, renormalize, false);
   return {r[0], r[1], r[2], r[3], r[4]};
@@ -321,8 +330,10 @@ struct Grouped : torch::autograd::Function<Grouped> {
   }
 };
 
-Tensor grouped(const Tensor& x, const Tensor& w, const std::optional<Tensor>& bias, const Tensor& offsets,
+Tensor grouped(const Tensor& x0, const Tensor& w0, const std::optional<Tensor>& bias0, const Tensor& offsets,
                const std::optional<Tensor>& rows, const std::optional<Tensor>& slots) {
+  const Tensor x = plain(x0), w = plain(w0);
+  const std::optional<Tensor> bias = plain(bias0);
   const Tensor b = or_none(bias), r = or_none(rows);
   if (wants_grad({&x, &w, &b})) return Grouped::apply(x, w, bias, offsets, rows, slots);
   return grouped_forward(x, w, 1, 2, b, offsets, r, r.defined() ? r.size(0) : x.size(0), x.scalar_type());
@@ -357,7 +368,8 @@ struct Combine : torch::autograd::Function<Combine> {
   }
 };
 
-Tensor combine(const Tensor& y, const Tensor& gates, const Tensor& slots, const Tensor& offsets) {
+Tensor combine(const Tensor& y0, const Tensor& gates0, const Tensor& slots, const Tensor& offsets) {
+  const Tensor y = plain(y0), gates = plain(gates0);
   if (wants_grad({&y, &gates})) return Combine::apply(y, gates, slots, offsets);
   return combine_forward(y, gates, slots, offsets, y.scalar_type());
 }
