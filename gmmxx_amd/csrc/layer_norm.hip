@@ -6,11 +6,13 @@
 //
 // A group of G threads holds a row in registers (up to 16 elements a thread, 32 above
 // 16384 columns and 64 above 32768, where part of it spills), so x is read once and
-// the mean is taken out before the squares are summed: rows whose mean is large beside
-// their spread lose nothing.  Everything is fp32; the one rounding is the store.  G is
-// the smallest group that holds the row, so narrow rows share a wave.  Groups stride
-// over the rows, keep w and b in registers and have the next row's loads in flight
-// while a row's sums pass between lanes.
+// the mean is taken out before the squares are summed.  A sum's mean is off by units of
+// the mean itself; the mean of what it left, which comes with the squares, is taken out
+// too, so rows whose mean is large beside their spread keep the spread's precision (the
+// backward pass reads the two together, rounded to fp32: half a unit of the mean).
+// Everything is fp32; the one rounding is the store.  G is the smallest group that holds
+// the row, so narrow rows share a wave.  Groups stride over the rows, keep w and b in
+// registers and have the next row's loads in flight while a row's sums pass between lanes.
 //
 // The backward pass keeps each column's Σ dy·h and Σ dy in registers over the rows
 // of its workgroup, writes one partial row per workgroup, and a second kernel adds
@@ -75,12 +77,18 @@ struct Norm {
   }
 };
 
+// a b, rounded: not fused into what uses it.
+__device__ __forceinline__ float product(float a, float b) {
+#pragma clang fp contract(off)
+  return a * b;
+}
+
 template <typename T, typename WT, int G, int NV, bool SHORT>
 __global__ __launch_bounds__((Norm<T, WT, G, NV, SHORT>::Threads)) void norm_fwd_kernel(NormArgs a) {
   using L = Norm<T, WT, G, NV, SHORT>;
   constexpr int V = L::V;
-  __shared__ float red[2][16][1];
-  int turn = 0;
+  __shared__ float red_sum[2][16][1], red[2][16][2];
+  int turn_sum = 0, turn = 0;
   const int lane = threadIdx.x % G, sub = threadIdx.x / G;
   const int64_t step = (int64_t)gridDim.x * L::RPB;
   int64_t row = (int64_t)blockIdx.x * L::RPB + sub;
@@ -101,27 +109,30 @@ __global__ __launch_bounds__((Norm<T, WT, G, NV, SHORT>::Threads)) void norm_fwd
     for (int i = 0; i < NV; ++i)
 #pragma unroll
       for (int j = 0; j < V; ++j) s[0] += x[i][j];
-    group_sums<G>(s, red, turn);
-    const float mean = s[0] * inv;
-    float q[1] = {0.f};
+    group_sums<G>(s, red_sum, turn_sum);
+    const float about = product(s[0], inv);
+    float q[2] = {0.f, 0.f};
 #pragma unroll
     for (int i = 0; i < NV; ++i)
 #pragma unroll
       for (int j = 0; j < V; ++j) {
-        x[i][j] = L::col(i, lane) + j < a.D ? x[i][j] - mean : 0.f;
+        x[i][j] = L::col(i, lane) + j < a.D ? x[i][j] - about : 0.f;
         q[0] = fmaf(x[i][j], x[i][j], q[0]);
+        q[1] += x[i][j];
       }
     group_sums<G>(q, red, turn);
-    const float rstd = 1.f / sqrtf(q[0] * inv + a.eps);
+    const float rest = q[1] * inv, var = q[0] * inv - rest * rest;
+    const float rstd = 1.f / sqrtf((var < 0.f ? 0.f : var) + a.eps);      // (NaN stays)
+    const float shift = -rest * rstd;
     T* out = static_cast<T*>(a.y) + row * a.D;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
 #pragma unroll
-      for (int j = 0; j < V; ++j) x[i][j] = fmaf(x[i][j] * rstd, w[i][j], b[i][j]);
+      for (int j = 0; j < V; ++j) x[i][j] = fmaf(fmaf(x[i][j], rstd, shift), w[i][j], b[i][j]);
       store_row(out + L::col(i, lane), a.D - L::col(i, lane), x[i]);
     }
     if (lane == 0 && a.mean) {
-      a.mean[row] = mean;
+      a.mean[row] = about + rest;
       a.rstd[row] = rstd;
     }
   }
