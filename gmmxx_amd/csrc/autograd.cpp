@@ -82,7 +82,14 @@ void check(int rc, const char* what) {
 int elem(at::ScalarType t) { return t == at::kFloat ? GMMXX_F32 : t == at::kBFloat16 ? GMMXX_BF16 : GMMXX_F16; }
 int elem(const Tensor& t) { return elem(t.scalar_type()); }
 
-void* ptr(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
+// A tensor that stands for values without holding them (a fake or functional tensor, torch's efficient zeros) gives
+// a null pointer, which the library takes for an operand that is not there.
+void* ptr(const Tensor& t) {
+  if (!t.defined()) return nullptr;
+  void* p = t.data_ptr();
+  TORCH_CHECK_NOT_IMPLEMENTED(p || t.numel() == 0, "gmmxx_amd operators need tensors that hold their values");
+  return p;
+}
 float* floats(const Tensor& t) { return static_cast<float*>(ptr(t)); }
 int32_t* ints(const Tensor& t) { return static_cast<int32_t*>(ptr(t)); }
 

@@ -1,5 +1,6 @@
-"""Operands that are views of the negatives of their memory, as the imaginary part of a
-conjugate is: the values count, in every operand and in the results' gradients."""
+"""Operands whose memory does not hold their values.  Views of the negatives of it, as the
+imaginary part of a conjugate is: the values count, in every operand and in the results'
+gradients.  Tensors without memory: refused, optional operands among them."""
 
 import pytest
 import torch
@@ -64,3 +65,15 @@ def test_imaginary_part_of_a_conjugate(hip):
     assert x.is_neg()
     w, off = rand(2, 1, 8, seed=3), torch.tensor([0, 2, 6], dtype=torch.int32, device=DEV)
     assert torch.equal(gmmxx_amd.grouped_matmul(x, w, off), gmmxx_amd.grouped_matmul(-z.imag.contiguous(), w, off))
+
+
+@pytest.mark.parametrize("call,shapes", CALLS, ids=[c.__name__ for c, _ in CALLS])
+def test_operands_without_memory(hip, call, shapes):
+    """None of them is taken for an operand that was left out."""
+    args = [rand(*s, seed=i) for i, s in enumerate(shapes)]
+    for i, t in enumerate(args):
+        zeros = torch._efficientzerotensor(t.shape, device=DEV)
+        with pytest.raises(NotImplementedError, match="hold their values"):
+            call(*[zeros if i == j else a for j, a in enumerate(args)])
+        with pytest.raises(NotImplementedError, match="hold their values"):
+            torch.func.functionalize(lambda v: call(*[v if i == j else a for j, a in enumerate(args)]))(t)
