@@ -109,7 +109,8 @@ __device__ __forceinline__ float with_other(float v, F&& op) {
 }
 
 // op over aligned groups of G consecutive lanes (G a power of two up to 64): the same value, by the same order
-// of operations, in every lane of the group.  All 64 lanes take part.
+// of operations, in every lane of the group.  A group's lanes take part together; no exchange crosses a group, so
+// other groups of the wave may have left.
 template <int G, typename F>
 __device__ __forceinline__ float lanes_reduce(float v, F&& op) {
   if constexpr (G > 1) v = with_other<1>(v, op);
@@ -126,7 +127,7 @@ __device__ __forceinline__ float lanes_sum(float v) {
 }
 
 // Sums of N values over groups of G threads: lanes_sum within a wave, `red` (two slots of 16 waves' values, used
-// in turn so that one barrier separates writers from readers) above it.
+// in turn so that one barrier separates writers from readers) above it, of which each lane reads one wave's.
 template <int G, int N>
 __device__ __forceinline__ void group_sums(float (&v)[N], float (*red)[16][N], int& turn) {
 #pragma unroll
@@ -140,11 +141,7 @@ __device__ __forceinline__ void group_sums(float (&v)[N], float (*red)[16][N], i
     }
     __syncthreads();
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-      v[i] = 0.f;
-#pragma unroll
-      for (int w = 0; w < G / 64; ++w) v[i] += slot[w][i];
-    }
+    for (int i = 0; i < N; ++i) v[i] = lanes_sum<G / 64>(slot[threadIdx.x % (G / 64)][i]);
   }
 }
 
