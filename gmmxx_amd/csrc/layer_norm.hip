@@ -18,8 +18,8 @@
 // of its workgroup, writes one partial row per workgroup, and a second kernel adds
 // the partials: two fixed orders of additions, no atomics.
 //
-// Bound by bytes.  16384 x 4096 bf16: forward 47 us (5.7 TB/s), backward 86 us (4.7 TB/s),
-// the partials' sum 8 us; 100003 x 100 fp32: 18 us (4.4), 24 us (5.1) and 4 us.  One row
+// Bound by bytes.  16384 x 4096 bf16: forward 48 us (5.5 TB/s), backward 87 us (4.6 TB/s),
+// the partials' sum 8 us; 100003 x 100 fp32: 19 us (4.3), 24 us (5.1) and 4 us.  One row
 // is a launch: 2.6 us.
 
 #include "experts.hpp"
@@ -251,8 +251,8 @@ __global__ __launch_bounds__(kSumCols* kSumRows) void norm_sum_kernel(NormArgs a
 }
 
 // Calls f.template operator()<G, NV, SHORT>() for the smallest group that holds a row of D.
-// (the backward pass of 1024 threads would spill: 4096 x 16384 bf16 293 us by them, 202 us by 512)
-template <typename T, bool BWD, typename F>
+// (4096 x 16384 bf16: backward 199 us by 1024 threads, 207 us by 512 with twice the vectors)
+template <typename T, typename F>
 void with_group(int D, F&& f) {
   constexpr int N16 = 16 / kVec<T>;    // vectors of 16 elements
   if (D < kVec<T>) f.template operator()<8, N16, true>();
@@ -262,7 +262,7 @@ void with_group(int D, F&& f) {
   else if (D <= 64 * 16) f.template operator()<64, N16, false>();
   else if (D <= 256 * 16) f.template operator()<256, N16, false>();
   else if (D <= 512 * 16) f.template operator()<512, N16, false>();
-  else if (D <= 1024 * 16) f.template operator()<BWD ? 512 : 1024, BWD ? 2 * N16 : N16, false>();
+  else if (D <= 1024 * 16) f.template operator()<1024, N16, false>();
   else if (D <= 1024 * 32) f.template operator()<1024, 2 * N16, false>();
   else f.template operator()<1024, 4 * N16, false>();
 }
@@ -286,7 +286,7 @@ struct FwdOp {
   const NormArgs& a; hipStream_t s;
   template <typename T, typename WT> void operator()() {
     Go<T, WT> go{a, s};
-    with_group<T, false>(a.D, go);
+    with_group<T>(a.D, go);
   }
   template <typename T, typename WT> struct Go {
     const NormArgs& a; hipStream_t s;
@@ -303,7 +303,7 @@ struct BwdOp {
   const NormArgs& a; hipStream_t s; int blocks;
   template <typename T, typename WT> void operator()() {
     Go<T, WT> go{a, s, blocks};
-    with_group<T, true>(a.D, go);
+    with_group<T>(a.D, go);
     if (a.part) norm_sum_kernel<WT><<<(2 * a.D + kSumCols - 1) / kSumCols, kSumCols * kSumRows, 0, s>>>(a, blocks);
   }
   template <typename T, typename WT> struct Go {
