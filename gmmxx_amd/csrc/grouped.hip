@@ -87,8 +87,11 @@ __global__ __launch_bounds__(kThreads) void grouped_reduce_kernel(GroupedArgs a,
 
 // Whether tiles of 256 (one to a CU) beat tiles of 128 (two at a time): the most tiles that a CU gets, in
 // 128 x 128 tiles, over the rate measured for each (1170 and 880 TFLOP/s for one product of 8192 x 8192 x
-// 8192).  8192 rows of 16 experts, 2048 -> 1024: 56.8 us by 256, 39.5 us by 128; 32768 rows of 32 experts,
-// 1024 -> 2048: 172 and 203 us, its gradient for x 190 and 209 us (near ties go to the larger).
+// 8192).  The groups' sizes are on the device, so they are taken to be uneven; near ties go to the larger.  Calls by
+// 256 and by 128, bf16: 8192 rows of 16 uneven experts, 2048 -> 1024, 60 and 67 us (of 8 experts 54 and 60; exactly
+// even groups, whose last tiles are full, 63 and 49); 16384 rows of 16, 113 and 106 us (even 70 and 84); 32768 rows
+// of 32 experts, 1024 -> 2048, 190 and 201 us.  The weight's gradient there: 191 and 205 us, but 307 and 234 us where
+// a few groups have most of the rows, which tiles of 128 cut into parts.
 bool larger_tiles(double tiles256, double tiles128) {
   return ceil(tiles256 / 256.0) * 4.0 / 1.17 < 1.1 * ceil(tiles128 / 256.0) / 0.88;
 }

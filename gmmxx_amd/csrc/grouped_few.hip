@@ -183,10 +183,13 @@ void few(const GroupedArgs& a, hipStream_t s) {
 
 }  // namespace
 
-// Up to which number of positions this beats the tiles.  Whole 16-bit chunks: 8 (1024 x 2048 matrices, 16
-// experts: 9.8 and 12.7 us at 8 positions, 28 and 16 us at 32).  Other 16-bit shapes: two an expert (100 x 77:
-// 7.2 and 10.5 us at 32).  fp32: one an expert or 32 (256 x 512, 16 experts: 6 and 14 us at 32 positions; 64
-// experts, two an expert: 22 and 14.5 us; 1024 x 2048 likewise: 168 and 87 us).
+// Up to which number of positions this is taken, and what calls in a row took by it and by the tiles.  Whole 16-bit
+// chunks: 8 (1024 x 2048 matrices, 16 experts: 14.0 and 14.5 us at 8 positions, 24 and 19.5 us at 16).  Other 16-bit
+// shapes: two an expert (100 x 77, 64 experts, 32 positions: 7.4 and 8.2 us with the columns adjacent, 9.0 and 7.4 us
+// with the reduction).  fp32: one an expert or 32 (256 x 512: 16 experts 8.0 and 14.4 us at 32 positions, 12.0 and
+// 14.4 us at 64; 64 experts 12.1 and 14.5 us at 32, 17.6 and 14.9 us at 64).  The rule does not know the matrices'
+// size: 100 x 77 would stay faster by this up to 256 positions (6.3 and 12.4 us), 1024 x 2048 of 64 experts would be
+// faster by the tiles from 32 positions on (72 and 47 us; 113 and 77 us at 64).
 bool grouped_few_better(const GroupedArgs& a) {
   if (a.elem == ELEM_F32) return a.M <= (a.E > 32 ? a.E : 32);
   return a.M <= 8 || (!grouped_direct(a) && a.M <= 2 * (int64_t)a.E);

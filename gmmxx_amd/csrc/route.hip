@@ -15,8 +15,8 @@
 //          equal experts found by ballots over the index bits.
 // Integer counts do not depend on the order of the additions.
 //
-// The choice is bound by instructions (see choose_rows), the gradient by bytes, the
-// rest by waits.  100000 x 500 fp32, 4 of all: top 76 us (the scores at 2.6 TB/s), scan
+// The choice takes mostly instructions (see choose_rows), the gradient of gates over all
+// candidates bytes, the rest waits.  100000 x 500 fp32, 4 of all: top 76 us (the scores at 2.6 TB/s), scan
 // 13 us, place 10 us, gradient 79 us (5.1 TB/s).  65537 x 64, 8 of 64: 13, 7, 7 and
 // 10 us.  Three rows of 64 in one launch: 4.4 us.
 

@@ -9,14 +9,15 @@ them:
     y = grouped_matmul(h, experts, routing, b)  # every expert's matrix on its own rows
     out = combine_rows(y, routing)              # added up by gate
 
-``scores`` are a gate's outputs or a mixture's log joint densities (log
-responsibilities serve as well: a row's constant cancels).  Every function runs
-on the caller's current stream, never synchronises, and is differentiable (once)
-by torch's autograd; where no gradient is wanted, nothing is saved.  Forward-mode
-derivatives and traces (``torch.jit.trace``, ``make_fx``) are refused with
-``NotImplementedError``.  Elements are float32, bfloat16 or float16; sums and
-statistics are float32 and results are rounded once.  Results are the same from
-run to run: no sum depends on the order in which workgroups finish.
+``scores`` are a gate's outputs or the logarithms of a mixture's responsibilities
+(``torch.log(mixture.predict_proba(x))``).  Every function runs on the caller's
+current stream, never synchronises, and is differentiable (once) by torch's
+autograd; where no gradient is wanted, nothing is saved.  Forward-mode
+derivatives, traces (``torch.jit.trace``, ``make_fx``) and tensors that hold no
+values of their own are refused with ``NotImplementedError``.  Elements are
+float32, bfloat16 or float16; sums and statistics are float32 and results are
+rounded once.  Results are the same from run to run: no sum depends on the order
+in which workgroups finish.
 
 The kernels are hand-written HIP behind the C ABI (include/gmmxx_hip.h); the
 autograd functions around it are the native module ``gmmxx_amd._autograd``
@@ -163,7 +164,7 @@ def route_rows(scores: torch.Tensor, top_k: int, *, renormalize: bool = True) ->
     fewer than ``top_k`` candidates are left, the remaining choices are expert -1 with
     gate 0.  ``gates`` are the softmax of the scores over the chosen experts, or, with
     ``renormalize=False``, over all candidates (the mixture's responsibilities where
-    the scores are its log joint densities); candidates of +inf share the whole weight.
+    the scores are their logarithms); candidates of +inf share the whole weight.
     ``gates`` is differentiable in ``scores``."""
     _operand(scores, "scores")
     if scores.ndim != 2 or not 1 <= scores.shape[1] <= MAX_EXPERTS:
