@@ -12,8 +12,10 @@ own spellings of them.  ``hip_ops`` mirrors the reference's experimental
 
 ``layer_norm``, ``route_rows``, ``grouped_matmul`` and ``combine_rows``
 (``gmmxx_amd.experts``) make a mixture's components, or any gate's outputs, into
-a sparsely gated layer of experts with gradients; they have no reference
-counterpart.
+a sparsely gated layer of experts with gradients; ``embed_rows``, ``dropout``,
+``log_probs``, ``quantize_rows`` and ``quantized_matmul`` (``gmmxx_amd.tokens``)
+take labels as tokens, in front of such a layer and behind it.  They have no
+reference counterpart.
 """
 
 from ._hip import HipBackendUnavailable, HipRuntimeError, HipRuntimeFallback, has_hip, require_hip
@@ -33,6 +35,7 @@ from .interface import GMMXX
 from .large_n import (batch_gmm_largeN_cpu, fit_large_n, large_n_predict_cpu, large_n_predict_proba_cpu,
                       large_n_score_samples_cpu, predict_large_n, predict_proba_large_n, score_samples_large_n)
 from .experts import Routing, combine_rows, grouped_matmul, layer_norm, route_rows
+from .tokens import LogProbs, Quantized, dropout, embed_rows, log_probs, quantize_rows, quantized_matmul
 from . import hip_ops
 
 __all__ = [
@@ -53,6 +56,7 @@ __all__ = [
     "batch_gmm_Spherical_hip", "batch_gmm_Diagonal_hip", "batch_gmm_Tied_hip", "batch_gmm_Full_hip",
     "fit_large_n", "predict_large_n", "predict_proba_large_n", "score_samples_large_n", "hip_ops",
     "Routing", "combine_rows", "grouped_matmul", "layer_norm", "route_rows",
+    "LogProbs", "Quantized", "dropout", "embed_rows", "log_probs", "quantize_rows", "quantized_matmul",
 ]
 
 __version__ = "0.1.0"

@@ -74,6 +74,7 @@ _load_error: Optional[BaseException] = None
 def _declare(lib):
     P = ctypes.POINTER(_Problem)
     vp, i64, f64, i32 = ctypes.c_void_p, ctypes.c_int64, ctypes.c_double, ctypes.c_int32
+    u64 = ctypes.c_uint64
     sig = {
         "gmmxx_hip_abi_version": (ctypes.c_int, []),
         "gmmxx_hip_last_error": (ctypes.c_char_p, []),
@@ -114,6 +115,16 @@ def _declare(lib):
         "gmmxx_hip_combine": (ctypes.c_int, [i32, i64, i64, i64, i64, vp, i32, i64, vp, vp, vp, vp, vp]),
         "gmmxx_hip_combine_backward": (ctypes.c_int, [i32, i64, i64, i64, i64, vp, i64, vp, vp, vp, vp, i64, vp, vp,
                                                       vp]),
+        "gmmxx_hip_embed": (ctypes.c_int, [i32, i64, i64, i64, vp, i64, vp, i32, f64, vp, vp]),
+        "gmmxx_hip_embed_workspace_bytes": (i64, [i64, i64, i64]),
+        "gmmxx_hip_embed_backward": (ctypes.c_int, [i32, i64, i64, i64, vp, i64, vp, i32, f64, vp, vp, i64, vp]),
+        "gmmxx_hip_dropout": (ctypes.c_int, [i32, i64, f64, u64, vp, u64, vp, vp, vp, vp]),
+        "gmmxx_hip_log_probs_workspace_bytes": (i64, [i64, i64, i64]),
+        "gmmxx_hip_log_probs": (ctypes.c_int, [i32, i64, i64, i64, vp, i64, vp, i32, vp, vp, vp, vp, vp, vp, i64, vp]),
+        "gmmxx_hip_log_probs_backward": (ctypes.c_int, [i32, i64, i64, i64, vp, i64, vp, i32, vp, vp, vp, vp, vp, vp,
+                                                        vp]),
+        "gmmxx_hip_quantize": (ctypes.c_int, [i32, i64, i64, vp, i64, vp, i64, vp, vp]),
+        "gmmxx_hip_quantized_matmul": (ctypes.c_int, [i32, i64, i64, i64, vp, i64, vp, vp, i64, vp, vp, vp, vp]),
     }
     for name, (res, args) in sig.items():
         fn = getattr(lib, name)
@@ -134,7 +145,10 @@ def exported_symbols() -> Tuple[str, ...]:
             "gmmxx_hip_layer_norm", "gmmxx_hip_layer_norm_workspace_bytes", "gmmxx_hip_layer_norm_backward",
             "gmmxx_hip_route_workspace_bytes", "gmmxx_hip_route", "gmmxx_hip_route_backward",
             "gmmxx_hip_grouped_matmul", "gmmxx_hip_grouped_workspace_bytes", "gmmxx_hip_grouped_weight_grad",
-            "gmmxx_hip_combine", "gmmxx_hip_combine_backward")
+            "gmmxx_hip_combine", "gmmxx_hip_combine_backward",
+            "gmmxx_hip_embed", "gmmxx_hip_embed_workspace_bytes", "gmmxx_hip_embed_backward", "gmmxx_hip_dropout",
+            "gmmxx_hip_log_probs_workspace_bytes", "gmmxx_hip_log_probs", "gmmxx_hip_log_probs_backward",
+            "gmmxx_hip_quantize", "gmmxx_hip_quantized_matmul")
 
 
 def load_library(path: Optional[str] = None):

@@ -4,7 +4,7 @@
 
 Each translation unit is compiled separately (in parallel) and linked into a
 shared library next to this file, where ``gmmxx_amd._hip`` loads it.  The
-autograd functions of ``gmmxx_amd.experts`` are a Python extension beside it,
+autograd functions of ``gmmxx_amd.experts`` and ``gmmxx_amd.tokens`` are a Python extension beside it,
 ``_autograd.so``, compiled against the installed torch; where a C++ compiler, torch
 or Python's headers are missing, the library is built without it.
 """
@@ -29,7 +29,8 @@ AUTOGRAD_PATH = os.path.join(PKG_DIR, "_autograd.so")
 SOURCES = ("em_tile.hip", "em_sph_bf16.hip", "em_fused.hip", "em_coop.hip", "em_one.hip", "em_label.hip", "em_full_wide.hip", "em_full_stats.hip", "em_full_infer.hip",
            "params.hip",
            "kmeans.hip", "abi.hip",
-           "layer_norm.hip", "route.hip", "grouped.hip", "grouped_bf16.hip", "grouped_f16.hip", "grouped_f32.hip", "grouped_few.hip", "combine.hip", "experts_abi.hip")
+           "layer_norm.hip", "route.hip", "grouped.hip", "grouped_bf16.hip", "grouped_f16.hip", "grouped_f32.hip", "grouped_few.hip", "combine.hip", "experts_abi.hip",
+           "embed.hip", "dropout.hip", "log_probs.hip", "quant.hip", "tokens_abi.hip")
 ARCH = os.environ.get("GMMXX_HIP_ARCH", "gfx950")
 
 # -packed-fp32-ops: keep the compiler from emitting packed fp32 VALU ops.
@@ -121,7 +122,7 @@ def build(verbose: bool = False) -> str:
     if (extension is None or extension.exception()) and os.path.exists(AUTOGRAD_PATH):
         os.remove(AUTOGRAD_PATH)
     if extension is None:
-        warnings.warn(f"{os.path.basename(AUTOGRAD_PATH)} is not built for want of {lacks}; gmmxx_amd.experts needs it",
+        warnings.warn(f"{os.path.basename(AUTOGRAD_PATH)} is not built for want of {lacks}; gmmxx_amd.experts and gmmxx_amd.tokens need it",
                       RuntimeWarning, stacklevel=2)
     else:
         extension.result()

@@ -1,0 +1,413 @@
+// Rows of a table looked up by token, and the table's gradient.
+//
+//   out[t] = scale table[index[t]],   dtable[v] = scale Σ_{t: index[t] = v} dy[t]
+//
+// A token outside 0 .. V-1 gives zeros and adds nothing.  The gradient is summed in the
+// order of the sorted tokens (equal ones by position): a stable radix sort of the tokens,
+// then tiles of kTile sorted positions, which add each run of equal tokens in fp32.  A run
+// inside a tile is a row of the result, rounded once; the parts of a run that reaches over
+// tiles are written as fp32 (at most two rows a tile: the run that enters it and the run
+// that leaves it) and added in order by a second kernel, a workgroup for each run and
+// columns.  Rows without a token are written by workgroups of the same launch, which find
+// them by binary searches in the sorted tokens.  No sum depends on the order in which
+// workgroups finish.
+//
+// The sort takes the fewest passes of at most 11 bits; a pass counts digits by block,
+// turns the counts into prefixes over the blocks and places: waves rank 64 tokens at a
+// time by ballots over the digit's bits.
+
+#include <type_traits>
+
+#include "rows.hpp"
+#include "tokens.hpp"
+
+namespace gx::layer {
+
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int kTile = 32;              // sorted positions whose rows one group of threads adds
+constexpr int kMaxBits = 11;
+constexpr int kSortRows = 2048;        // tokens of a block of the sort, more where that gives over kMaxSortBlocks
+constexpr int64_t kMaxSortBlocks = 4096;
+constexpr int64_t kMaxBlocks = 1 << 20;
+
+__host__ __device__ inline int key_bits(int64_t V) {
+  int b = 1;
+  while ((int64_t(1) << b) <= V) ++b;  // keys 0 .. V
+  return b;
+}
+
+int64_t sort_rows(int64_t N) {
+  int64_t r = kSortRows;
+  while ((N + r - 1) / r > kMaxSortBlocks) r *= 2;
+  return r;
+}
+
+__device__ __forceinline__ int64_t token_at(const EmbedArgs& a, int64_t t) {
+  return a.index64 ? static_cast<const int64_t*>(a.index)[t] : static_cast<const int32_t*>(a.index)[t];
+}
+
+// --- lookup -------------------------------------------------------------------
+
+// tx threads (a power of two) share a row's vectors; each takes four rows at a time.
+template <typename T, bool SHORT>
+__global__ __launch_bounds__(kThreads) void embed_kernel(EmbedArgs a, int tx) {
+  constexpr int V = kVec<T>, U = 4;
+  const int lane = threadIdx.x & (tx - 1), rpb = kThreads / tx;
+  const T* table = static_cast<const T*>(a.table);
+  for (int64_t n0 = (int64_t)blockIdx.x * rpb * U + threadIdx.x / tx; n0 < a.N; n0 += (int64_t)gridDim.x * rpb * U) {
+    int64_t row[U];
+#pragma unroll
+    for (int j = 0; j < U; ++j) {
+      const int64_t n = n0 + j * rpb;
+      row[j] = n < a.N ? token_at(a, n) : -1;
+      if ((uint64_t)row[j] >= (uint64_t)a.V) row[j] = -1;
+    }
+    for (int c = lane * V; c < a.D; c += tx * V) {
+      uint4 u[U];
+#pragma unroll
+      for (int j = 0; j < U; ++j) u[j] = fetch16<SHORT>(table + (row[j] < 0 ? 0 : row[j]) * a.ldt + c, a.D - c);
+#pragma unroll
+      for (int j = 0; j < U; ++j) {
+        const int64_t n = n0 + j * rpb;
+        float v[V];
+        unpack16<T>(keep16<SHORT, T>(u[j], a.D - c, a.D), v);
+#pragma unroll
+        for (int i = 0; i < V; ++i) v[i] = row[j] < 0 ? 0.f : v[i] * a.scale;
+        if (n < a.N) store_row(static_cast<T*>(a.out) + n * a.D + c, a.D - c, v);
+      }
+    }
+  }
+}
+
+// --- sort ---------------------------------------------------------------------
+
+// The token of sorted-so-far place i: of the first pass the given ones, V for none.
+__device__ __forceinline__ uint32_t key_at(const EmbedArgs& a, int from, int64_t i) {
+  if (from >= 0) return a.key[from][i];
+  const int64_t t = token_at(a, i);
+  return (uint64_t)t < (uint64_t)a.V ? (uint32_t)t : (uint32_t)a.V;
+}
+
+__global__ __launch_bounds__(kThreads) void sort_count_kernel(EmbedArgs a, int from, int shift, int bits, int64_t rpb) {
+  extern __shared__ int count[];
+  const int bins = 1 << bits;
+  for (int b = threadIdx.x; b < bins; b += kThreads) count[b] = 0;
+  __syncthreads();
+  const int64_t first = blockIdx.x * rpb, last = first + rpb < a.N ? first + rpb : a.N;
+  for (int64_t i = first + threadIdx.x; i < last; i += kThreads)
+    atomicAdd(&count[(key_at(a, from, i) >> shift) & (bins - 1)], 1);
+  __syncthreads();
+  int32_t* hist = a.hist + (int64_t)blockIdx.x * bins;
+  for (int b = threadIdx.x; b < bins; b += kThreads) hist[b] = count[b];
+}
+
+// Exclusive prefixes over the blocks for 16 digits a workgroup: 64 parts of the blocks,
+// added up, then written in a second sweep.
+constexpr int kScanCols = 16, kScanParts = 64;
+__global__ __launch_bounds__(kScanCols* kScanParts) void sort_scan_kernel(EmbedArgs a, int bits, int blocks) {
+  __shared__ int part[kScanParts][kScanCols + 1];
+  const int cl = threadIdx.x % kScanCols, p = threadIdx.x / kScanCols, bins = 1 << bits;
+  const int b = blockIdx.x * kScanCols + cl;
+  const int per = (blocks + kScanParts - 1) / kScanParts;
+  const int b0 = p * per < blocks ? p * per : blocks, b1 = b0 + per < blocks ? b0 + per : blocks;
+  int s = 0;
+  if (b < bins)
+    for (int i = b0; i < b1; ++i) s += a.hist[(int64_t)i * bins + b];
+  part[p][cl] = s;
+  __syncthreads();
+  int before = 0;
+  for (int q = 0; q < p; ++q) before += part[q][cl];
+  if (b < bins) {
+    for (int i = b0; i < b1; ++i) {
+      int32_t* h = a.hist + (int64_t)i * bins + b;
+      const int n = *h;
+      *h = before;
+      before += n;
+    }
+    if (p == kScanParts - 1) a.totals[b] = before;
+  }
+}
+
+__global__ __launch_bounds__(kThreads) void sort_place_kernel(EmbedArgs a, int from, int to, int shift, int bits,
+                                                              int64_t rpb) {
+  constexpr int W = kThreads / 64;
+  extern __shared__ int next[];        // [W][bins]: counts of a wave's part, then the next place of each digit
+  __shared__ int wave_sum[W];
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, bins = 1 << bits;
+  const int64_t first = blockIdx.x * rpb, last = first + rpb < a.N ? first + rpb : a.N;
+  const int64_t per = (last - first + W * 64 - 1) / (W * 64) * 64;
+  const int64_t lo = first + w * per < last ? first + w * per : last, hi = lo + per < last ? lo + per : last;
+  for (int b = threadIdx.x; b < W * bins; b += kThreads) next[b] = 0;
+  __syncthreads();
+  for (int64_t i = lo + lane; i < hi; i += 64) atomicAdd(&next[w * bins + ((key_at(a, from, i) >> shift) & (bins - 1))], 1);
+  // The digits' first places: an exclusive scan of the totals, each thread a contiguous part.
+  const int chunk = (bins + kThreads - 1) / kThreads;
+  const int b0 = threadIdx.x * chunk < bins ? threadIdx.x * chunk : bins, b1 = b0 + chunk < bins ? b0 + chunk : bins;
+  int s = 0;
+  for (int b = b0; b < b1; ++b) s += a.totals[b];
+  int incl = s;
+#pragma unroll
+  for (int off = 1; off < 64; off *= 2) {
+    const int v = __shfl_up(incl, off);
+    if (lane >= off) incl += v;
+  }
+  if (lane == 63) wave_sum[w] = incl;
+  __syncthreads();
+  int at0 = incl - s;
+  for (int q = 0; q < w; ++q) at0 += wave_sum[q];
+  for (int b = b0; b < b1; ++b) {
+    int at = at0 + a.hist[(int64_t)blockIdx.x * bins + b];
+#pragma unroll
+    for (int q = 0; q < W; ++q) {
+      const int n = next[q * bins + b];
+      next[q * bins + b] = at;
+      at += n;
+    }
+    at0 += a.totals[b];
+  }
+  __syncthreads();
+  for (int64_t i0 = lo; i0 < hi; i0 += 64) {
+    const int64_t i = i0 + lane;
+    const bool in = i < hi;
+    const uint32_t key = in ? key_at(a, from, i) : 0;
+    const int d = (key >> shift) & (bins - 1);
+    uint64_t same = __ballot(in);
+    for (int b = 0; b < bits; ++b) {
+      const uint64_t set = __ballot((d >> b) & 1);
+      same &= (d >> b) & 1 ? set : ~set;
+    }
+    const int rank = __popcll(same & ((1ull << lane) - 1));
+    const int at = next[w * bins + d] + rank;
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    if (in && rank == 0) next[w * bins + d] += __popcll(same);
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    if (in) {
+      a.key[to][at] = key;
+      a.pos[to][at] = from < 0 ? (int32_t)i : a.pos[from][i];
+    }
+  }
+}
+
+// --- sums ---------------------------------------------------------------------
+
+// The first sorted place whose token is v or more.
+__device__ __forceinline__ int64_t lower_bound(const uint32_t* key, int64_t N, uint32_t v) {
+  int64_t lo = 0, hi = N;
+  while (lo < hi) {
+    const int64_t mid = (lo + hi) >> 1;
+    if (key[mid] < v) lo = mid + 1;
+    else hi = mid;
+  }
+  return lo;
+}
+
+template <typename T>
+__device__ __forceinline__ void store_scaled(T* p, int valid, const float (&v)[kVec<T>], float scale) {
+  float o[kVec<T>];
+#pragma unroll
+  for (int i = 0; i < kVec<T>; ++i) o[i] = v[i] * scale;
+  store_row(p, valid, o);
+}
+template <int V>
+__device__ __forceinline__ void store_part(float* p, int valid, const float (&v)[V]) {
+#pragma unroll
+  for (int h = 0; h < V; h += 4) {
+    const float q[4] = {v[h], v[h + 1], v[h + 2], v[h + 3]};
+    if (valid > h) store_row(p + h, valid - h, q);
+  }
+}
+
+// The first `tiles` workgroups along x add tiles, the others zero rows without a token (64 rows each).  tx threads
+// share a tile's columns; y counts columns of tx V.
+template <typename T, bool SHORT>
+__global__ __launch_bounds__(kThreads) void embed_sum_kernel(EmbedArgs a, int tx, int64_t tile_blocks, int sorted) {
+  constexpr int V = kVec<T>, U = 8;
+  const uint32_t* key = a.key[sorted];
+  T* out = static_cast<T*>(a.out);
+  if ((int64_t)blockIdx.x >= tile_blocks) {
+    __shared__ int64_t first[65];
+    const int64_t v0 = ((int64_t)blockIdx.x - tile_blocks) * 64;
+    if (threadIdx.x <= 64) first[threadIdx.x] = lower_bound(key, a.N, (uint32_t)(v0 + threadIdx.x < a.V ? v0 + threadIdx.x : a.V));
+    __syncthreads();
+    const int lane = threadIdx.x & (tx - 1), step = kThreads / tx;
+    float zero[V] = {};
+    const int c = ((int)blockIdx.y * tx + lane) * V;
+    if (c < a.D)
+      for (int r = threadIdx.x / tx; r < 64 && v0 + r < a.V; r += step)
+        if (first[r] == first[r + 1]) store_row(out + (v0 + r) * a.D + c, a.D - c, zero);
+    return;
+  }
+  const int lane = threadIdx.x & (tx - 1), sub = threadIdx.x / tx, per = kThreads / tx;
+  __shared__ uint32_t keys[kThreads / 8][kTile + 2];
+  __shared__ int32_t pos[kThreads / 8][kTile];
+  // the tokens of this workgroup's tiles, and of the places before and after each
+  const int64_t t0 = (int64_t)blockIdx.x * per;
+  for (int i = threadIdx.x; i < per * (kTile + 2); i += kThreads) {
+    const int64_t at = (t0 + i / (kTile + 2)) * kTile + i % (kTile + 2) - 1;
+    keys[i / (kTile + 2)][i % (kTile + 2)] = at >= 0 && at < a.N ? key[at] : (uint32_t)a.V;
+  }
+  for (int i = threadIdx.x; i < per * kTile; i += kThreads) {
+    const int64_t at = t0 * kTile + i;
+    const int32_t p = at < a.N ? a.pos[sorted][at] : 0;
+    pos[i / kTile][i % kTile] = p;
+  }
+  __syncthreads();
+  const int c = ((int)blockIdx.y * tx + lane) * V;
+  const int64_t tile = t0 + sub;
+  if (c >= a.D || tile * kTile >= a.N) return;
+  const uint32_t none = (uint32_t)a.V;
+  const uint32_t* k = keys[sub] + 1;
+  const T* dy = static_cast<const T*>(a.dy);
+  float acc[V] = {};
+  bool entered = k[-1] == k[0] && tile > 0;        // the run at hand began in an earlier tile
+  for (int i0 = 0; i0 < kTile; i0 += U) {
+    if (k[i0] == none) break;                      // (the others follow)
+    uint4 u[U];
+#pragma unroll
+    for (int j = 0; j < U; ++j) u[j] = fetch16<SHORT>(dy + (int64_t)pos[sub][i0 + j] * a.lddy + c, a.D - c);
+#pragma unroll
+    for (int j = 0; j < U; ++j) {
+      const uint32_t at = k[i0 + j];
+      if (at == none) break;
+      float v[V];
+      unpack16<T>(keep16<SHORT, T>(u[j], a.D - c, a.D), v);
+#pragma unroll
+      for (int i = 0; i < V; ++i) acc[i] += v[i];
+      const bool leaves = i0 + j == kTile - 1 && k[kTile] == at;
+      if (k[i0 + j + 1] == at && !leaves) continue;
+      if (entered || leaves) store_part(a.part + (tile * 2 + !entered) * a.D + c, a.D - c, acc);
+      else store_scaled(out + (int64_t)at * a.D + c, a.D - c, acc, a.scale);
+#pragma unroll
+      for (int i = 0; i < V; ++i) acc[i] = 0.f;
+      entered = false;
+    }
+  }
+}
+
+// The runs that leave the tile in which they began: that tile's part and those of the tiles after it.  A workgroup
+// takes a tile and 64 V columns, its four waves contiguous parts of the run.
+template <typename T>
+__global__ __launch_bounds__(kThreads) void embed_join_kernel(EmbedArgs a, int sorted) {
+  constexpr int V = 4, W = kThreads / 64;
+  const uint32_t* key = a.key[sorted];
+  const int64_t tiles = (a.N + kTile - 1) / kTile;
+  __shared__ float sums[W][64][V + 1];
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+  const int c = ((int)blockIdx.y * 64 + lane) * V;
+  for (int64_t tile = blockIdx.x; tile + 1 < tiles; tile += gridDim.x) {
+    const int64_t last = tile * kTile + kTile - 1;
+    const uint32_t v = key[last];
+    if (v == (uint32_t)a.V || key[last + 1] != v || (key[tile * kTile] == v && tile > 0 && key[tile * kTile - 1] == v))
+      continue;
+    const int64_t end = lower_bound(key, a.N, v + 1);           // of the run
+    const int64_t parts = (end - 1) / kTile - tile;             // tiles after this one
+    const int64_t per = (parts + W - 1) / W, lo = w * per < parts ? w * per : parts, hi = lo + per < parts ? lo + per : parts;
+    float acc[V] = {};
+    if (c < a.D) {
+      const float* p = a.part + (tile + 1) * 2 * a.D + c;
+      if (w == 0) {
+#pragma unroll
+        for (int i = 0; i < V; ++i) if (c + i < a.D) acc[i] = a.part[(tile * 2 + 1) * a.D + c + i];
+      }
+#pragma unroll 8
+      for (int64_t q = lo; q < hi; ++q)
+#pragma unroll
+        for (int i = 0; i < V; ++i) if (c + i < a.D) acc[i] += p[q * 2 * a.D + i];
+    }
+#pragma unroll
+    for (int i = 0; i < V; ++i) sums[w][lane][i] = acc[i];
+    __syncthreads();
+    if (w == 0 && c < a.D) {
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        float s = acc[i];
+#pragma unroll
+        for (int q = 1; q < W; ++q) s += sums[q][lane][i];
+        if (c + i < a.D) static_cast<T*>(a.out)[(int64_t)v * a.D + c + i] = (T)(s * a.scale);
+      }
+    }
+    __syncthreads();
+  }
+}
+
+int threads_for(int nvec) {
+  int tx = 8;
+  while (tx < nvec && tx < kThreads) tx *= 2;
+  return tx;
+}
+
+template <typename T>
+void embed_typed(const EmbedArgs& a, hipStream_t s) {
+  const int tx = threads_for((a.D + kVec<T> - 1) / kVec<T>);
+  const int64_t rows = kThreads / tx * 4, need = (a.N + rows - 1) / rows;
+  const unsigned grid = (unsigned)(need < kMaxBlocks ? need : kMaxBlocks);
+  if (a.D < kVec<T>) embed_kernel<T, true><<<grid, kThreads, 0, s>>>(a, tx);
+  else embed_kernel<T, false><<<grid, kThreads, 0, s>>>(a, tx);
+}
+
+template <typename T>
+void embed_sum_typed(const EmbedArgs& a, int sorted, hipStream_t s) {
+  const int nvec = (a.D + kVec<T> - 1) / kVec<T>, tx = threads_for(nvec), per = kThreads / tx;
+  const int64_t tiles = (a.N + kTile - 1) / kTile, tile_blocks = (tiles + per - 1) / per;
+  const dim3 grid((unsigned)(tile_blocks + (a.V + 63) / 64), (unsigned)((nvec + tx - 1) / tx));
+  if (a.D < kVec<T>) embed_sum_kernel<T, true><<<grid, kThreads, 0, s>>>(a, tx, tile_blocks, sorted);
+  else embed_sum_kernel<T, false><<<grid, kThreads, 0, s>>>(a, tx, tile_blocks, sorted);
+  if (tiles > 1) {
+    const dim3 join((unsigned)(tiles - 1 < 65536 ? tiles - 1 : 65536), (unsigned)((a.D + 255) / 256));
+    embed_join_kernel<T><<<join, kThreads, 0, s>>>(a, sorted);
+  }
+}
+
+int64_t align256(int64_t v) { return (v + 255) / 256 * 256; }
+
+}  // namespace
+
+int64_t embed_workspace_bytes(int64_t N, int64_t V, int D) {
+  EmbedArgs a{};
+  a.N = N; a.V = V; a.D = D;
+  embed_workspace(a, nullptr);
+  const int64_t tiles = (N + kTile - 1) / kTile;
+  return reinterpret_cast<int64_t>(a.part) + align256(tiles * 2 * D * 4);
+}
+
+void embed_workspace(EmbedArgs& a, void* ws) {
+  char* p = static_cast<char*>(ws);
+  auto take = [&](auto*& at, int64_t bytes) {
+    at = reinterpret_cast<std::decay_t<decltype(at)>>(p);
+    p += align256(bytes);
+  };
+  const int64_t rpb = sort_rows(a.N), blocks = (a.N + rpb - 1) / rpb;
+  const int bits = key_bits(a.V), passes = (bits + kMaxBits - 1) / kMaxBits, digit = (bits + passes - 1) / passes;
+  for (int i = 0; i < 2; ++i) take(a.key[i], a.N * 4);
+  for (int i = 0; i < 2; ++i) take(a.pos[i], a.N * 4);
+  take(a.hist, blocks * (int64_t(1) << digit) * 4);
+  take(a.totals, (int64_t(1) << digit) * 4);
+  a.part = reinterpret_cast<float*>(p);
+}
+
+void launch_embed(const EmbedArgs& a, hipStream_t s) {
+  if (a.elem == ELEM_F32) embed_typed<float>(a, s);
+  else if (a.elem == ELEM_BF16) embed_typed<__bf16>(a, s);
+  else embed_typed<_Float16>(a, s);
+}
+
+void launch_embed_bwd(const EmbedArgs& a, hipStream_t s) {
+  const int64_t rpb = sort_rows(a.N);
+  const unsigned blocks = (unsigned)((a.N + rpb - 1) / rpb);
+  const int all = key_bits(a.V), passes = (all + kMaxBits - 1) / kMaxBits, bits = (all + passes - 1) / passes;
+  int from = -1;
+  for (int p = 0; p < passes; ++p) {
+    const int to = p & 1, bins = 1 << bits;
+    sort_count_kernel<<<blocks, kThreads, bins * 4, s>>>(a, from, p * bits, bits, rpb);
+    sort_scan_kernel<<<(bins + kScanCols - 1) / kScanCols, kScanCols * kScanParts, 0, s>>>(a, bits, (int)blocks);
+    sort_place_kernel<<<blocks, kThreads, kThreads / 64 * bins * 4, s>>>(a, from, to, p * bits, bits, rpb);
+    from = to;
+  }
+  if (a.elem == ELEM_F32) embed_sum_typed<float>(a, from, s);
+  else if (a.elem == ELEM_BF16) embed_sum_typed<__bf16>(a, from, s);
+  else embed_sum_typed<_Float16>(a, from, s);
+}
+
+}  // namespace gx::layer

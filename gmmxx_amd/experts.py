@@ -88,7 +88,9 @@ def _rows(t: torch.Tensor) -> torch.Tensor:
 
 _ENTRY_POINTS = ("last_error", "layer_norm", "layer_norm_workspace_bytes", "layer_norm_backward",
                  "route_workspace_bytes", "route", "route_backward", "grouped_matmul", "grouped_workspace_bytes",
-                 "grouped_weight_grad", "combine", "combine_backward")
+                 "grouped_weight_grad", "combine", "combine_backward", "embed", "embed_workspace_bytes",
+                 "embed_backward", "dropout", "log_probs_workspace_bytes", "log_probs", "log_probs_backward",
+                 "quantize", "quantized_matmul")
 _ops = None
 
 

@@ -374,6 +374,70 @@ int gmmxx_hip_combine_backward(int elem, int64_t N, int64_t k, int64_t E, int64_
                                const float* gates, const int32_t* slots, const int32_t* offsets, const void* dout,
                                int64_t lddout, void* dy, float* dgates, void* stream);
 
+/* -------------------------------------------------------------------------
+ * Token operators: rows of a table by token (a mixture's labels, or any codes),
+ * dropout, log probabilities of tokens under rows of scores, and products of rows
+ * in 8-bit integers.  No reference counterpart.  Elements, rows and strides as in
+ * the section above; token indices have 32 or 64 bits (index_bits), and one outside
+ * 0 .. V - 1 stands for no token.
+ * ------------------------------------------------------------------------- */
+
+/* out[n] = scale table[index[n]] for N < 2^30 tokens and a table of V <= 2^24 rows of
+ * D <= 2^22 elements (N D and V D at most 2^40); zeros where there is no token.  scale
+ * is finite; the product is rounded once. */
+int gmmxx_hip_embed(int elem, int64_t N, int64_t V, int64_t D, const void* table, int64_t ldt, const void* index,
+                    int index_bits, double scale, void* out, void* stream);
+
+/* dtable[v] = scale times the sum of dy[n] over the places n with token v, in the
+ * order of the places: fp32, rounded once; zeros in rows without a place.  The
+ * workspace takes gmmxx_hip_embed_workspace_bytes.  With N = 0 nothing is written. */
+int64_t gmmxx_hip_embed_workspace_bytes(int64_t N, int64_t V, int64_t D);
+int gmmxx_hip_embed_backward(int elem, int64_t N, int64_t V, int64_t D, const void* dy, int64_t lddy,
+                             const void* index, int index_bits, double scale, void* dtable, void* workspace,
+                             int64_t workspace_bytes, void* stream);
+
+/* out[i] = (word(i) >= round(p 2^32) ? x[i] / (1 - p) : 0) + residual[i] for n adjacent
+ * elements (residual NULL: none), 0 <= p <= 1.  word(i) is word i % 4 of Philox 4x32-10
+ * with counter (i / 4, offset) and key seed, or *seed_at, which the kernel reads, where
+ * seed_at is not NULL.  The gradient of x is the same call on dy without a residual. */
+int gmmxx_hip_dropout(int elem, int64_t n, double p, uint64_t seed, const int64_t* seed_at, uint64_t offset,
+                      const void* x, const void* residual, void* out, void* stream);
+
+/* For each of N rows of V <= 2^22 scores, with p the softmax over the row's candidates
+ * (scores that are neither -inf nor NaN; of several +inf each weighs the same):
+ *   chosen (N): log p of the row's token; -inf where it is no candidate, 0 without one;
+ *   entropy (N): -sum p log p, 0 in a row without candidates;
+ *   top, top_index (N, k), k <= min(V, 64): the k largest log p and where they are, the lower
+ *     index first among equals; -inf and -1 where no candidate is left;
+ *   stats (N, 3; NULL: not wanted): what the backward pass reads. */
+int64_t gmmxx_hip_log_probs_workspace_bytes(int64_t N, int64_t V, int64_t k);
+int gmmxx_hip_log_probs(int elem, int64_t N, int64_t V, int64_t k, const void* scores, int64_t ld, const void* index,
+                        int index_bits, float* chosen, float* entropy, float* top, int32_t* top_index, float* stats,
+                        void* workspace, int64_t workspace_bytes, void* stream);
+
+/* dscores (N, V) from the gradients of chosen and entropy (N) and top (N, k), each of
+ * which may be NULL; zeros at what is no candidate. */
+int gmmxx_hip_log_probs_backward(int elem, int64_t N, int64_t V, int64_t k, const void* scores, int64_t ld,
+                                 const void* index, int index_bits, const int32_t* top_index, const float* stats,
+                                 const float* dchosen, const float* dentropy, const float* dtop, void* dscores,
+                                 void* stream);
+
+/* N rows of D <= 2^17 elements in 8 bits: with a the largest absolute value of a row,
+ * values = round(x (127 / a)) (ties to even) and scales = a / 127, in fp32.  A row of zeros has
+ * scale 0, a row with a NaN or an infinity scale NaN and values 0.  Rows of values lie ldv
+ * apart, a multiple of 16 that is at least D, from a multiple of 16 on; zeros follow the
+ * D values up to the next multiple of 16. */
+int gmmxx_hip_quantize(int elem, int64_t N, int64_t D, const void* x, int64_t ldx, int8_t* values, int64_t ldv,
+                       float* scales, void* stream);
+
+/* out[n][f] = (sum over d of x[n][d] w[f][d]) xscales[n] wscales[f] + bias[f] (bias NULL: none;
+ * of `elem`, as out).  The sum is exact.  Rows lie multiples of 16 bytes (at most 2^23) apart
+ * from a multiple of 16 on, and may be read up to the next multiple of 16 after their D values,
+ * whatever is there. */
+int gmmxx_hip_quantized_matmul(int elem, int64_t N, int64_t F, int64_t D, const int8_t* x, int64_t ldx,
+                               const float* xscales, const int8_t* w, int64_t ldw, const float* wscales,
+                               const void* bias, void* out, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,209 @@
+"""log_probs against its definition in 64 bits: row lengths, counts and alternatives at which the kernels change
+their ways, ties, masked and empty rows, infinities and NaN, places that do not count, and the gradients of all
+three results against the formula and against differences."""
+
+import pytest
+import torch
+
+import gmmxx_amd
+from tests import experts_ref, tokens_ref as ref
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
+F32, BF16, F16 = experts_ref.DTYPES
+INF = float("inf")
+
+
+def make(n, v, dtype, seed=0, spread=3.0):
+    g = torch.Generator().manual_seed(seed)
+    s = (spread * torch.randn((n, v), generator=g)).to(dtype)
+    t = torch.randint(0, v, (n,), generator=g)
+    t[3::7] = -1
+    return s.to(DEV), t.to(DEV)
+
+
+def compare(got, want):
+    for name in ("chosen", "entropy", "top"):
+        experts_ref.close(getattr(got, name), *want[name], name)
+    assert got.top_index.dtype == torch.int32
+    assert torch.equal(got.top_index.cpu().long(), want["top_index"][0]), "top_index"
+
+
+def check(s, t, k, seed=0):
+    n = s.shape[0]
+    g = torch.Generator().manual_seed(seed)
+    dc, dh, dt = (torch.randn(sh, generator=g).to(DEV) for sh in ((n,), (n,), (n, k)))
+    leaf = s.detach().requires_grad_()
+    r = gmmxx_amd.log_probs(leaf, t, top_k=k)
+    outs, grads = (r.chosen, r.entropy, r.top), (dc, dh, dt)
+    if k == 0:
+        outs, grads = outs[:2], grads[:2]
+    ds, = torch.autograd.grad(outs, leaf, grads)
+    want = ref.log_probs(s, t, k, dc, dh, dt if k else None)
+    compare(r, want)
+    assert ds.dtype == s.dtype
+    experts_ref.close(ds, *want["dscores"], "dscores")
+    plain = gmmxx_amd.log_probs(s, t, top_k=k)
+    assert all(torch.equal(a, b) for a, b in zip(plain, r))
+
+
+LENGTHS = [1, 2, 3, 4, 7, 8, 9, 31, 63, 100, 127, 128, 129, 500, 512, 513, 1000, 2047, 2048, 2049, 4095, 4097, 8193, 20001,
+           65536, 131073]
+
+
+@pytest.mark.parametrize("dtype", experts_ref.DTYPES, ids=str)
+@pytest.mark.parametrize("v", LENGTHS)
+def test_lengths(hip, v, dtype):
+    for k in sorted({0, 1, min(v, 5), min(v, 64)}):
+        print(f"[log_probs] v={v} k={k} {dtype}", flush=True)
+        check(*make(5, v, dtype, seed=v), k)
+
+
+@pytest.mark.parametrize("n", [1, 2, 3, 17, 64, 257, 1025, 3000])
+@pytest.mark.parametrize("v,k", [(77, 0), (77, 3), (300, 0), (2100, 0), (5001, 4)])
+def test_counts(hip, n, v, k):
+    print(f"[log_probs] n={n} v={v} k={k}", flush=True)
+    check(*make(n, v, BF16, seed=n), k)
+
+
+@pytest.mark.parametrize("v", [6, 700, 3000, 40_000])
+@pytest.mark.parametrize("k", [0, 4])
+@pytest.mark.parametrize("dtype", experts_ref.DTYPES, ids=str)
+def test_masks(hip, v, k, dtype):
+    """Masks of -inf, of the type's lowest value and of NaN; rows of each alone; one candidate; some +inf."""
+    print(f"[log_probs] masks v={v} k={k} {dtype}", flush=True)
+    s, t = make(13, v, dtype)
+    low = torch.finfo(dtype).min
+    off = torch.rand((13, v), generator=torch.Generator().manual_seed(1)).to(DEV) < 0.4
+    s[0][off[0]] = -INF
+    s[1][off[1]] = low
+    s[2][off[2]] = float("nan")
+    s[3], s[4], s[5] = -INF, low, float("nan")
+    s[6] = -INF
+    s[6, v - 1] = 2.0
+    s[7, 1], s[7, v - 1] = INF, INF
+    s[8] = INF
+    s[9], s[9, 2] = -INF, low
+    s[10, v // 2] = INF
+    s[11] = -INF
+    s[11, ::2] = float("nan")
+    s[12] = 0.0
+    t[:] = torch.arange(13, device=DEV) % min(v, 5)
+    t[8] = -5
+    t[9] = 2
+    check(s, t, k)
+
+
+@pytest.mark.parametrize("v", [200, 10_000, 100_000])
+@pytest.mark.parametrize("order", ["equal", "ascending", "descending", "two values", "few"])
+def test_orders(hip, v, order):
+    """Rows whose order or ties fill the list of alternatives: the lower index comes first."""
+    print(f"[log_probs] {order} v={v}", flush=True)
+    i = torch.arange(v, dtype=torch.float32)
+    row = {"equal": torch.zeros(v), "ascending": i / v, "descending": -i / v, "two values": (i % 7 == 3).float(),
+           "few": torch.where(i % (v // 5) == 9, i / v, torch.full((v,), -INF))}[order]
+    s = torch.stack([row, row.flip(0)]).to(DEV)
+    for k in (1, 64):
+        check(s, torch.tensor([v - 1, 9], device=DEV), k)
+
+
+def test_many_rows_of_ties(hip):
+    s = torch.randint(0, 3, (2000, 9000), generator=torch.Generator().manual_seed(0)).to(BF16).to(DEV)
+    r = gmmxx_amd.log_probs(s, torch.zeros(2000, dtype=torch.int64, device=DEV), top_k=20)
+    want = torch.sort(s.float(), dim=1, descending=True, stable=True).indices[:, :20]
+    assert torch.equal(r.top_index.long(), want)
+
+
+@pytest.mark.parametrize("scale", [1e-3, 1.0, 30.0, 1000.0])
+@pytest.mark.parametrize("v", [400, 9000])
+def test_spreads(hip, scale, v):
+    check(*make(6, v, F32, spread=scale), 3)
+    s, t = make(6, v, F32, spread=scale)
+    check(s + 5000.0, t, 0)                # far from zero
+
+
+@pytest.mark.parametrize("dtype", experts_ref.DTYPES, ids=str)
+@pytest.mark.parametrize("v", [150, 5000])
+def test_strides_and_types(hip, dtype, v):
+    s, t = make(12, v, dtype)
+    wide = torch.full((12, v + 50), 30.0, dtype=dtype, device=DEV)
+    wide[:, 33:33 + v] = s
+    for k in (0, 3):
+        check(wide[:, 33:33 + v], t.int(), k)
+        check(s.t().contiguous().t(), torch.stack([t, t], 1)[:, 0], k)
+    r = gmmxx_amd.log_probs(s.reshape(3, 4, v), t.reshape(3, 4), top_k=2)
+    want = gmmxx_amd.log_probs(s, t, top_k=2)
+    assert r.top.shape == (3, 4, 2) and all(torch.equal(a.reshape(b.shape), b) for a, b in zip(r, want))
+    one = gmmxx_amd.log_probs(s[0], t[0], top_k=2)
+    assert one.chosen.shape == () and torch.equal(one.top_index, want.top_index[0])
+
+
+def test_some_gradients(hip):
+    """Each result's gradient alone."""
+    s, t = make(9, 300, F32)
+    dc, dh, dt = torch.randn(9), torch.randn(9), torch.randn(9, 3)
+    for which in ("chosen", "entropy", "top"):
+        leaf = s.detach().requires_grad_()
+        r = gmmxx_amd.log_probs(leaf, t, top_k=3)
+        g = {"chosen": dc, "entropy": dh, "top": dt}[which]
+        ds, = torch.autograd.grad(getattr(r, which), leaf, g.to(DEV))
+        experts_ref.close(ds, *ref.log_probs(s, t, 3, **{"d" + which: g})["dscores"], which)
+    leaf = s.detach().requires_grad_()
+    gmmxx_amd.log_probs(leaf, t).chosen.sum().backward()          # a gradient with strides of zero
+    experts_ref.close(leaf.grad, *ref.log_probs(s, t, 0, dchosen=torch.ones(9))["dscores"], "ones")
+
+
+def test_differences(hip):
+    """Gradients against central differences of the 64-bit form."""
+    s, t = make(4, 11, F32)
+    leaf = s.detach().requires_grad_()
+    r = gmmxx_amd.log_probs(leaf, t, top_k=2)
+    w = [torch.randn(sh, generator=torch.Generator().manual_seed(5)) for sh in ((4,), (4,), (4, 2))]
+    ds, = torch.autograd.grad((r.chosen, r.entropy, r.top), leaf, [x.to(DEV) for x in w])
+
+    def value(x):
+        o = ref.log_probs(x, t, 2)
+        return sum(float((o[name][0] * wi.double()).sum()) for name, wi in zip(("chosen", "entropy", "top"), w))
+
+    base, h = s.double().cpu(), 1e-5
+    for r0 in range(4):
+        for c in range(11):
+            up, down = base.clone(), base.clone()
+            up[r0, c] += h
+            down[r0, c] -= h
+            # the difference's own error: h^2 / 6 times third derivatives (of order 10), and the values' rounding over h
+            assert abs((value(up) - value(down)) / (2 * h) - float(ds[r0, c])) < 1e-4
+
+
+def test_no_rows(hip):
+    s, t = make(3, 20, F32)
+    leaf = s[:0].detach().requires_grad_()
+    r = gmmxx_amd.log_probs(leaf, t[:0], top_k=2)
+    assert r.chosen.shape == (0,) and r.top.shape == (0, 2)
+    assert torch.autograd.grad(r.chosen.sum() + r.entropy.sum(), leaf)[0].shape == (0, 20)
+
+
+def test_tokens_outside(hip):
+    s, t = make(6, 50, F32)
+    for bad in (-1, -100, 50, 1 << 40, -(1 << 40)):
+        t[:] = bad
+        leaf = s.detach().requires_grad_()
+        r = gmmxx_amd.log_probs(leaf, t)
+        assert not r.chosen.any()
+        assert not torch.autograd.grad(r.chosen.sum(), leaf)[0].any()
+
+
+def test_past_32_bits(hip):
+    """Scores past 2^31 elements and 2^32 bytes, at the far rows."""
+    n, v = 36_000, 65_536
+    s = torch.empty((n, v), dtype=BF16, device=DEV)
+    for i in range(0, n, 4000):
+        s[i:i + 4000].normal_()
+    t = torch.randint(0, v, (n,), device=DEV)
+    leaf = s.requires_grad_()
+    r = gmmxx_amd.log_probs(leaf, t, top_k=2)
+    far = torch.tensor([0, 1, n // 2, n - 1], device=DEV)
+    want = ref.log_probs(s.detach()[far], t[far], 2, dchosen=torch.ones(4))
+    compare(gmmxx_amd.LogProbs(*(x[far] for x in r)), want)
+    ds, = torch.autograd.grad(r.chosen.sum(), leaf)
+    experts_ref.close(ds[far], *want["dscores"], "dscores")
