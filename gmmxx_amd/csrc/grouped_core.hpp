@@ -66,18 +66,6 @@ __device__ __forceinline__ int xcd_tile(int id, int total) {
   return x * per + (x < rest ? x : rest) + id / 8;
 }
 
-// op over lanes 0 .. l in lane l, for values that are not negative (0 changes nothing): within rows of 16 lanes,
-// then across them.
-template <typename F>
-__device__ __forceinline__ int lanes_scan(int v, F&& op) {
-  v = op(v, __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, false));      // shifted by 1, 2, 4 and 8 lanes
-  v = op(v, __builtin_amdgcn_update_dpp(0, v, 0x112, 0xF, 0xF, false));
-  v = op(v, __builtin_amdgcn_update_dpp(0, v, 0x114, 0xF, 0xF, false));
-  v = op(v, __builtin_amdgcn_update_dpp(0, v, 0x118, 0xF, 0xF, false));
-  v = op(v, __builtin_amdgcn_update_dpp(0, v, 0x142, 0xA, 0xF, false));      // lane 15 to rows 1 and 3
-  return op(v, __builtin_amdgcn_update_dpp(0, v, 0x143, 0xC, 0xF, false));   // lane 31 to rows 2 and 3
-}
-
 // The tile of workgroup `id`: its group, positions (BM a tile) and column tile (of `ntiles`, innermost).
 // Group E is the rows past the last group.  False: there is no such tile; the grid holds the most that
 // ascending offsets can give.  Every wave counts the groups' tiles for itself, 256 groups at a time: four a lane,

@@ -8,19 +8,22 @@
 // p = 1 / their number.  The gradient from g (chosen), h (entropy) and q (alternatives) is
 //   ds_j = g [j = t] + Σ_i q_i [j = top_i] - p_j (g + Σ_i q_i + h (log p_j + H)).
 //
-// One pass over the scores: a thread keeps its own (m, Z, U), brought to a larger m where
-// one comes up (once a 16-byte vector at most), and the threads' are merged at the end, in
-// a fixed order.  Rows are cut into parts where there are too few for the card, and joined by
+// One pass over the scores: a thread keeps its own sums beside a reference near its largest score, brought to a
+// larger one where that comes up (once a 16-byte vector at most), and the threads' are merged at the
+// end, in a fixed order.  Rows are cut into parts where there are too few for the card, and joined by
 // a second kernel.
 //
 // Alternatives are found in the same pass.  A score's rank is a 64-bit number, its value
 // above its complemented index, so no two are equal and ties go to the lower index.  The
 // first scores give a bound that k of them reach; scores that reach the bound go to a list in LDS,
-// which is cut back to its k largest when it may overflow (its k-th by bisection over the
-// rank's bits) and raises the bound.  The list's order depends on the waves', what is kept of it
+// which is cut back to its k largest where it would overflow (its k-th by bisection over the
+// rank's bits), which raises the bound.  The list's order depends on the waves', what is kept of it
 // does not.
 
+#include <float.h>
 #include <math.h>
+
+#include <algorithm>
 
 #include "rows.hpp"
 #include "tokens.hpp"
@@ -38,28 +41,29 @@ __device__ __forceinline__ float exp_below(float& d) {
   return fast_exp2(d * kLog2e);
 }
 
-// Scores seen: the largest, Σ e^(s - m), Σ e^(s - m) (s - m).  m = -inf: none yet.  A largest of +inf leaves sums
-// that do not count (see finish).
-struct Stats {
-  float m = -INFINITY, z = 0.f, u = 0.f;
-  __device__ __forceinline__ void raise(float to) {      // to >= m
-    const float by = m - to;
-    if (by == 0.f || m == to) return;
-    const float f = m == -INFINITY ? 0.f : __expf(fmaxf(by, -110.f));
+// Scores taken in by one thread, as the slow form: the largest (`ref`), Σ e^(s - m), Σ e^(s - m) (s - m).  -inf: none yet.  A largest
+// of +inf leaves sums that do not count (see resolve).
+struct Plain {
+  float ref = -INFINITY, z = 0.f, u = 0.f;
+  __device__ __forceinline__ void raise(float to) {      // to >= ref
+    const float by = ref - to;
+    if (by == 0.f || ref == to) return;
+    const float f = ref == -INFINITY ? 0.f : __expf(fmaxf(by, -110.f));
     u = f == 0.f ? 0.f : f * fmaf(z, by, u);
     z *= f;
-    m = to;
+    ref = to;
   }
+  // (no s is +inf)
   template <int V>
   __device__ __forceinline__ void add(const float (&s)[V]) {
-    float top = s[0];
+    float top = -INFINITY;
 #pragma unroll
-    for (int i = 1; i < V; ++i) top = fmaxf(top, s[i]);
-    if (top > m) raise(top);
+    for (int i = 0; i < V; ++i) top = fmaxf(top, s[i]);
+    if (top > ref) raise(top);
     float zv = 0.f, uv = 0.f;
 #pragma unroll
     for (int i = 0; i < V; ++i) {
-      float d = s[i] - m;
+      float d = s[i] - ref;
       const float e = exp_below(d);
       zv += e;
       uv = fmaf(e, d, uv);
@@ -69,8 +73,55 @@ struct Stats {
   }
 };
 
-__device__ __forceinline__ Stats merge(Stats a, Stats b) {
-  const float to = fmaxf(a.m, b.m);
+// The same in half the instructions: sums of 2^l and 2^l l with l = s L - ref, L = log2(e) in fp32, where ref
+// need not be the largest s L, only near it.  Where a vector's sum passes 2^10, ref is raised to
+// its largest.  A ref that is not finite at the end (no score, or scores past 2^100) says that the row is to be
+// taken in as Plain.
+constexpr float kFar = 0x1p100f;
+struct Lean {
+  float ref = -INFINITY, z = 0.f, u = 0.f;
+  __device__ __forceinline__ void raise(float to) {
+    const float by = ref - to;
+    if (ref == to) return;
+    const float f = ref == -INFINITY ? 0.f : fast_exp2(fmaxf(by, -160.f));
+    u = f == 0.f ? 0.f : f * fmaf(z, by, u);
+    z *= f;
+    ref = to;
+  }
+  template <int V>
+  __device__ __forceinline__ void sums(const float (&s)[V], float& zv, float& uv) const {
+    zv = uv = 0.f;
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      const float l = fmaxf(fmaf(s[i], kLog2e, -ref), -160.f);      // (-inf and NaN too: 2^l is 0)
+      const float e = fast_exp2(l);
+      zv += e;
+      uv = fmaf(e, l, uv);
+    }
+  }
+  template <int V>
+  __device__ __forceinline__ void add(const float (&s)[V]) {
+    float zv, uv;
+    sums(s, zv, uv);
+    if (!(zv <= 1024.f)) {
+      float top = -INFINITY;
+#pragma unroll
+      for (int i = 0; i < V; ++i) top = fmaxf(top, s[i]);
+      if (top <= -kFar) {                              // (beside any other score they weigh nothing)
+        if (ref == -INFINITY && top > -INFINITY) z = 1.f;
+        return;
+      }
+      raise(top < kFar ? fmaxf(ref, top * kLog2e) : INFINITY);
+      sums(s, zv, uv);
+    }
+    z += zv;
+    u += uv;
+  }
+};
+
+template <typename S>
+__device__ __forceinline__ S merge(S a, S b) {
+  const float to = fmaxf(a.ref, b.ref);
   a.raise(to);
   b.raise(to);
   a.z += b.z;
@@ -78,30 +129,31 @@ __device__ __forceinline__ Stats merge(Stats a, Stats b) {
   return a;
 }
 
-// The statistics of G lanes' scores, in all of them.
-template <int G>
-__device__ __forceinline__ Stats lanes_merge(Stats s) {
-  const float to = lanes_reduce<G>(s.m, [](float a, float b) { return fmaxf(a, b); });
+// What G lanes took in, in all of them.
+template <int G, typename S>
+__device__ __forceinline__ S lanes_merge(S s) {
+  const float to = lanes_reduce<G>(s.ref, [](float a, float b) { return fmaxf(a, b); });
   s.raise(to);
   s.z = lanes_sum<G>(s.z);
   s.u = lanes_sum<G>(s.u);
   return s;
 }
 
-// ... of a workgroup's; `red` takes three floats a wave.
-__device__ __forceinline__ Stats block_merge(Stats s, float (*red)[3]) {
+// ... what a workgroup did; `red` takes three floats a wave.
+template <typename S>
+__device__ __forceinline__ S block_merge(S s, float (*red)[3]) {
   s = lanes_merge<64>(s);
   if ((threadIdx.x & 63) == 0) {
-    red[threadIdx.x >> 6][0] = s.m;
+    red[threadIdx.x >> 6][0] = s.ref;
     red[threadIdx.x >> 6][1] = s.z;
     red[threadIdx.x >> 6][2] = s.u;
   }
   __syncthreads();
-  Stats r;
-  r.m = red[0][0], r.z = red[0][1], r.u = red[0][2];
+  S r;
+  r.ref = red[0][0], r.z = red[0][1], r.u = red[0][2];
   for (int w = 1; w < (int)blockDim.x / 64; ++w) {
-    Stats o;
-    o.m = red[w][0], o.z = red[w][1], o.u = red[w][2];
+    S o;
+    o.ref = red[w][0], o.z = red[w][1], o.u = red[w][2];
     r = merge(r, o);
   }
   return r;
@@ -112,36 +164,91 @@ __device__ __forceinline__ int64_t token_at(const LogpArgs& a, int64_t n) {
   return (uint64_t)t < (uint64_t)a.V ? t : -1;
 }
 
-// log p of a score v in a row with largest m.
+// log p of a score v: m and log Z need not be the largest score's, only belong together.
 __device__ __forceinline__ float log_p(float v, float m, float logz) {
   return v > -INFINITY ? (v == m ? -logz : (v - m) - logz) : -INFINITY;
 }
 
-// A row's results, by one thread.
-template <typename T>
-__device__ __forceinline__ float2 finish(const LogpArgs& a, int64_t n, Stats s) {
-  const bool some = s.m > -INFINITY;
-  const float logz = some ? logf(s.z) : 0.f, h = some ? logz - s.u / s.z : 0.f;
-  const int64_t t = token_at(a, n);
-  a.chosen[n] = t < 0 ? 0.f : log_p(to_f32(static_cast<const T*>(a.scores)[n * a.lds + t]), s.m, logz);
-  a.entropy[n] = h;
-  if (a.stats) {
-    a.stats[n * 3] = s.m;
-    a.stats[n * 3 + 1] = logz;
-    a.stats[n * 3 + 2] = h;
-  }
-  return make_float2(s.m, logz);
+struct Row { float m, logz, entropy; };
+
+__device__ __forceinline__ Row resolved(Plain s) {
+  if (!(s.ref > -INFINITY)) return Row{-INFINITY, 0.f, 0.f};
+  const float logz = logf(s.z);
+  return Row{s.ref, logz, logz - s.u / s.z};
+}
+// 2^ref = e^M exactly with M = ref / L: m is M in fp32, and what that rounds off goes to log Z.
+__device__ __forceinline__ Row resolved(Lean s) {
+  const double exact = (double)s.ref / (double)kLog2e;
+  const float m = (float)exact, lz = logf(s.z);
+  return Row{m, lz + (float)(exact - (double)m), lz - s.u / (s.z * kLog2e)};
 }
 
-// How many of a row's scores are +inf, counted by G lanes (at a row whose largest is).
-template <typename T, int G>
-__device__ __forceinline__ Stats infinite(const LogpArgs& a, int64_t n, int lane) {
-  float count = 0.f;
-  for (int c = lane; c < a.V; c += G) count += to_f32(static_cast<const T*>(a.scores)[n * a.lds + c]) == INFINITY;
-  Stats s;
-  s.m = INFINITY;
-  s.z = lanes_sum<(G < 64 ? G : 64)>(count);
-  return s;
+// A row by G lanes (or the workgroup's threads, G = kThreads) as Plain; of +inf each weighs 1.
+template <typename T, int G, bool SHORT>
+__device__ __forceinline__ Row resolve_slowly(const LogpArgs& a, int64_t n, int lane, float (*red)[3]) {
+  constexpr int V = kVec<T>, U = 8;    // vectors in flight
+  const T* row = static_cast<const T*>(a.scores) + n * a.lds;
+  Plain s;
+  float infinite = 0.f;
+  for (int c0 = lane * V; c0 < a.V; c0 += G * V * U) {
+    uint4 u[U];
+#pragma unroll
+    for (int j = 0; j < U; ++j) {
+      const int c = c0 + j * G * V;
+      u[j] = fetch16<SHORT>(row + (c < a.V ? c : 0), c < a.V ? a.V - c : a.V);
+    }
+#pragma unroll
+    for (int j = 0; j < U; ++j) {
+      const int c = c0 + j * G * V;
+      if (c >= a.V) break;
+      float v[V];
+      unpack16<T>(keep16<SHORT, T>(u[j], a.V - c, a.V), v);
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        const bool inf = c + i < a.V && v[i] == INFINITY;
+        infinite += inf ? 1.f : 0.f;
+        v[i] = c + i < a.V && !inf ? v[i] : -INFINITY;
+      }
+      s.add(v);
+    }
+  }
+  if constexpr (G <= 64) {
+    s = lanes_merge<G>(s);
+    infinite = lanes_sum<G>(infinite);
+  } else {
+    __syncthreads();
+    s = block_merge(s, red);
+    infinite = lanes_sum<64>(infinite);
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6][0] = infinite;
+    __syncthreads();
+    infinite = 0.f;
+    for (int w = 0; w < kThreads / 64; ++w) infinite += red[w][0];
+  }
+  if (infinite > 0.f) {
+    s = Plain();
+    s.ref = INFINITY;
+    s.z = infinite;
+  }
+  return resolved(s);
+}
+template <typename T, int G, bool SHORT>
+__device__ __forceinline__ Row resolve(const LogpArgs& a, int64_t n, int lane, float (*red)[3], Lean s) {
+  if (s.ref == INFINITY || (s.ref == -INFINITY && s.z > 0.f)) return resolve_slowly<T, G, SHORT>(a, n, lane, red);
+  return s.ref == -INFINITY ? Row{-INFINITY, 0.f, 0.f} : resolved(s);
+}
+
+// Writes a row's results, by one thread.
+template <typename T>
+__device__ __forceinline__ void finish(const LogpArgs& a, int64_t n, Row r) {
+  const int64_t t = token_at(a, n);
+  a.chosen[n] = t < 0 ? 0.f : log_p(to_f32(static_cast<const T*>(a.scores)[n * a.lds + t]), r.m, r.logz);
+  a.entropy[n] = r.entropy;
+  if (a.stats) {
+    a.stats[n * 3] = r.m;
+    a.stats[n * 3 + 1] = r.logz;
+    a.stats[n * 3 + 2] = r.entropy;
+  }
 }
 
 // --- no alternatives ------------------------------------------------------------
@@ -153,7 +260,7 @@ __global__ __launch_bounds__(kThreads) void logp_rows_kernel(LogpArgs a) {
   const int lane = threadIdx.x % G;
   for (int64_t n = (int64_t)blockIdx.x * R + threadIdx.x / G; n < a.N; n += (int64_t)gridDim.x * R) {
     const T* row = static_cast<const T*>(a.scores) + n * a.lds;
-    Stats s;
+    Lean s;
     for (int c0 = lane * V; c0 < a.V; c0 += G * V * U) {
       uint4 u[U];
 #pragma unroll
@@ -167,14 +274,15 @@ __global__ __launch_bounds__(kThreads) void logp_rows_kernel(LogpArgs a) {
         if (c >= a.V) break;
         float v[V];
         unpack16<T>(keep16<SHORT, T>(u[j], a.V - c, a.V), v);
+        if (c + V > a.V) {
 #pragma unroll
-        for (int i = 0; i < V; ++i) v[i] = c + i < a.V ? v[i] : -INFINITY;
+          for (int i = 0; i < V; ++i) v[i] = c + i < a.V ? v[i] : -INFINITY;
+        }
         s.add(v);
       }
     }
-    s = lanes_merge<G>(s);
-    if (s.m == INFINITY) s = infinite<T, G>(a, n, lane);
-    if (lane == 0) finish<T>(a, n, s);
+    const Row r = resolve<T, G, SHORT>(a, n, lane, nullptr, lanes_merge<G>(s));
+    if (lane == 0) finish<T>(a, n, r);
   }
 }
 
@@ -190,26 +298,38 @@ __device__ __forceinline__ float value_of(uint32_t key) {
 }
 __device__ __forceinline__ uint64_t rank_of(uint32_t key, int index) { return (uint64_t)key << 32 | (uint32_t)~index; }
 
-constexpr int kTopVectors = 2;                          // a thread's vectors between looks at the list's length
-template <typename T>
-constexpr int kListRoom = kThreads * kTopVectors * kVec<T>;      // that they may add
-template <typename T>
-constexpr int kListSize = kListRoom<T> + 1024;
+constexpr int kTile = 4096;            // scores of a workgroup at a time
+constexpr int kListSize = 1024;
 
 // Keeps the k largest of list[0 .. count - 1] (count > k) in list[0 .. k - 1], in some order; returns the least of
-// them.  Their bits are found from the highest: the largest number that at least k of the list reach.
+// them.  Their bits are found from the highest in which the list's ranks differ: the largest number that at least k of
+// them reach.
 template <int SIZE>
 __device__ __forceinline__ uint64_t cut(uint64_t* list, int count, int k, int* scratch) {
   constexpr int PER = (SIZE + kThreads - 1) / kThreads, W = kThreads / 64;
-  uint64_t mine[PER];
+  uint64_t mine[PER], differ = 0;
+  const uint64_t first = list[0];
 #pragma unroll
   for (int i = 0; i < PER; ++i) {
     const int at = i * kThreads + threadIdx.x;
     mine[i] = at < count ? list[at] : 0;
+    differ |= at < count ? mine[i] ^ first : 0;
   }
-  uint64_t bound = 0;
-  int turn = 0;
-  for (int b = 63; b >= 0; --b) {
+  int high = 63;                       // the highest bit that differs somewhere
+  {
+    uint32_t hi = (uint32_t)(differ >> 32), lo = (uint32_t)differ;
+#pragma unroll
+    for (int off = 32; off; off /= 2) hi |= __shfl_xor(hi, off), lo |= __shfl_xor(lo, off);
+    if ((threadIdx.x & 63) == 0)
+      scratch[threadIdx.x >> 6] = hi ? 63 - __clz((int)hi) : (lo ? 31 - __clz((int)lo) : 0);
+    __syncthreads();
+    high = 0;
+#pragma unroll
+    for (int w = 0; w < W; ++w) high = max(high, scratch[w]);
+  }
+  uint64_t bound = high < 63 ? first >> (high + 1) << (high + 1) : 0;
+  int turn = 1;
+  for (int b = high; b >= 0; --b) {
     const uint64_t test = bound | 1ull << b;
     int n = 0;
 #pragma unroll
@@ -232,6 +352,7 @@ __device__ __forceinline__ uint64_t cut(uint64_t* list, int count, int k, int* s
   for (int i = 0; i < PER; ++i)
     if (mine[i] >= bound) list[atomicAdd(&scratch[0], 1)] = mine[i];
   __syncthreads();
+#pragma unroll 8
   for (int i = 0; i < k; ++i) least = list[i] < least ? list[i] : least;
   __syncthreads();
   return least;
@@ -247,8 +368,11 @@ __device__ __forceinline__ void sorted(uint64_t* list, int count, int k, int* sc
   __syncthreads();
   if ((int)threadIdx.x < count) {
     const uint64_t mine = list[threadIdx.x];
-    int above = 0;
-    for (int i = 0; i < count; ++i) above += list[i] > mine;
+    int above = 0, i = 0;
+    for (; i + 16 <= count; i += 16)
+#pragma unroll
+      for (int q = 0; q < 16; ++q) above += list[i + q] > mine;
+    for (; i < count; ++i) above += list[i] > mine;
     if (above < k) out[above] = mine;
   }
   if ((int)threadIdx.x >= count && (int)threadIdx.x < k) out[threadIdx.x] = 0;
@@ -256,112 +380,165 @@ __device__ __forceinline__ void sorted(uint64_t* list, int count, int k, int* sc
 }
 
 // Writes a row's alternatives from their sorted ranks.
-__device__ __forceinline__ void write_top(const LogpArgs& a, int64_t n, const uint64_t* top, float2 row) {
+__device__ __forceinline__ void write_top(const LogpArgs& a, int64_t n, const uint64_t* top, Row row) {
   if ((int)threadIdx.x < a.k) {
     const uint64_t r = top[threadIdx.x];
     const float v = value_of((uint32_t)(r >> 32));
-    a.top[n * a.k + threadIdx.x] = r ? log_p(v, row.x, row.y) : -INFINITY;
+    a.top[n * a.k + threadIdx.x] = r ? log_p(v, row.m, row.logz) : -INFINITY;
     a.top_index[n * a.k + threadIdx.x] = r ? (int32_t)~(uint32_t)r : -1;
   }
 }
 
-// A part of a row (x) of each row (y), with k alternatives (or none); one part: the row's results.
+// The k-th largest of the threads' ranks, or a number that is no larger and that k of them reach: its bits from the
+// highest, by every wave for itself.
+__device__ __forceinline__ uint64_t reached(uint64_t mine, int k, uint64_t* ranks) {
+  constexpr int PER = kThreads / 64;
+  ranks[threadIdx.x] = mine;
+  __syncthreads();
+  uint64_t rank[PER], bound = 0;
+#pragma unroll
+  for (int i = 0; i < PER; ++i) rank[i] = ranks[i * 64 + (threadIdx.x & 63)];
+  for (uint64_t bit = 1ull << 63; bit; bit >>= 1) {
+    const uint64_t test = bound | bit;
+    int n = 0;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) n += __popcll(__ballot(rank[i] >= test));
+    if (n >= k) bound = test;
+    if (n == k) break;
+  }
+  return bound;
+}
+
+// The scores of a row's part from c on, c + V G ..., U vectors of a thread.
+template <typename T, int U, bool SHORT>
+struct Vectors {
+  static constexpr int V = kVec<T>;
+  uint4 u[U];
+  __device__ __forceinline__ void fetch(const T* row, int base, int last, int length) {
+#pragma unroll
+    for (int j = 0; j < U; ++j) {
+      const int c = base + (j * kThreads + (int)threadIdx.x) * V;
+      u[j] = fetch16<SHORT>(row + (c < last ? c : 0), c < last ? length - c : length);
+    }
+  }
+  // -inf past the part.
+  __device__ __forceinline__ void unpack(int j, int base, int last, int length, float (&v)[V]) const {
+    const int c = base + (j * kThreads + (int)threadIdx.x) * V;
+    unpack16<T>(keep16<SHORT, T>(u[j], c < last ? length - c : length, length), v);
+    if (c + V > last) {
+#pragma unroll
+      for (int i = 0; i < V; ++i) v[i] = c + i < last ? v[i] : -INFINITY;
+    }
+  }
+};
+
+// A part of a row (x) of each row (y), with k alternatives (or none); one part: the row's results.  The next
+// scores are in flight while those at hand are taken in.
 template <typename T, bool TOP, bool SHORT>
 __global__ __launch_bounds__(kThreads) void logp_part_kernel(LogpArgs a) {
-  constexpr int V = kVec<T>, U = TOP ? kTopVectors : 4;
-  __shared__ uint64_t list[TOP ? kListSize<T> : 1];
+  constexpr int V = kVec<T>, U = kTile / kThreads / V;
+  __shared__ uint64_t list[TOP ? kListSize : 1];
   __shared__ uint64_t out[kLogpMaxK];
   __shared__ float red[kThreads / 64][3];
-  __shared__ uint32_t tops[kThreads];
-  __shared__ int scratch[2 * kThreads / 64], count, bound0;
-  __shared__ float2 result;
+  __shared__ uint64_t ranks[TOP ? kThreads : 1];
+  __shared__ int scratch[2 * kThreads / 64], count;
   const int split = blockIdx.x;
   for (int64_t n = blockIdx.y; n < a.N; n += gridDim.y) {
     const T* row = static_cast<const T*>(a.scores) + n * a.lds;
     const int per = (int)((((int64_t)a.V + a.splits - 1) / a.splits + V - 1) / V * V);
     const int first = (int64_t)split * per < a.V ? split * per : a.V;
     const int last = first + (int64_t)per < a.V ? first + per : a.V;
-    Stats s;
+    Lean s;
     uint64_t bound = 1;               // (0: no candidate)
-    bool fresh = true;
-    if (threadIdx.x == 0) count = 0, bound0 = 0;
-    __syncthreads();
-    for (int base = first; base < last; base += kThreads * V * U) {
-      uint4 u[U];
+    if (threadIdx.x == 0) count = 0;
+    Vectors<T, U, SHORT> next;
+    next.fetch(row, first, last, a.V);
+    for (int base = first; base < last; base += kTile) {
+      const Vectors<T, U, SHORT> now = next;
+      if (base + kTile < last) next.fetch(row, base + kTile, last, a.V);
       float v[U][V];
 #pragma unroll
       for (int j = 0; j < U; ++j) {
-        const int c = base + (j * kThreads + (int)threadIdx.x) * V;
-        u[j] = fetch16<SHORT>(row + (c < last ? c : 0), c < last ? a.V - c : a.V);
-      }
-#pragma unroll
-      for (int j = 0; j < U; ++j) {
-        const int c = base + (j * kThreads + (int)threadIdx.x) * V;
-        unpack16<T>(keep16<SHORT, T>(u[j], c < last ? a.V - c : a.V, a.V), v[j]);
-#pragma unroll
-        for (int i = 0; i < V; ++i) v[j][i] = c + i < last ? v[j][i] : -INFINITY;
+        now.unpack(j, base, last, a.V, v[j]);
         s.add(v[j]);
       }
-      if constexpr (!TOP) continue;
-      if (fresh) {                    // a value that k threads' largest reach
-        fresh = false;
-        uint32_t mine = 0;
+      if constexpr (TOP) {
+        float most = -INFINITY;        // (also where all of a thread's are NaN)
 #pragma unroll
         for (int j = 0; j < U; ++j)
 #pragma unroll
-          for (int i = 0; i < V; ++i) mine = max(mine, key_of(v[j][i]));
-        tops[threadIdx.x] = mine;
-        __syncthreads();
-        int reach = 0;
-#pragma unroll 8
-        for (int i = 0; i < kThreads; ++i) reach += tops[i] >= mine;
-        if (reach >= a.k) atomicMax(reinterpret_cast<uint32_t*>(&bound0), mine);
-        __syncthreads();
-        const uint64_t b = (uint64_t)(uint32_t)bound0 << 32;
-        bound = b > bound ? b : bound;
-      }
-      const float least = value_of((uint32_t)(bound >> 32));
+          for (int i = 0; i < V; ++i) most = fmaxf(most, v[j][i]);
+        if (base == first) {
+          int at = 0;                  // the first place of a thread's largest
 #pragma unroll
-      for (int j = 0; j < U; ++j) {
-        const int c = base + (j * kThreads + (int)threadIdx.x) * V;
-        float top = v[j][0];
+          for (int j = U - 1; j >= 0; --j)
 #pragma unroll
-        for (int i = 1; i < V; ++i) top = fmaxf(top, v[j][i]);
-        if ((bound >> 32) == 0 ? top > -INFINITY : top >= least) {
+            for (int i = V - 1; i >= 0; --i)
+              at = v[j][i] == most ? base + (j * kThreads + (int)threadIdx.x) * V + i : at;
+          const uint32_t key = key_of(most);
+          bound = max(bound, reached(key ? rank_of(key, at) : 0, a.k, ranks));
+        }
+        // Each thread's scores that reach the bound, as bits; what the list has no room for waits until the list is
+        // cut and the bound is higher.
+        const auto reach = [&](int j, int i) {
+          const int c = base + (j * kThreads + (int)threadIdx.x) * V;
+          return rank_of(key_of(v[j][i]), c + i);
+        };
+        const float least = (bound >> 32) != 0 ? value_of((uint32_t)(bound >> 32)) : -FLT_MAX;
+        uint32_t waiting = 0;
+        if (most >= least) {
 #pragma unroll
-          for (int i = 0; i < V; ++i) {
-            const uint64_t r = rank_of(key_of(v[j][i]), c + i);
-            if ((r >> 32) != 0 && r >= bound) list[atomicAdd(&count, 1)] = r;
+          for (int j = 0; j < U; ++j)
+#pragma unroll
+            for (int i = 0; i < V; ++i) waiting |= v[j][i] >= least ? 1u << (j * V + i) : 0;
+        }
+        for (;;) {
+          if ((uint32_t)bound > 1 && __any(waiting)) {   // (a bound with an index: equal scores after it do not reach it)
+#pragma unroll
+            for (int j = 0; j < U; ++j)
+#pragma unroll
+              for (int i = 0; i < V; ++i)
+                if (reach(j, i) < bound) waiting &= ~(1u << (j * V + i));
           }
+          // places in the list: a wave's share of it, in which a lane's scores follow those of the lanes before it
+          if (__any(waiting)) {
+            const int mine = __popc(waiting), before = lanes_scan(mine, [](int p, int q) { return p + q; });
+            const int all = __builtin_amdgcn_readlane(before, 63);
+            int at = 0;
+            if ((threadIdx.x & 63) == 0) at = atomicAdd(&count, all);
+            at = __builtin_amdgcn_readfirstlane(at) + before - mine;
+#pragma unroll
+            for (int j = 0; j < U; ++j)
+#pragma unroll
+              for (int i = 0; i < V; ++i)
+                if (waiting >> (j * V + i) & 1) {
+                  if (at < kListSize) {
+                    list[at] = reach(j, i);
+                    waiting &= ~(1u << (j * V + i));
+                  }
+                  ++at;
+                }
+          }
+          __syncthreads();
+          const int have = count;
+          __syncthreads();
+          if (have <= kListSize) break;
+          bound = cut<kListSize>(list, kListSize, a.k, scratch);
+          if (threadIdx.x == 0) count = a.k;
+          __syncthreads();
         }
       }
-      __syncthreads();
-      const int have = count;
-      if (have > kListSize<T> - kListRoom<T>) {
-        bound = cut<kListSize<T>>(list, have, a.k, scratch);
-        if (threadIdx.x == 0) count = a.k;
-      }
-      __syncthreads();
     }
     s = block_merge(s, red);
-    if constexpr (TOP) sorted<kListSize<T>>(list, count, a.k, scratch, out);
+    if constexpr (TOP) sorted<kListSize>(list, count, a.k, scratch, out);
     if (a.splits > 1) {
       const int64_t at = n * a.splits + split;
-      if (threadIdx.x == 0) a.part[at * 3] = s.m, a.part[at * 3 + 1] = s.z, a.part[at * 3 + 2] = s.u;
+      if (threadIdx.x == 0) a.part[at * 3] = s.ref, a.part[at * 3 + 1] = s.z, a.part[at * 3 + 2] = s.u;
       if (TOP && (int)threadIdx.x < a.k) a.part_top[at * a.k + threadIdx.x] = out[threadIdx.x];
     } else {
-      if (s.m == INFINITY) {
-        Stats mine = infinite<T, kThreads>(a, n, threadIdx.x);
-        __syncthreads();
-        if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6][1] = mine.z;
-        __syncthreads();
-        s = Stats();
-        s.m = INFINITY;
-        for (int w = 0; w < kThreads / 64; ++w) s.z += red[w][1];
-      }
-      if (threadIdx.x == 0) result = finish<T>(a, n, s);
-      __syncthreads();
-      if constexpr (TOP) write_top(a, n, out, result);
+      const Row r = resolve<T, kThreads, SHORT>(a, n, threadIdx.x, red, s);
+      if (threadIdx.x == 0) finish<T>(a, n, r);
+      if constexpr (TOP) write_top(a, n, out, r);
     }
     __syncthreads();
   }
@@ -369,49 +546,56 @@ __global__ __launch_bounds__(kThreads) void logp_part_kernel(LogpArgs a) {
 
 // The parts of a row.
 constexpr int kMaxSplits = 64;
-template <typename T>
+template <typename T, bool TOP>
 __global__ __launch_bounds__(kThreads) void logp_join_kernel(LogpArgs a) {
-  __shared__ uint64_t list[kMaxSplits * kLogpMaxK];
+  __shared__ uint64_t list[TOP ? kMaxSplits * kLogpMaxK : 1];
   __shared__ uint64_t out[kLogpMaxK];
   __shared__ float red[kThreads / 64][3];
   __shared__ int scratch[2 * kThreads / 64], count;
-  __shared__ float2 result;
+  __shared__ uint64_t lowest;
   for (int64_t n = blockIdx.x; n < a.N; n += gridDim.x) {
-    Stats s;
+    Lean s;
+    const uint64_t* p = a.part_top + n * a.splits * a.k;
+    uint64_t bound = 1;
     if ((int)threadIdx.x < a.splits) {
-      const float* p = a.part + (n * a.splits + threadIdx.x) * 3;
-      s.m = p[0], s.z = p[1], s.u = p[2];
+      const float* q = a.part + (n * a.splits + threadIdx.x) * 3;
+      s.ref = q[0], s.z = q[1], s.u = q[2];
+      // every part's list is sorted: no score below a part's last is among the row's k best
+      if (TOP) bound = max(bound, p[threadIdx.x * a.k + a.k - 1]);
+    }
+    const int all = a.splits * a.k;
+    constexpr int PER = 4;             // of them in flight before the bound is known
+    uint64_t mine[PER];
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      const int at = i * kThreads + threadIdx.x;
+      mine[i] = at < all ? p[at] : 0;
+    }
+    if constexpr (TOP) {                         // (the parts are the first wave's)
+#pragma unroll
+      for (int off = 32; off; off /= 2) {
+        const uint64_t o = (uint64_t)__shfl_xor((int)(bound >> 32), off) << 32 | (uint32_t)__shfl_xor((int)bound, off);
+        bound = max(bound, o);
+      }
+      if (threadIdx.x == 0) lowest = bound, count = 0;
     }
     s = block_merge(s, red);
-    if (s.m == INFINITY) {
-      Stats mine = infinite<T, kThreads>(a, n, threadIdx.x);
-      __syncthreads();
-      if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6][1] = mine.z;
-      __syncthreads();
-      s = Stats();
-      s.m = INFINITY;
-      for (int w = 0; w < kThreads / 64; ++w) s.z += red[w][1];
+    const Row r = resolve<T, kThreads, false>(a, n, threadIdx.x, red, s);
+    if constexpr (TOP) {
+      bound = lowest;
+#pragma unroll
+      for (int i = 0; i < PER; ++i)
+        if (mine[i] >= bound) list[atomicAdd(&count, 1)] = mine[i];
+      for (int at = PER * kThreads + threadIdx.x; at < all; at += kThreads) {
+        const uint64_t o = p[at];
+        if (o >= bound) list[atomicAdd(&count, 1)] = o;
+      }
     }
-    if (threadIdx.x == 0) {
-      result = finish<T>(a, n, s);
-      count = 0;
-    }
+    if (threadIdx.x == 0) finish<T>(a, n, r);
     __syncthreads();
-    if (a.k) {
-      // every part's list is sorted: no score below a part's last is among the row's k best
-      const uint64_t* p = a.part_top + n * a.splits * a.k;
-      uint64_t bound = 1;
-      for (int i = 0; i < a.splits; ++i) {
-        const uint64_t b = p[i * a.k + a.k - 1];
-        bound = b > bound ? b : bound;
-      }
-      for (int i = threadIdx.x; i < a.splits * a.k; i += kThreads) {
-        const uint64_t r = p[i];
-        if (r >= bound) list[atomicAdd(&count, 1)] = r;
-      }
-      __syncthreads();
+    if constexpr (TOP) {
       sorted<kMaxSplits * kLogpMaxK>(list, count, a.k, scratch, out);
-      write_top(a, n, out, result);
+      write_top(a, n, out, r);
     }
     __syncthreads();
   }
@@ -419,12 +603,12 @@ __global__ __launch_bounds__(kThreads) void logp_join_kernel(LogpArgs a) {
 
 // --- gradient ---------------------------------------------------------------------
 
-// The factors of a row's p: ds = p (c + h (log p + H)) before what the chosen get.
+// What a row's gradient is made of: ds = p (c + h (log p + H)) before what the chosen get.
 struct Factors {
   float m, logz, entropy, c, h;
 };
 
-// Σ over the alternatives that exist.
+// (dtop: the sum over the alternatives that exist)
 __device__ __forceinline__ Factors factors_of(const LogpArgs& a, int64_t n, float dtop) {
   Factors f;
   f.m = a.stats[n * 3], f.logz = a.stats[n * 3 + 1], f.entropy = a.stats[n * 3 + 2];
@@ -433,34 +617,61 @@ __device__ __forceinline__ Factors factors_of(const LogpArgs& a, int64_t n, floa
   return f;
 }
 
-template <bool INF>
+// The gradient of score s, of any row.
 __device__ __forceinline__ float slope(const Factors& f, float s) {
-  float d = s - f.m;
-  if constexpr (INF) d = s == f.m ? 0.f : d;
+  const float d = s == f.m ? 0.f : s - f.m;
   float lp = d - f.logz;
   const float p = exp_below(lp);
-  return p * fmaf(f.h, lp + f.entropy, f.c);
+  return s > -INFINITY ? p * fmaf(f.h, lp + f.entropy, f.c) : 0.f;
 }
 
-// tx threads share a row's part: y counts parts of tx V U columns.
-template <typename T, bool SHORT>
-__global__ __launch_bounds__(kThreads) void logp_bwd_kernel(LogpArgs a, int tx) {
-  constexpr int V = kVec<T>, U = 4;
+// The same in fewer instructions, where |m| < 2^100: with l = s L - k, L = log2(e) in fp32 and k = m L + log2 Z rounded
+// to fp32, p = 2^(l - off) by what k's rounding left, off, and so ds = 2^l (c' + h' l).
+struct Quick {
+  float k, c, h;
+  __device__ __forceinline__ explicit Quick(const Factors& f) {
+#pragma clang fp contract(off)      // (what roundings leave is taken from rounded values)
+    const float m = f.m > -INFINITY ? f.m : 0.f;                // (an empty row: every 2^l is 0)
+    const float a = m * kLog2e, b = f.logz * kLog2e;
+    k = a + b;
+    const float bb = k - a;                                     // (a + b = k + ((a - (k - bb)) + (b - bb)) exactly)
+    const float off = fmaf(m, kLog2e, -a) + fmaf(f.logz, kLog2e, -b) + f.logz * 1.925963033500e-8f +
+                      ((a - (k - bb)) + (b - bb));              // (log2(e) = kLog2e + 1.926e-8)
+    const float back = fast_exp2(-off);
+    c = fmaf(f.h, f.entropy - off * kLn2, f.c) * back;
+    h = f.h * kLn2 * back;
+  }
+  __device__ __forceinline__ float slope(float s) const {
+    const float l = fmaxf(fmaf(s, kLog2e, -k), -160.f);
+    return fast_exp2(l) * fmaf(h, l, c);
+  }
+};
+
+// WHOLE: a workgroup takes `tiles` times kThreads V U columns of a row (y counts such parts), the next scores in flight.
+// Otherwise tx threads share a row of at most tx V U columns.
+template <typename T, bool WHOLE, bool SHORT>
+__global__ __launch_bounds__(kThreads) void logp_bwd_kernel(LogpArgs a, int tx_, int tiles) {
+  constexpr int V = kVec<T>, U = WHOLE ? 2 : 4;
+  const int tx = WHOLE ? kThreads : tx_;
   const int lane = threadIdx.x & (tx - 1), rpb = kThreads / tx;
   __shared__ float sums[kThreads / 4];
   for (int64_t n0 = (int64_t)blockIdx.x * rpb; n0 < a.N; n0 += (int64_t)gridDim.x * rpb) {
-    const int64_t n = n0 + threadIdx.x / tx;
-    const bool there = n < a.N;
+    const int64_t n = WHOLE ? n0 : n0 + threadIdx.x / tx;
+    const bool there = WHOLE || n < a.N;
     const int64_t r = there ? n : a.N - 1;
     const T* row = static_cast<const T*>(a.scores) + r * a.lds;
     T* out = static_cast<T*>(a.dscores) + r * a.V;
-    const int first = (int)blockIdx.y * tx * V * U;
-    uint4 u[U];
+    const int span = tx * V * U, first = WHOLE ? (int)blockIdx.y * tiles * span : 0;
+    const int last = WHOLE ? min(first + tiles * span, a.V) : a.V;
+    uint4 next[U];
+    const auto fetch = [&](int base) {
 #pragma unroll
-    for (int j = 0; j < U; ++j) {
-      const int c = first + (j * tx + lane) * V;
-      u[j] = fetch16<SHORT>(row + (c < a.V ? c : 0), c < a.V ? a.V - c : a.V);
-    }
+      for (int j = 0; j < U; ++j) {
+        const int c = base + (j * tx + lane) * V;
+        next[j] = fetch16<SHORT>(row + (c < a.V ? c : 0), c < a.V ? a.V - c : a.V);
+      }
+    };
+    fetch(first);
     float dtop = 0.f;
     if (a.dtop) {
       if (lane == 0)
@@ -471,23 +682,36 @@ __global__ __launch_bounds__(kThreads) void logp_bwd_kernel(LogpArgs a, int tx) 
       dtop = sums[threadIdx.x / tx];
     }
     const Factors f = factors_of(a, r, dtop);
-    const int64_t t = a.dchosen ? token_at(a, r) : -1;
+    const int t = a.dchosen ? (int)token_at(a, r) : -1;
     const float dc = t >= 0 ? a.dchosen[r] : 0.f;
+    const bool quick = fabsf(f.m) < kFar || f.m == -INFINITY;
+    const Quick q(f);
     if (there) {
+      for (int base = first; base < last; base += span) {
+        uint4 u[U];
 #pragma unroll
-      for (int j = 0; j < U; ++j) {
-        const int c = first + (j * tx + lane) * V;
-        if (c >= a.V) break;
-        float v[V];
-        unpack16<T>(keep16<SHORT, T>(u[j], a.V - c, a.V), v);
-        const int at = t >= c && t < c + V ? (int)(t - c) : -1;
+        for (int j = 0; j < U; ++j) u[j] = next[j];
+        if (WHOLE && base + span < last) fetch(base + span);
 #pragma unroll
-        for (int i = 0; i < V; ++i) {
-          const float s = v[i];
-          v[i] = f.m == INFINITY ? slope<true>(f, s) : slope<false>(f, s);
-          if (at == i && s > -INFINITY) v[i] += dc;
+        for (int j = 0; j < U; ++j) {
+          const int c = base + (j * tx + lane) * V;
+          if (c >= a.V) break;
+          float v[V], o[V];
+          unpack16<T>(keep16<SHORT, T>(u[j], a.V - c, a.V), v);
+          if (quick) {
+#pragma unroll
+            for (int i = 0; i < V; ++i) o[i] = q.slope(v[i]);
+          } else {
+#pragma unroll
+            for (int i = 0; i < V; ++i) o[i] = slope(f, v[i]);
+          }
+          const int at = t - c;
+          if ((unsigned)at < (unsigned)V) {
+#pragma unroll
+            for (int i = 0; i < V; ++i) o[i] += at == i && v[i] > -INFINITY ? dc : 0.f;
+          }
+          store_row(out + c, a.V - c, o);
         }
-        store_row(out + c, a.V - c, v);
       }
     }
     if (a.dtop) {
@@ -496,9 +720,9 @@ __global__ __launch_bounds__(kThreads) void logp_bwd_kernel(LogpArgs a, int tx) 
       if (there) {
         for (int i = lane; i < a.k; i += tx) {
           const int32_t c = a.top_index[r * a.k + i];
-          if (c < first || c >= first + tx * V * U) continue;
+          if (c < first || c >= last) continue;
           const float s = to_f32(row[c]);
-          float g = f.m == INFINITY ? slope<true>(f, s) : slope<false>(f, s);
+          float g = quick ? q.slope(s) : slope(f, s);
           if (c == t) g += dc;
           out[c] = (T)(g + a.dtop[r * a.k + i]);
         }
@@ -529,20 +753,30 @@ void logp_typed(const LogpArgs& a, hipStream_t s) {
   if (a.k == 0) logp_part_kernel<T, false, false><<<grid, kThreads, 0, s>>>(a);      // (V > 2048)
   else if (a.V < kVec<T>) logp_part_kernel<T, true, true><<<grid, kThreads, 0, s>>>(a);
   else logp_part_kernel<T, true, false><<<grid, kThreads, 0, s>>>(a);
-  if (a.splits > 1) logp_join_kernel<T><<<(unsigned)(a.N < kMaxBlocks ? a.N : kMaxBlocks), kThreads, 0, s>>>(a);
+  if (a.splits == 1) return;
+  const unsigned rows = (unsigned)(a.N < kMaxBlocks ? a.N : kMaxBlocks);
+  if (a.k == 0) logp_join_kernel<T, false><<<rows, kThreads, 0, s>>>(a);
+  else logp_join_kernel<T, true><<<rows, kThreads, 0, s>>>(a);
 }
 
 template <typename T>
 void logp_bwd_typed(const LogpArgs& a, hipStream_t s) {
   constexpr int V = kVec<T>;
   const int nvec = (a.V + V * 4 - 1) / (V * 4);
+  const auto grid = [](int64_t need) { return (unsigned)(need < kMaxBlocks ? need : kMaxBlocks); };
+  if (nvec > kThreads / 2) {
+    // parts of a row as long as 4096 workgroups allow
+    const int64_t spans = (a.V + (int64_t)kThreads * V * 2 - 1) / (kThreads * V * 2);
+    const int64_t parts = std::min(spans, std::max<int64_t>(1, 4096 / a.N)), tiles = (spans + parts - 1) / parts;
+    const dim3 blocks(grid(a.N), (unsigned)((spans + tiles - 1) / tiles));
+    logp_bwd_kernel<T, true, false><<<blocks, kThreads, 0, s>>>(a, kThreads, (int)tiles);
+    return;
+  }
   int tx = 4;
-  while (tx < nvec && tx < kThreads) tx *= 2;
-  const int64_t need = (a.N + kThreads / tx - 1) / (kThreads / tx);
-  const int64_t parts = (a.V + (int64_t)tx * V * 4 - 1) / ((int64_t)tx * V * 4);
-  const dim3 grid((unsigned)(need < kMaxBlocks ? need : kMaxBlocks), (unsigned)parts);
-  if (a.V < V) logp_bwd_kernel<T, true><<<grid, kThreads, 0, s>>>(a, tx);
-  else logp_bwd_kernel<T, false><<<grid, kThreads, 0, s>>>(a, tx);
+  while (tx < nvec) tx *= 2;
+  const unsigned blocks = grid((a.N + kThreads / tx - 1) / (kThreads / tx));
+  if (a.V < V) logp_bwd_kernel<T, false, true><<<blocks, kThreads, 0, s>>>(a, tx, 1);
+  else logp_bwd_kernel<T, false, false><<<blocks, kThreads, 0, s>>>(a, tx, 1);
 }
 
 int64_t align256(int64_t v) { return (v + 255) / 256 * 256; }
@@ -552,7 +786,8 @@ int64_t align256(int64_t v) { return (v + 255) / 256 * 256; }
 // Parts of a row: none with enough rows for the card, else parts of 4096 scores or more.
 int logp_splits(int64_t N, int V, int k) {
   if (k == 0 && V <= 2048) return 1;
-  int64_t parts = (1024 + N - 1) / (N > 0 ? N : 1);
+  const int64_t blocks = k ? 512 : 1024;
+  int64_t parts = (blocks + N - 1) / (N > 0 ? N : 1);
   const int64_t most = (V + 4095) / 4096;
   if (parts > most) parts = most;
   return (int)(parts < 1 ? 1 : (parts < kMaxSplits ? parts : kMaxSplits));

@@ -25,10 +25,10 @@ __device__ __forceinline__ float larger_bits(float a, float b) {
   return __uint_as_float(max(__float_as_uint(a), __float_as_uint(b)));
 }
 
-// G threads share a row.
-template <typename T, int G, bool SHORT>
+// A row by G threads, which keep its elements: NV vectors each.  0: any row, read twice.
+template <typename T, int G, int NV, bool SHORT>
 __global__ __launch_bounds__(kThreads) void quantize_kernel(QuantArgs a) {
-  constexpr int V = kVec<T>, R = kThreads / G;
+  constexpr int V = kVec<T>, R = kThreads / G, KEEP = NV ? NV : 1;
   __shared__ float red[kThreads / 64];
   const int lane = threadIdx.x % G;
   const int padded = (a.D + 15) / 16 * 16;
@@ -37,11 +37,27 @@ __global__ __launch_bounds__(kThreads) void quantize_kernel(QuantArgs a) {
     const bool there = n < a.N;
     const T* row = static_cast<const T*>(a.x) + (there ? n : a.N - 1) * a.ldx;
     uint32_t most = 0;       // (bits: a NaN is the largest, then an infinity)
-    for (int c = lane * V; c < a.D; c += G * V) {
-      float v[V];
-      unpack16<T>(keep16<SHORT, T>(fetch16<SHORT>(row + c, a.D - c), a.D - c, a.D), v);
+    // vector c's elements, zeros past the row
+    const auto fetch = [&](int c) { return fetch16<SHORT>(row + (c < a.D ? c : 0), c < a.D ? a.D - c : a.D); };
+    const auto unpack = [&](uint4 u, int c, float (&v)[V]) { unpack16<T>(keep16<SHORT, T>(u, a.D - c, a.D), v); };
+    uint4 kept[KEEP];
+    if constexpr (NV > 0) {
 #pragma unroll
-      for (int i = 0; i < V; ++i) most = max(most, __float_as_uint(v[i]) & 0x7fffffffu);
+      for (int i = 0; i < NV; ++i) kept[i] = fetch((i * G + lane) * V);
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+        float v[V];
+        unpack(kept[i], (i * G + lane) * V, v);
+#pragma unroll
+        for (int j = 0; j < V; ++j) most = max(most, __float_as_uint(v[j]) & 0x7fffffffu);
+      }
+    } else {
+      for (int c = lane * V; c < a.D; c += G * V) {
+        float v[V];
+        unpack(fetch(c), c, v);
+#pragma unroll
+        for (int j = 0; j < V; ++j) most = max(most, __float_as_uint(v[j]) & 0x7fffffffu);
+      }
     }
     most = __float_as_uint(lanes_reduce<(G < 64 ? G : 64)>(__uint_as_float(most), larger_bits));
     if constexpr (G > 64) {
@@ -53,34 +69,44 @@ __global__ __launch_bounds__(kThreads) void quantize_kernel(QuantArgs a) {
     const bool finite = most < 0x7f800000u;
     const float top = __uint_as_float(most), lift = top < 0x1p-100f ? 0x1p100f : 1.f;
     const float by = finite && most ? 127.f / (top * lift) : 0.f;
-    if (there) {
-      if (lane == 0) a.scales[n] = finite ? top / 127.f : __uint_as_float(0x7fc00000u);
-      int8_t* out = a.values + n * a.ldv;
-      for (int c = lane * V; c < padded; c += G * V) {
-        float v[V];
-        const int left = a.D - c;
-        unpack16<T>(keep16<SHORT, T>(fetch16<SHORT>(row + (left > 0 ? c : 0), left > 0 ? left : a.D), left, a.D), v);
-        union { uint64_t u; uint32_t w; int8_t b[8]; } o;
-        o.u = 0;
+    if (!there) continue;
+    if (lane == 0) a.scales[n] = finite ? top / 127.f : __uint_as_float(0x7fc00000u);
+    int8_t* out = a.values + n * a.ldv;
+    const auto store = [&](uint4 u, int c) {
+      float v[V];
+      unpack(u, c, v);
+      union { uint64_t u; uint32_t w; int8_t b[8]; } o;
 #pragma unroll
-        for (int i = 0; i < V; ++i) o.b[i] = finite && i < left ? (int8_t)(int)rintf(v[i] * lift * by) : 0;
-        if constexpr (V == 8) *reinterpret_cast<uint64_t*>(out + c) = o.u;
-        else *reinterpret_cast<uint32_t*>(out + c) = o.w;
-      }
+      for (int i = 0; i < 8; ++i) o.b[i] = i < V && finite ? (int8_t)(int)rintf(v[i % V] * lift * by) : 0;
+      if constexpr (V == 8) *reinterpret_cast<uint64_t*>(out + c) = o.u;
+      else *reinterpret_cast<uint32_t*>(out + c) = o.w;
+    };
+    if constexpr (NV > 0) {
+#pragma unroll
+      for (int i = 0; i < NV; ++i)
+        if ((i * G + lane) * V < padded) store(kept[i], (i * G + lane) * V);
+    } else {
+      for (int c = lane * V; c < padded; c += G * V) store(fetch(c), c);
     }
   }
 }
 
+template <typename T, int G, int NV, bool SHORT = false>
+void quantize_shaped(const QuantArgs& a, hipStream_t s) {
+  const int64_t need = (a.N + kThreads / G - 1) / (kThreads / G);
+  quantize_kernel<T, G, NV, SHORT><<<(unsigned)(need < kMaxBlocks ? need : kMaxBlocks), kThreads, 0, s>>>(a);
+}
+
 template <typename T>
 void quantize_typed(const QuantArgs& a, hipStream_t s) {
-  const auto grid = [&](int rows) {
-    const int64_t need = (a.N + rows - 1) / rows;
-    return (unsigned)(need < kMaxBlocks ? need : kMaxBlocks);
-  };
-  if (a.D < kVec<T>) quantize_kernel<T, 16, true><<<grid(16), kThreads, 0, s>>>(a);
-  else if (a.D <= 16 * kVec<T>) quantize_kernel<T, 16, false><<<grid(16), kThreads, 0, s>>>(a);
-  else if (a.D <= 128 * kVec<T>) quantize_kernel<T, 64, false><<<grid(4), kThreads, 0, s>>>(a);
-  else quantize_kernel<T, 256, false><<<grid(1), kThreads, 0, s>>>(a);
+  const int nvec = (a.D + kVec<T> - 1) / kVec<T>;
+  if (a.D < kVec<T>) quantize_shaped<T, 16, 1, true>(a, s);
+  else if (nvec <= 32) quantize_shaped<T, 16, 2>(a, s);
+  else if (nvec <= 128) quantize_shaped<T, 64, 2>(a, s);
+  else if (nvec <= 256) quantize_shaped<T, 64, 4>(a, s);
+  else if (nvec <= 512) quantize_shaped<T, 64, 8>(a, s);
+  else if (nvec <= 2048) quantize_shaped<T, 256, 8>(a, s);
+  else quantize_shaped<T, 256, 0>(a, s);
 }
 
 // --- products: tiles -------------------------------------------------------------

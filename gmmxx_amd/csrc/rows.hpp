@@ -1,5 +1,5 @@
 // Shared helpers of the sparsely gated layer's kernels (layer_norm.hip, route.hip,
-// grouped.hip, combine.hip): element types, 16-byte row access at any alignment and
+// grouped.hip, combine.hip) and the token operators': element types, 16-byte row access at any alignment and
 // sums over groups of lanes.
 #pragma once
 
@@ -124,6 +124,18 @@ __device__ __forceinline__ float lanes_reduce(float v, F&& op) {
 template <int G>
 __device__ __forceinline__ float lanes_sum(float v) {
   return lanes_reduce<G>(v, [](float a, float b) { return a + b; });
+}
+
+// op over lanes 0 .. l in lane l, for values that are not negative (0 changes nothing): within rows of 16 lanes,
+// then across them.
+template <typename F>
+__device__ __forceinline__ int lanes_scan(int v, F&& op) {
+  v = op(v, __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, false));      // shifted by 1, 2, 4 and 8 lanes
+  v = op(v, __builtin_amdgcn_update_dpp(0, v, 0x112, 0xF, 0xF, false));
+  v = op(v, __builtin_amdgcn_update_dpp(0, v, 0x114, 0xF, 0xF, false));
+  v = op(v, __builtin_amdgcn_update_dpp(0, v, 0x118, 0xF, 0xF, false));
+  v = op(v, __builtin_amdgcn_update_dpp(0, v, 0x142, 0xA, 0xF, false));      // lane 15 to rows 1 and 3
+  return op(v, __builtin_amdgcn_update_dpp(0, v, 0x143, 0xC, 0xF, false));   // lane 31 to rows 2 and 3
 }
 
 // Sums of N values over groups of G threads: lanes_sum within a wave, `red` (two slots of 16 waves' values, used

@@ -207,3 +207,31 @@ def test_past_32_bits(hip):
     compare(gmmxx_amd.LogProbs(*(x[far] for x in r)), want)
     ds, = torch.autograd.grad(r.chosen.sum(), leaf)
     experts_ref.close(ds[far], *want["dscores"], "dscores")
+
+
+@pytest.mark.parametrize("v,k", [(4096, 64), (5000, 4), (9000, 33)])
+def test_few_candidates_among_nan(hip, v, k):
+    """Candidates in a few places only, the rest NaN: a bound from some of the scores must not pass any of them."""
+    g = torch.Generator().manual_seed(v)
+    s = torch.full((40, v), float("nan"))
+    for r in range(40):
+        at = torch.randperm(v, generator=g)[:1 + 2 * r]
+        s[r, at] = torch.randn(at.numel(), generator=g)
+    check(s.to(DEV), torch.randint(0, v, (40,), generator=g).to(DEV), k)
+
+
+@pytest.mark.parametrize("k", [0, 3])
+@pytest.mark.parametrize("v", [9, 600, 5000, 40_000])
+@pytest.mark.parametrize("dtype", (F32, BF16), ids=str)
+def test_far_scores(hip, v, k, dtype):
+    """Rows around 2^100 in size and at the type's ends, among ordinary scores and alone."""
+    big = torch.finfo(dtype).max
+    s, t = make(12, v, dtype)
+    for r, x in enumerate((2.0 ** 99, 2.0 ** 100, 2.0 ** 101, big)):
+        s[r, v // 3] = x
+        s[r, v // 2] = x
+        s[4 + r] = -x
+        s[4 + r, v // 4] = -x / 2
+    s[8], s[9, 5], s[10], s[11, 1::2] = big, -big, -big, -2.0 ** 100
+    t[:] = torch.tensor([v // 3, 0, v // 2, v // 3, 1, v // 4, v // 4, 2, 3, 5, 0, 1], device=DEV)
+    check(s, t, k)

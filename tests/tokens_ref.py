@@ -76,8 +76,9 @@ def log_probs(scores, index, k=0, dchosen=None, dentropy=None, dtop=None):
 
     The error of one e^d: d is rounded (relative error |d| U), d log2(e) is rounded and its factor is (|d| U each),
     the exponential is good to 2 U; and a sum is brought to a larger maximum at most once a vector, whose
-    exponents add up to at most |d|: another 3 |d| U, and 4 U for each of them.  `adds` bounds a thread's
-    vectors (which also are the additions of its chain, but for 8 in a vector, 10 levels and 64 parts above them)."""
+    exponents add up to at most |d|: another 3 |d| U, and 4 U for each of them.  The reference may lie below the largest
+    score by up to 7: 6 |d| is 42 more.  `adds` bounds a thread's vectors (which also are the additions of its
+    chain, but for 8 in a vector, 10 levels and 64 parts above them)."""
     dt = scores.dtype
     s, t = f64(scores), index.cpu().long()
     n, v = s.shape
@@ -95,9 +96,9 @@ def log_probs(scores, index, k=0, dchosen=None, dentropy=None, dtop=None):
     mean, square = (p * size).sum(1, keepdim=True), (p * size * size).sum(1, keepdim=True)
     entropy = torch.where(some, logz + mean, 0.0)
     adds = -(-v // 512) + 90.0
-    dz = U * (6 * mean + 5 * adds + 8)                   # relative error of Z, so absolute of log Z
+    dz = U * (6 * mean + 42 + 5 * adds + 8)                   # relative error of Z, so absolute of log Z
     dlogz = dz + 4 * U * logz.abs()
-    dh = dlogz + U * (6 * square + (5 * adds + 8) * mean) + mean * dz + 4 * U * entropy.abs()
+    dh = dlogz + U * (6 * square + (42 + 5 * adds + 8) * (mean + 7)) + (mean + 7) * dz + 4 * U * entropy.abs()
     counts = (t >= 0) & (t < v)
     at = torch.where(counts, t, 0)[:, None]
 
