@@ -28,8 +28,10 @@ namespace {
 constexpr int kThreads = 256;
 constexpr int kTile = 32;              // sorted positions whose rows one group of threads adds
 constexpr int kMaxBits = 11;
-constexpr int kSortRows = 2048;        // tokens of a block of the sort, more where that gives over kMaxSortBlocks
+constexpr int kSortThreads = 512;
+constexpr int kSortRows = 1024;        // tokens of a block of the sort, more where that gives over kMaxSortBlocks
 constexpr int64_t kMaxSortBlocks = 4096;
+constexpr int kFewBlocks = 32;         // up to which the blocks form the prefixes themselves
 constexpr int64_t kMaxBlocks = 1 << 20;
 
 __host__ __device__ inline int key_bits(int64_t V) {
@@ -90,17 +92,19 @@ __device__ __forceinline__ uint32_t key_at(const EmbedArgs& a, int from, int64_t
   return (uint64_t)t < (uint64_t)a.V ? (uint32_t)t : (uint32_t)a.V;
 }
 
-__global__ __launch_bounds__(kThreads) void sort_count_kernel(EmbedArgs a, int from, int shift, int bits, int64_t rpb) {
+__global__ __launch_bounds__(kSortThreads) void sort_count_kernel(EmbedArgs a, int from, int shift, int bits,
+                                                                  int64_t rpb) {
   extern __shared__ int count[];
   const int bins = 1 << bits;
-  for (int b = threadIdx.x; b < bins; b += kThreads) count[b] = 0;
+  for (int b = threadIdx.x; b < bins; b += kSortThreads) count[b] = 0;
   __syncthreads();
   const int64_t first = blockIdx.x * rpb, last = first + rpb < a.N ? first + rpb : a.N;
-  for (int64_t i = first + threadIdx.x; i < last; i += kThreads)
+#pragma unroll 2
+  for (int64_t i = first + threadIdx.x; i < last; i += kSortThreads)
     atomicAdd(&count[(key_at(a, from, i) >> shift) & (bins - 1)], 1);
   __syncthreads();
   int32_t* hist = a.hist + (int64_t)blockIdx.x * bins;
-  for (int b = threadIdx.x; b < bins; b += kThreads) hist[b] = count[b];
+  for (int b = threadIdx.x; b < bins; b += kSortThreads) hist[b] = count[b];
 }
 
 // Exclusive prefixes over the blocks for 16 digits a workgroup: 64 parts of the blocks,
@@ -113,13 +117,16 @@ __global__ __launch_bounds__(kScanCols* kScanParts) void sort_scan_kernel(EmbedA
   const int per = (blocks + kScanParts - 1) / kScanParts;
   const int b0 = p * per < blocks ? p * per : blocks, b1 = b0 + per < blocks ? b0 + per : blocks;
   int s = 0;
-  if (b < bins)
+  if (b < bins) {
+#pragma unroll 4
     for (int i = b0; i < b1; ++i) s += a.hist[(int64_t)i * bins + b];
+  }
   part[p][cl] = s;
   __syncthreads();
   int before = 0;
   for (int q = 0; q < p; ++q) before += part[q][cl];
   if (b < bins) {
+#pragma unroll 4
     for (int i = b0; i < b1; ++i) {
       int32_t* h = a.hist + (int64_t)i * bins + b;
       const int n = *h;
@@ -130,48 +137,72 @@ __global__ __launch_bounds__(kScanCols* kScanParts) void sort_scan_kernel(EmbedA
   }
 }
 
-__global__ __launch_bounds__(kThreads) void sort_place_kernel(EmbedArgs a, int from, int to, int shift, int bits,
-                                                              int64_t rpb) {
-  constexpr int W = kThreads / 64;
+// FEW: the counts are as they were counted.
+template <bool FEW>
+__global__ __launch_bounds__(kSortThreads) void sort_place_kernel(EmbedArgs a, int from, int to, int shift, int bits,
+                                                                  int64_t rpb) {
+  constexpr int W = kSortThreads / 64, PER = (1 << kMaxBits) / kSortThreads;
   extern __shared__ int next[];        // [W][bins]: counts of a wave's part, then the next place of each digit
   __shared__ int wave_sum[W];
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, bins = 1 << bits;
   const int64_t first = blockIdx.x * rpb, last = first + rpb < a.N ? first + rpb : a.N;
   const int64_t per = (last - first + W * 64 - 1) / (W * 64) * 64;
   const int64_t lo = first + w * per < last ? first + w * per : last, hi = lo + per < last ? lo + per : last;
-  for (int b = threadIdx.x; b < W * bins; b += kThreads) next[b] = 0;
-  __syncthreads();
-  for (int64_t i = lo + lane; i < hi; i += 64) atomicAdd(&next[w * bins + ((key_at(a, from, i) >> shift) & (bins - 1))], 1);
-  // The digits' first places: an exclusive scan of the totals, each thread a contiguous part.
-  const int chunk = (bins + kThreads - 1) / kThreads;
-  const int b0 = threadIdx.x * chunk < bins ? threadIdx.x * chunk : bins, b1 = b0 + chunk < bins ? b0 + chunk : bins;
-  int s = 0;
-  for (int b = b0; b < b1; ++b) s += a.totals[b];
-  int incl = s;
+  // This thread's digits, a contiguous part of them: how many there are in all, and in the blocks before.
+  const int chunk = (bins + kSortThreads - 1) / kSortThreads, b0 = threadIdx.x * chunk;
+  int total[PER], before[PER];
 #pragma unroll
-  for (int off = 1; off < 64; off *= 2) {
-    const int v = __shfl_up(incl, off);
-    if (lane >= off) incl += v;
+  for (int j = 0; j < PER; ++j) {
+    const int b = b0 + j;
+    const bool in = j < chunk && b < bins;
+    total[j] = before[j] = 0;
+    if constexpr (FEW) {
+      if (in) {
+#pragma unroll 8
+        for (int i = 0; i < (int)gridDim.x; ++i) {
+          const int n = a.hist[i * bins + b];
+          total[j] += n;
+          before[j] += i < (int)blockIdx.x ? n : 0;
+        }
+      }
+    } else if (in) {
+      total[j] = a.totals[b];
+      before[j] = a.hist[(int64_t)blockIdx.x * bins + b];
+    }
   }
+  for (int b = threadIdx.x; b < W * bins; b += kSortThreads) next[b] = 0;
+  __syncthreads();
+#pragma unroll 2
+  for (int64_t i = lo + lane; i < hi; i += 64) atomicAdd(&next[w * bins + ((key_at(a, from, i) >> shift) & (bins - 1))], 1);
+  // The digits' first places: an exclusive scan of the totals.
+  int s = 0;
+#pragma unroll
+  for (int j = 0; j < PER; ++j) s += total[j];
+  const int incl = lanes_scan(s, [](int p, int q) { return p + q; });
   if (lane == 63) wave_sum[w] = incl;
   __syncthreads();
   int at0 = incl - s;
   for (int q = 0; q < w; ++q) at0 += wave_sum[q];
-  for (int b = b0; b < b1; ++b) {
-    int at = at0 + a.hist[(int64_t)blockIdx.x * bins + b];
 #pragma unroll
-    for (int q = 0; q < W; ++q) {
-      const int n = next[q * bins + b];
-      next[q * bins + b] = at;
-      at += n;
+  for (int j = 0; j < PER; ++j) {
+    const int b = b0 + j;
+    if (j < chunk && b < bins) {
+      int at = at0 + before[j];
+#pragma unroll
+      for (int q = 0; q < W; ++q) {
+        const int n = next[q * bins + b];
+        next[q * bins + b] = at;
+        at += n;
+      }
+      at0 += total[j];
     }
-    at0 += a.totals[b];
   }
   __syncthreads();
   for (int64_t i0 = lo; i0 < hi; i0 += 64) {
     const int64_t i = i0 + lane;
     const bool in = i < hi;
     const uint32_t key = in ? key_at(a, from, i) : 0;
+    const int32_t pos = !in ? 0 : from < 0 ? (int32_t)i : a.pos[from][i];
     const int d = (key >> shift) & (bins - 1);
     uint64_t same = __ballot(in);
     for (int b = 0; b < bits; ++b) {
@@ -185,7 +216,7 @@ __global__ __launch_bounds__(kThreads) void sort_place_kernel(EmbedArgs a, int f
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     if (in) {
       a.key[to][at] = key;
-      a.pos[to][at] = from < 0 ? (int32_t)i : a.pos[from][i];
+      a.pos[to][at] = pos;
     }
   }
 }
@@ -288,7 +319,7 @@ __global__ __launch_bounds__(kThreads) void embed_sum_kernel(EmbedArgs a, int tx
 
 // The runs that leave the tile in which they began: that tile's part and those of the tiles after it.  A workgroup
 // takes a tile and 64 V columns, its four waves contiguous parts of the run.
-template <typename T>
+template <typename T, bool SHORT>
 __global__ __launch_bounds__(kThreads) void embed_join_kernel(EmbedArgs a, int sorted) {
   constexpr int V = 4, W = kThreads / 64;
   const uint32_t* key = a.key[sorted];
@@ -297,24 +328,38 @@ __global__ __launch_bounds__(kThreads) void embed_join_kernel(EmbedArgs a, int s
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
   const int c = ((int)blockIdx.y * 64 + lane) * V;
   for (int64_t tile = blockIdx.x; tile + 1 < tiles; tile += gridDim.x) {
-    const int64_t last = tile * kTile + kTile - 1;
-    const uint32_t v = key[last];
-    if (v == (uint32_t)a.V || key[last + 1] != v || (key[tile * kTile] == v && tile > 0 && key[tile * kTile - 1] == v))
-      continue;
-    const int64_t end = lower_bound(key, a.N, v + 1);           // of the run
-    const int64_t parts = (end - 1) / kTile - tile;             // tiles after this one
+    // (the keys at the tile's ends and at the starts of the next 64 tiles, in flight together)
+    const uint32_t v = key[tile * kTile + kTile - 1], start = key[tile * kTile], prior = tile > 0 ? key[tile * kTile - 1] : ~0u;
+    const auto starts = [&](int64_t q) { return (tile + q) * kTile < a.N ? key[(tile + q) * kTile] : ~0u; };
+    uint64_t same = __ballot(starts(1 + lane) == v);
+    if (v == (uint32_t)a.V || !(same & 1) || (start == v && prior == v)) continue;
+    int64_t parts = 0;                                          // tiles after this one that the run enters
+    while (same == ~0ull) {
+      parts += 64;
+      same = __ballot(starts(parts + 1 + lane) == v);
+    }
+    parts += __ffsll((unsigned long long)~same) - 1;
     const int64_t per = (parts + W - 1) / W, lo = w * per < parts ? w * per : parts, hi = lo + per < parts ? lo + per : parts;
     float acc[V] = {};
     if (c < a.D) {
-      const float* p = a.part + (tile + 1) * 2 * a.D + c;
-      if (w == 0) {
+      const auto part = [&](int64_t row) { return fetch16<SHORT>(a.part + row * a.D + c, a.D - c); };
+      const auto add = [&](uint4 u) {
+        float v[V];
+        unpack16<float>(keep16<SHORT, float>(u, a.D - c, a.D), v);
 #pragma unroll
-        for (int i = 0; i < V; ++i) if (c + i < a.D) acc[i] = a.part[(tile * 2 + 1) * a.D + c + i];
+        for (int i = 0; i < V; ++i) acc[i] += v[i];
+      };
+      if (w == 0) add(part(tile * 2 + 1));
+      constexpr int U = 8;             // rows in flight
+      int64_t q = lo;
+      for (; q + U <= hi; q += U) {
+        uint4 u[U];
+#pragma unroll
+        for (int j = 0; j < U; ++j) u[j] = part((tile + 1 + q + j) * 2);
+#pragma unroll
+        for (int j = 0; j < U; ++j) add(u[j]);
       }
-#pragma unroll 8
-      for (int64_t q = lo; q < hi; ++q)
-#pragma unroll
-        for (int i = 0; i < V; ++i) if (c + i < a.D) acc[i] += p[q * 2 * a.D + i];
+      for (; q < hi; ++q) add(part((tile + 1 + q) * 2));
     }
 #pragma unroll
     for (int i = 0; i < V; ++i) sums[w][lane][i] = acc[i];
@@ -322,10 +367,9 @@ __global__ __launch_bounds__(kThreads) void embed_join_kernel(EmbedArgs a, int s
     if (w == 0 && c < a.D) {
 #pragma unroll
       for (int i = 0; i < V; ++i) {
-        float s = acc[i];
 #pragma unroll
-        for (int q = 1; q < W; ++q) s += sums[q][lane][i];
-        if (c + i < a.D) static_cast<T*>(a.out)[(int64_t)v * a.D + c + i] = (T)(s * a.scale);
+        for (int q = 1; q < W; ++q) acc[i] += sums[q][lane][i];
+        if (c + i < a.D) static_cast<T*>(a.out)[(int64_t)v * a.D + c + i] = (T)(acc[i] * a.scale);
       }
     }
     __syncthreads();
@@ -356,7 +400,8 @@ void embed_sum_typed(const EmbedArgs& a, int sorted, hipStream_t s) {
   else embed_sum_kernel<T, false><<<grid, kThreads, 0, s>>>(a, tx, tile_blocks, sorted);
   if (tiles > 1) {
     const dim3 join((unsigned)(tiles - 1 < 65536 ? tiles - 1 : 65536), (unsigned)((a.D + 255) / 256));
-    embed_join_kernel<T><<<join, kThreads, 0, s>>>(a, sorted);
+    if (a.D < 4) embed_join_kernel<T, true><<<join, kThreads, 0, s>>>(a, sorted);
+    else embed_join_kernel<T, false><<<join, kThreads, 0, s>>>(a, sorted);
   }
 }
 
@@ -400,9 +445,14 @@ void launch_embed_bwd(const EmbedArgs& a, hipStream_t s) {
   int from = -1;
   for (int p = 0; p < passes; ++p) {
     const int to = p & 1, bins = 1 << bits;
-    sort_count_kernel<<<blocks, kThreads, bins * 4, s>>>(a, from, p * bits, bits, rpb);
-    sort_scan_kernel<<<(bins + kScanCols - 1) / kScanCols, kScanCols * kScanParts, 0, s>>>(a, bits, (int)blocks);
-    sort_place_kernel<<<blocks, kThreads, kThreads / 64 * bins * 4, s>>>(a, from, to, p * bits, bits, rpb);
+    const size_t lds = kSortThreads / 64 * bins * 4;
+    sort_count_kernel<<<blocks, kSortThreads, bins * 4, s>>>(a, from, p * bits, bits, rpb);
+    if ((int)blocks <= kFewBlocks) {
+      sort_place_kernel<true><<<blocks, kSortThreads, lds, s>>>(a, from, to, p * bits, bits, rpb);
+    } else {
+      sort_scan_kernel<<<(bins + kScanCols - 1) / kScanCols, kScanCols * kScanParts, 0, s>>>(a, bits, (int)blocks);
+      sort_place_kernel<false><<<blocks, kSortThreads, lds, s>>>(a, from, to, p * bits, bits, rpb);
+    }
     from = to;
   }
   if (a.elem == ELEM_F32) embed_sum_typed<float>(a, from, s);
