@@ -125,6 +125,9 @@ def _declare(lib):
                                                         vp]),
         "gmmxx_hip_quantize": (ctypes.c_int, [i32, i64, i64, vp, i64, vp, i64, vp, vp]),
         "gmmxx_hip_quantized_matmul": (ctypes.c_int, [i32, i64, i64, i64, vp, i64, vp, vp, i64, vp, vp, vp, vp]),
+        "gmmxx_hip_quantized_linear_workspace_bytes": (i64, [i32, i64, i64]),
+        "gmmxx_hip_quantized_linear": (ctypes.c_int, [i32, i32, i64, i64, i64, vp, i64, vp, i64, vp, vp, vp, vp, i64,
+                                                      vp]),
     }
     for name, (res, args) in sig.items():
         fn = getattr(lib, name)
@@ -148,7 +151,8 @@ def exported_symbols() -> Tuple[str, ...]:
             "gmmxx_hip_combine", "gmmxx_hip_combine_backward",
             "gmmxx_hip_embed", "gmmxx_hip_embed_workspace_bytes", "gmmxx_hip_embed_backward", "gmmxx_hip_dropout",
             "gmmxx_hip_log_probs_workspace_bytes", "gmmxx_hip_log_probs", "gmmxx_hip_log_probs_backward",
-            "gmmxx_hip_quantize", "gmmxx_hip_quantized_matmul")
+            "gmmxx_hip_quantize", "gmmxx_hip_quantized_matmul", "gmmxx_hip_quantized_linear_workspace_bytes",
+            "gmmxx_hip_quantized_linear")
 
 
 def load_library(path: Optional[str] = None):

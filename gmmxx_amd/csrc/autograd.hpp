@@ -43,6 +43,8 @@ struct Library {
   decltype(&gmmxx_hip_log_probs_backward) log_probs_backward = nullptr;
   decltype(&gmmxx_hip_quantize) quantize = nullptr;
   decltype(&gmmxx_hip_quantized_matmul) quantized_matmul = nullptr;
+  decltype(&gmmxx_hip_quantized_linear_workspace_bytes) quantized_linear_workspace_bytes = nullptr;
+  decltype(&gmmxx_hip_quantized_linear) quantized_linear = nullptr;
 } lib;
 
 void bind(const std::unordered_map<std::string, uintptr_t>& at) {
@@ -70,6 +72,8 @@ void bind(const std::unordered_map<std::string, uintptr_t>& at) {
   take(lib.log_probs_backward, "log_probs_backward");
   take(lib.quantize, "quantize");
   take(lib.quantized_matmul, "quantized_matmul");
+  take(lib.quantized_linear_workspace_bytes, "quantized_linear_workspace_bytes");
+  take(lib.quantized_linear, "quantized_linear");
 }
 
 // The device of a call: current while it lives, with its current stream.

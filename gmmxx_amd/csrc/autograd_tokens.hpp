@@ -205,14 +205,20 @@ Tensor quantized_matmul(const Tensor& x0, const std::optional<Tensor>& xscales, 
   Tensor out = at::empty({n, f}, x.options().dtype(type));
   if (n == 0) return out;
   On on(x);
-  Tensor values = x, xs = xs0;
-  if (!xs.defined()) std::tie(values, xs) = quantize_forward(x);
-  else values = whole_rows(x);
   const Tensor w = whole_rows(w0);
-  const int64_t whole = (d + 15) / 16 * 16;
+  const int64_t whole = (d + 15) / 16 * 16, ldw = f > 1 ? w.stride(0) : whole;
+  const int8_t* wp = static_cast<int8_t*>(ptr(w));
+  if (!xs0.defined()) {
+    const int64_t need = lib.quantized_linear_workspace_bytes(elem(x), n, d);
+    const Tensor ws = need ? bytes(need, x) : Tensor();
+    check(lib.quantized_linear(elem(x), elem(type), n, f, d, ptr(x), x.stride(0), wp, ldw, floats(plain(wscales)),
+                               ptr(bias), ptr(out), ptr(ws), need, on.stream()),
+          "quantized_linear");
+    return out;
+  }
+  const Tensor values = whole_rows(x);
   check(lib.quantized_matmul(elem(type), n, f, d, static_cast<int8_t*>(ptr(values)), n > 1 ? values.stride(0) : whole,
-                             floats(plain(xs)), static_cast<int8_t*>(ptr(w)), f > 1 ? w.stride(0) : whole,
-                             floats(plain(wscales)), ptr(bias), ptr(out), on.stream()),
+                             floats(plain(xs0)), wp, ldw, floats(plain(wscales)), ptr(bias), ptr(out), on.stream()),
         "quantized_matmul");
   return out;
 }

@@ -155,8 +155,7 @@ struct Core {
       i32x4 m;
 #pragma unroll
       for (int d = 0; d < 4; ++d)
-        if constexpr (sizeof(T) == 1) m[d] = left >= 4 * d + 4 ? -1 : (left > 4 * d ? (1 << 8 * (left - 4 * d)) - 1 : 0);
-        else m[d] = sizeof(T) == 4 ? (left > d ? -1 : 0) : left >= 2 * d + 2 ? -1 : (left == 2 * d + 1 ? 0xffff : 0);
+        m[d] = sizeof(T) == 4 ? (left > d ? -1 : 0) : left >= 2 * d + 2 ? -1 : (left == 2 * d + 1 ? 0xffff : 0);
 #pragma unroll
       for (int i = 0; i < TP; ++i) p[i] &= m;
 #pragma unroll

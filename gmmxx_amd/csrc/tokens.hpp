@@ -87,5 +87,8 @@ struct QuantMatmulArgs {
   int D, elem;
 };
 void launch_quant_matmul(const QuantMatmulArgs& a, hipStream_t s);
+// The two one after the other (x.values is a.x), or one kernel without x.values and x.scales.
+bool quant_linear_at_once(int64_t N, int D, int elem);
+void launch_quant_linear(const QuantArgs& x, const QuantMatmulArgs& a, hipStream_t s);
 
 }  // namespace gx::layer

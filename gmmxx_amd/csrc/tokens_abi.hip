@@ -52,6 +52,25 @@ int check_logp(int elem, int64_t N, int64_t V, int64_t k, int index_bits) {
   return GMMXX_OK;
 }
 
+int check_quant(int elem, int64_t N, int64_t F, int64_t D) {
+  if (!is_elem(elem)) return invalid("elem must be GMMXX_F32, GMMXX_BF16 or GMMXX_F16");
+  if (N < 0 || F <= 0 || D <= 0) return invalid("N must be non-negative and F and D positive");
+  if (D > kQuantMaxD) return unsupported("D > 131072");
+  if (F > kMaxDim) return unsupported("F > 2^22");
+  if (N >= kMaxPositions) return unsupported("N >= 2^30");
+  return GMMXX_OK;
+}
+
+int check_values(const int8_t* values, int64_t ld) {
+  if (ld % 16 != 0 || ld < 0 || (uintptr_t)values % 16 != 0)
+    return invalid("x and w must lie in rows of whole, aligned 16 bytes");
+  if (ld > (1 << 23)) return unsupported("row strides > 2^23");
+  return GMMXX_OK;
+}
+
+int64_t values_row(int64_t D) { return (D + kQuantPad - 1) / kQuantPad * kQuantPad; }
+int64_t values_bytes(int64_t N, int64_t D) { return (N * values_row(D) + 255) / 256 * 256; }
+
 }  // namespace
 
 extern "C" {
@@ -172,21 +191,44 @@ int gmmxx_hip_quantize(int elem, int64_t N, int64_t D, const void* x, int64_t ld
 int gmmxx_hip_quantized_matmul(int elem, int64_t N, int64_t F, int64_t D, const int8_t* x, int64_t ldx,
                                const float* xscales, const int8_t* w, int64_t ldw, const float* wscales,
                                const void* bias, void* out, void* stream) {
-  if (!is_elem(elem)) return invalid("elem must be GMMXX_F32, GMMXX_BF16 or GMMXX_F16");
-  if (N < 0 || F <= 0 || D <= 0) return invalid("N must be non-negative and F and D positive");
-  if (D > kQuantMaxD) return unsupported("D > 131072");
-  if (F > kMaxDim) return unsupported("F > 2^22");
-  if (N >= kMaxPositions) return unsupported("N >= 2^30");
+  if (int rc = check_quant(elem, N, F, D)) return rc;
   if (N == 0) return GMMXX_OK;
   if (!x || !xscales || !w || !wscales || !out) return invalid("NULL buffer");
-  if (ldx % 16 != 0 || ldw % 16 != 0 || ldx < 0 || ldw < 0 || (uintptr_t)x % 16 != 0 || (uintptr_t)w % 16 != 0)
-    return invalid("x and w must lie in rows of whole, aligned 16 bytes");
-  if (ldx > (1 << 23) || ldw > (1 << 23)) return unsupported("row strides > 2^23");
+  if (int rc = check_values(x, ldx)) return rc;
+  if (int rc = check_values(w, ldw)) return rc;
   QuantMatmulArgs a{};
   a.x = x; a.ldx = ldx; a.xs = xscales; a.w = w; a.ldw = ldw; a.ws = wscales; a.bias = bias; a.out = out;
   a.N = N; a.F = F; a.D = (int)D; a.elem = elem;
   launch_quant_matmul(a, (hipStream_t)stream);
   return launch_status("quantized_matmul");
+}
+
+int64_t gmmxx_hip_quantized_linear_workspace_bytes(int elem, int64_t N, int64_t D) {
+  if (check_quant(elem, N, 1, D)) return -1;
+  if (N == 0 || quant_linear_at_once(N, (int)D, elem)) return 0;
+  return values_bytes(N, D) + (N * 4 + 255) / 256 * 256;
+}
+
+int gmmxx_hip_quantized_linear(int elem, int out_elem, int64_t N, int64_t F, int64_t D, const void* x, int64_t ldx,
+                               const int8_t* w, int64_t ldw, const float* wscales, const void* bias, void* out,
+                               void* workspace, int64_t workspace_bytes, void* stream) {
+  if (int rc = check_quant(elem, N, F, D)) return rc;
+  if (!is_elem(out_elem)) return invalid("out_elem must be GMMXX_F32, GMMXX_BF16 or GMMXX_F16");
+  if (N == 0) return GMMXX_OK;
+  if (!x || !w || !wscales || !out) return invalid("NULL buffer");
+  if (ldx < 0) return invalid("row strides must be non-negative");
+  if (int rc = check_values(w, ldw)) return rc;
+  if (const int64_t need = gmmxx_hip_quantized_linear_workspace_bytes(elem, N, D))
+    if (int rc = check_workspace(workspace, workspace_bytes, need)) return rc;
+  QuantArgs q{};
+  q.x = x; q.ldx = ldx; q.N = N; q.D = (int)D; q.elem = elem;
+  q.values = static_cast<int8_t*>(workspace); q.ldv = values_row(D);
+  q.scales = reinterpret_cast<float*>(static_cast<char*>(workspace) + values_bytes(N, D));
+  QuantMatmulArgs a{};
+  a.x = q.values; a.ldx = q.ldv; a.xs = q.scales; a.w = w; a.ldw = ldw; a.ws = wscales; a.bias = bias; a.out = out;
+  a.N = N; a.F = F; a.D = (int)D; a.elem = out_elem;
+  launch_quant_linear(q, a, (hipStream_t)stream);
+  return launch_status("quantized_linear");
 }
 
 }  // extern "C"

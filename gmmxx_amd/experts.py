@@ -90,7 +90,7 @@ _ENTRY_POINTS = ("last_error", "layer_norm", "layer_norm_workspace_bytes", "laye
                  "route_workspace_bytes", "route", "route_backward", "grouped_matmul", "grouped_workspace_bytes",
                  "grouped_weight_grad", "combine", "combine_backward", "embed", "embed_workspace_bytes",
                  "embed_backward", "dropout", "log_probs_workspace_bytes", "log_probs", "log_probs_backward",
-                 "quantize", "quantized_matmul")
+                 "quantize", "quantized_matmul", "quantized_linear_workspace_bytes", "quantized_linear")
 _ops = None
 
 

@@ -438,6 +438,15 @@ int gmmxx_hip_quantized_matmul(int elem, int64_t N, int64_t F, int64_t D, const 
                                const float* xscales, const int8_t* w, int64_t ldw, const float* wscales,
                                const void* bias, void* out, void* stream);
 
+/* The same of N rows of D elements that are brought into 8 bits here, as gmmxx_hip_quantize does:
+ * out (N, F) and bias are of out_elem.  The workspace takes
+ * gmmxx_hip_quantized_linear_workspace_bytes (0 for up to 8 rows that are not too long, which
+ * take one kernel). */
+int64_t gmmxx_hip_quantized_linear_workspace_bytes(int elem, int64_t N, int64_t D);
+int gmmxx_hip_quantized_linear(int elem, int out_elem, int64_t N, int64_t F, int64_t D, const void* x, int64_t ldx,
+                               const int8_t* w, int64_t ldw, const float* wscales, const void* bias, void* out,
+                               void* workspace, int64_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

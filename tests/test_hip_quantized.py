@@ -193,3 +193,44 @@ def test_past_32_bits(hip):
     w = whole(f, d, seed=1)
     y = gmmxx_amd.quantized_matmul(Quantized(x, torch.ones(n, device=DEV)), Quantized(w, ones[:f]))
     assert torch.equal(y[-3:], x[-3:].float() @ w.float().t())
+
+
+@pytest.mark.parametrize("dtype", experts_ref.DTYPES, ids=str)
+@pytest.mark.parametrize("d", [4, 7, 8, 9, 500, 1000, 4096, 4100, 8192, 16_000, 16_400, 32_768, 40_000])
+@pytest.mark.parametrize("n", [1, 2, 3, 4, 5, 8, 9])
+def test_few_rows(hip, n, d, dtype):
+    """Rows that are brought into 8 bits by the product's own workgroups, up to where they are too many or too long."""
+    print(f"[int8] few n={n} d={d} {dtype}", flush=True)
+    check(n, d, 40, dtype, seed=d)
+
+
+@pytest.mark.parametrize("n", [4, 30, 100])
+def test_other_result_types(hip, n):
+    q = gmmxx_amd.quantize_rows(rand(50, 333, seed=1))
+    for dtype in experts_ref.DTYPES:
+        x = rand(n, 333, dtype=dtype)
+        qx, sx = ref.quantize(x)
+        for out in experts_ref.DTYPES:
+            b = rand(50, seed=2, dtype=out)
+            y = gmmxx_amd.quantized_matmul(x, q, b, dtype=out)
+            assert y.dtype == out
+            experts_ref.close(y, *ref.quantized_matmul(qx, sx, q.values, q.scales, b, out), f"{dtype} {out}")
+
+
+@pytest.mark.parametrize("n", [1, 2, 4, 7, 20, 100])
+def test_rows_of_zeros_and_not_finite(hip, n):
+    x, q = rand(n, 300, dtype=F32), gmmxx_amd.quantize_rows(rand(70, 300, seed=1))
+    want = gmmxx_amd.quantized_matmul(x, q)
+    for bad in (float("nan"), float("inf")):
+        y = x.clone()
+        y[n // 2, 299] = bad
+        y = gmmxx_amd.quantized_matmul(y, q)
+        assert torch.isnan(y[n // 2]).all()
+        keep = [i for i in range(n) if i != n // 2]
+        assert torch.equal(y[keep], want[keep])
+    x[n // 2] = 0.0
+    y = gmmxx_amd.quantized_matmul(x, q, rand(70, seed=3))
+    assert torch.equal(y[n // 2], rand(70, seed=3))
+    wide = torch.zeros((n, 411), dtype=F16, device=DEV)
+    wide[:, 7:307] = rand(n, 300, dtype=F16)
+    assert torch.equal(gmmxx_amd.quantized_matmul(wide[:, 7:307], q), gmmxx_amd.quantized_matmul(rand(n, 300, dtype=F16), q))

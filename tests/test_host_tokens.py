@@ -65,6 +65,10 @@ def matmul(lib, elem=F32, n=3, f=5, d=8, x=P, ldx=16, xs=P, w=P, ldw=16, ws=P, o
     return lib.gmmxx_hip_quantized_matmul(elem, n, f, d, x, ldx, xs, w, ldw, ws, NULL, out, NULL)
 
 
+def linear(lib, elem=F32, out_elem=F32, n=30, f=5, d=8, x=P, ldx=8, w=P, ldw=16, ws=P, out=P, work=P, size=1 << 30):
+    return lib.gmmxx_hip_quantized_linear(elem, out_elem, n, f, d, x, ldx, w, ldw, ws, NULL, out, work, size, NULL)
+
+
 ODD = ctypes.c_void_p(4100)
 CASES = [
     (embed, dict(elem=7), INVALID, "elem"), (embed, dict(n=-1), INVALID, "N"), (embed, dict(v=0), INVALID, "V"),
@@ -111,6 +115,14 @@ CASES = [
     (matmul, dict(out=NULL), INVALID, "NULL"), (matmul, dict(ldx=24), INVALID, "16"), (matmul, dict(ldw=-16), INVALID, "16"),
     (matmul, dict(x=ODD), INVALID, "16"), (matmul, dict(w=ODD), INVALID, "16"),
     (matmul, dict(ldw=1 << 24), UNSUPPORTED, "2^23"),
+    (linear, dict(elem=9), INVALID, "elem"), (linear, dict(out_elem=4), INVALID, "out_elem"),
+    (linear, dict(n=-1), INVALID, "N"), (linear, dict(f=0), INVALID, "F"), (linear, dict(d=0), INVALID, "D"),
+    (linear, dict(d=(1 << 17) + 1), UNSUPPORTED, "131072"), (linear, dict(f=(1 << 22) + 1), UNSUPPORTED, "2^22"),
+    (linear, dict(x=NULL), INVALID, "NULL"), (linear, dict(w=NULL), INVALID, "NULL"),
+    (linear, dict(ws=NULL), INVALID, "NULL"), (linear, dict(out=NULL), INVALID, "NULL"),
+    (linear, dict(ldx=-8), INVALID, "strides"), (linear, dict(ldw=40), INVALID, "16"), (linear, dict(w=ODD), INVALID, "16"),
+    (linear, dict(work=NULL), WORKSPACE, "NULL"), (linear, dict(size=100), WORKSPACE, "small"),
+    (linear, dict(work=ODD), WORKSPACE, "aligned"),
 ]
 
 
@@ -129,6 +141,7 @@ def test_no_rows(lib):
     assert logp_back(lib, n=0, stats=NULL, ds=NULL) == OK
     assert quantize(lib, n=0, x=NULL, values=NULL, scales=NULL) == OK
     assert matmul(lib, n=0, x=NULL, out=NULL) == OK
+    assert linear(lib, n=0, x=NULL, out=NULL, work=NULL, size=0) == OK
 
 
 def test_workspace_sizes(lib):
@@ -140,6 +153,10 @@ def test_workspace_sizes(lib):
     assert lib.gmmxx_hip_log_probs_workspace_bytes(3, 9, 10) == -1
     assert lib.gmmxx_hip_log_probs_workspace_bytes(0, 9, 2) == 0
     assert lib.gmmxx_hip_log_probs_workspace_bytes(100_000, 500, 0) == 0
+    # rows of whole 128 bytes and a scale each, none where one kernel does it all
+    assert lib.gmmxx_hip_quantized_linear_workspace_bytes(F32, 30, 0) == -1
+    assert lib.gmmxx_hip_quantized_linear_workspace_bytes(BF16, 4, 4096) == 0
+    assert lib.gmmxx_hip_quantized_linear_workspace_bytes(BF16, 300, 129) >= 300 * 260
     # a long row in parts: three statistics and the alternatives of each
     assert lib.gmmxx_hip_log_probs_workspace_bytes(1, 1 << 20, 5) >= 2 * (12 + 40)
 
