@@ -8,8 +8,8 @@
 // inside a tile is a row of the result, rounded once; the parts of a run that reaches over
 // tiles are written as fp32 (at most two rows a tile: the run that enters it and the run
 // that leaves it) and added in order by a second kernel, a workgroup for each run and
-// columns.  Rows without a token are written by workgroups of the same launch, which find
-// them by binary searches in the sorted tokens.  No sum depends on the order in which
+// columns.  Rows without a token, of which the sort's last pass leaves a mark in every other, are zeroed
+// by workgroups of the same launch.  No sum depends on the order in which
 // workgroups finish.
 //
 // The sort takes the fewest passes of at most 11 bits; a pass counts digits by block,
@@ -92,10 +92,17 @@ __device__ __forceinline__ uint32_t key_at(const EmbedArgs& a, int from, int64_t
   return (uint64_t)t < (uint64_t)a.V ? (uint32_t)t : (uint32_t)a.V;
 }
 
+// Zeros in seen, by all threads of the grid (in a launch before those that set it).
+__device__ __forceinline__ void clear_seen(const EmbedArgs& a, int threads) {
+  for (int64_t i = ((int64_t)blockIdx.x * threads + threadIdx.x) * 16; i < a.V; i += (int64_t)gridDim.x * threads * 16)
+    *reinterpret_cast<uint4*>(a.seen + i) = make_uint4(0, 0, 0, 0);      // (room for whole 256 bytes)
+}
+
 __global__ __launch_bounds__(kSortThreads) void sort_count_kernel(EmbedArgs a, int from, int shift, int bits,
                                                                   int64_t rpb) {
   extern __shared__ int count[];
   const int bins = 1 << bits;
+  if (from < 0) clear_seen(a, kSortThreads);
   for (int b = threadIdx.x; b < bins; b += kSortThreads) count[b] = 0;
   __syncthreads();
   const int64_t first = blockIdx.x * rpb, last = first + rpb < a.N ? first + rpb : a.N;
@@ -140,7 +147,7 @@ __global__ __launch_bounds__(kScanCols* kScanParts) void sort_scan_kernel(EmbedA
 // FEW: the counts are as they were counted.
 template <bool FEW>
 __global__ __launch_bounds__(kSortThreads) void sort_place_kernel(EmbedArgs a, int from, int to, int shift, int bits,
-                                                                  int64_t rpb) {
+                                                                  int64_t rpb, int last_pass) {
   constexpr int W = kSortThreads / 64, PER = (1 << kMaxBits) / kSortThreads;
   extern __shared__ int next[];        // [W][bins]: counts of a wave's part, then the next place of each digit
   __shared__ int wave_sum[W];
@@ -217,22 +224,81 @@ __global__ __launch_bounds__(kSortThreads) void sort_place_kernel(EmbedArgs a, i
     if (in) {
       a.key[to][at] = key;
       a.pos[to][at] = pos;
+      if (last_pass && key < a.V) a.seen[key] = 1;
     }
   }
 }
 
-// --- sums ---------------------------------------------------------------------
-
-// The first sorted place whose token is v or more.
-__device__ __forceinline__ int64_t lower_bound(const uint32_t* key, int64_t N, uint32_t v) {
-  int64_t lo = 0, hi = N;
-  while (lo < hi) {
-    const int64_t mid = (lo + hi) >> 1;
-    if (key[mid] < v) lo = mid + 1;
-    else hi = mid;
+// The whole sort of up to kOneRows tokens by one workgroup in LDS, at most kOneBits a pass: a training step of few
+// tokens takes one launch for it where it took up to six (each several us of the host's time).
+constexpr int kOneRows = 4096, kOneThreads = 1024, kOneBits = 9;
+__global__ __launch_bounds__(kOneThreads) void sort_one_kernel(EmbedArgs a, int all, int bits) {
+  constexpr int W = kOneThreads / 64, Bins = 1 << kOneBits;
+  __shared__ uint32_t key[2][kOneRows];
+  __shared__ uint16_t pos[2][kOneRows];
+  __shared__ int next[W][Bins], wave_sum[Bins / 64];
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, N = (int)a.N;
+  const int per = (N + W * 64 - 1) / (W * 64) * 64, lo = min(w * per, N), hi = min(lo + per, N);
+  for (int i = threadIdx.x; i < N; i += kOneThreads) {
+    key[0][i] = key_at(a, -1, i);
+    pos[0][i] = (uint16_t)i;
   }
-  return lo;
+  clear_seen(a, kOneThreads);
+  int from = 0;
+  for (int shift = 0; shift < all; shift += bits, from ^= 1) {
+    for (int b = threadIdx.x; b < W * Bins; b += kOneThreads) next[0][b] = 0;
+    __syncthreads();
+    for (int i = lo + lane; i < hi; i += 64) atomicAdd(&next[w][key[from][i] >> shift & ((1 << bits) - 1)], 1);
+    __syncthreads();
+    int total = 0, incl = 0;
+    if (threadIdx.x < Bins) {
+#pragma unroll
+      for (int q = 0; q < W; ++q) total += next[q][threadIdx.x];
+      incl = lanes_scan(total, [](int p, int q) { return p + q; });
+      if (lane == 63) wave_sum[w] = incl;
+    }
+    __syncthreads();
+    if (threadIdx.x < Bins) {
+      int at = incl - total;
+      for (int q = 0; q < w; ++q) at += wave_sum[q];
+#pragma unroll
+      for (int q = 0; q < W; ++q) {
+        const int n = next[q][threadIdx.x];
+        next[q][threadIdx.x] = at;
+        at += n;
+      }
+    }
+    __syncthreads();
+    for (int i0 = lo; i0 < hi; i0 += 64) {
+      const int i = i0 + lane;
+      const bool in = i < hi;
+      const uint32_t k = in ? key[from][i] : 0;
+      const int d = k >> shift & ((1 << bits) - 1);
+      uint64_t same = __ballot(in);
+      for (int b = 0; b < bits; ++b) {
+        const uint64_t set = __ballot((d >> b) & 1);
+        same &= (d >> b) & 1 ? set : ~set;
+      }
+      const int rank = __popcll(same & ((1ull << lane) - 1));
+      const int at = next[w][d] + rank;
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      if (in && rank == 0) next[w][d] += __popcll(same);
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      if (in) {
+        key[from ^ 1][at] = k;
+        pos[from ^ 1][at] = pos[from][i];
+      }
+    }
+    __syncthreads();
+  }
+  for (int i = threadIdx.x; i < N; i += kOneThreads) {
+    a.key[0][i] = key[from][i];
+    a.pos[0][i] = pos[from][i];
+    if (key[from][i] < a.V) a.seen[key[from][i]] = 1;
+  }
 }
+
+// --- sums ---------------------------------------------------------------------
 
 template <typename T>
 __device__ __forceinline__ void store_scaled(T* p, int valid, const float (&v)[kVec<T>], float scale) {
@@ -258,61 +324,74 @@ __global__ __launch_bounds__(kThreads) void embed_sum_kernel(EmbedArgs a, int tx
   const uint32_t* key = a.key[sorted];
   T* out = static_cast<T*>(a.out);
   if ((int64_t)blockIdx.x >= tile_blocks) {
-    __shared__ int64_t first[65];
+    __shared__ uint8_t seen[64];
     const int64_t v0 = ((int64_t)blockIdx.x - tile_blocks) * 64;
-    if (threadIdx.x <= 64) first[threadIdx.x] = lower_bound(key, a.N, (uint32_t)(v0 + threadIdx.x < a.V ? v0 + threadIdx.x : a.V));
+    if (threadIdx.x < 64) seen[threadIdx.x] = v0 + threadIdx.x < a.V ? a.seen[v0 + threadIdx.x] : 1;
     __syncthreads();
     const int lane = threadIdx.x & (tx - 1), step = kThreads / tx;
     float zero[V] = {};
     const int c = ((int)blockIdx.y * tx + lane) * V;
     if (c < a.D)
       for (int r = threadIdx.x / tx; r < 64 && v0 + r < a.V; r += step)
-        if (first[r] == first[r + 1]) store_row(out + (v0 + r) * a.D + c, a.D - c, zero);
+        if (!seen[r]) store_row(out + (v0 + r) * a.D + c, a.D - c, zero);
     return;
   }
   const int lane = threadIdx.x & (tx - 1), sub = threadIdx.x / tx, per = kThreads / tx;
-  __shared__ uint32_t keys[kThreads / 8][kTile + 2];
+  // This workgroup's tiles: their tokens, with those before and after, their positions and where their runs end.
+  __shared__ uint32_t keys[kThreads / 8][kTile + 2], ends[kThreads / 8];
   __shared__ int32_t pos[kThreads / 8][kTile];
-  // the tokens of this workgroup's tiles, and of the places before and after each
+  const uint32_t none = (uint32_t)a.V;
   const int64_t t0 = (int64_t)blockIdx.x * per;
+  if ((int)threadIdx.x < per) ends[threadIdx.x] = 0;
   for (int i = threadIdx.x; i < per * (kTile + 2); i += kThreads) {
     const int64_t at = (t0 + i / (kTile + 2)) * kTile + i % (kTile + 2) - 1;
-    keys[i / (kTile + 2)][i % (kTile + 2)] = at >= 0 && at < a.N ? key[at] : (uint32_t)a.V;
+    keys[i / (kTile + 2)][i % (kTile + 2)] = at >= 0 && at < a.N ? key[at] : none;
   }
   for (int i = threadIdx.x; i < per * kTile; i += kThreads) {
     const int64_t at = t0 * kTile + i;
-    const int32_t p = at < a.N ? a.pos[sorted][at] : 0;
-    pos[i / kTile][i % kTile] = p;
+    pos[i / kTile][i % kTile] = at < a.N ? a.pos[sorted][at] : 0;
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < per * kTile; i += kThreads) {
+    const uint32_t* k = keys[i / kTile] + 1 + i % kTile;
+    if (k[0] != none && (k[0] != k[1] || i % kTile == kTile - 1)) atomicOr(&ends[i / kTile], 1u << (i % kTile));
   }
   __syncthreads();
   const int c = ((int)blockIdx.y * tx + lane) * V;
   const int64_t tile = t0 + sub;
-  if (c >= a.D || tile * kTile >= a.N) return;
-  const uint32_t none = (uint32_t)a.V;
+  const uint32_t marks = ends[sub];
+  if (c >= a.D || marks == 0) return;              // (no token in it)
+  const int n = 32 - __clz((int)marks);            // its tokens: a run ends with the last of them
   const uint32_t* k = keys[sub] + 1;
-  const T* dy = static_cast<const T*>(a.dy);
+  const T* dy = static_cast<const T*>(a.dy) + c;
   float acc[V] = {};
-  bool entered = k[-1] == k[0] && tile > 0;        // the run at hand began in an earlier tile
-  for (int i0 = 0; i0 < kTile; i0 += U) {
-    if (k[i0] == none) break;                      // (the others follow)
+  bool entered = tile > 0 && k[-1] == k[0];        // the run at hand began in an earlier tile
+  const bool leaves = n == kTile && k[kTile] == k[kTile - 1];
+  uint4 next[U];
+  const auto fetch = [&](int i0) {
+#pragma unroll
+    for (int j = 0; j < U; ++j) next[j] = fetch16<SHORT>(dy + (int64_t)pos[sub][i0 + j] * a.lddy, a.D - c);
+  };
+  fetch(0);
+  for (int i0 = 0; i0 < n; i0 += U) {
     uint4 u[U];
 #pragma unroll
-    for (int j = 0; j < U; ++j) u[j] = fetch16<SHORT>(dy + (int64_t)pos[sub][i0 + j] * a.lddy + c, a.D - c);
+    for (int j = 0; j < U; ++j) u[j] = next[j];
+    if (i0 + U < n) fetch(i0 + U);
 #pragma unroll
-    for (int j = 0; j < U; ++j) {
-      const uint32_t at = k[i0 + j];
-      if (at == none) break;
+    for (int j = 0; j < U; ++j) {                  // (what is added after the last end is not used)
       float v[V];
       unpack16<T>(keep16<SHORT, T>(u[j], a.D - c, a.D), v);
 #pragma unroll
       for (int i = 0; i < V; ++i) acc[i] += v[i];
-      const bool leaves = i0 + j == kTile - 1 && k[kTile] == at;
-      if (k[i0 + j + 1] == at && !leaves) continue;
-      if (entered || leaves) store_part(a.part + (tile * 2 + !entered) * a.D + c, a.D - c, acc);
-      else store_scaled(out + (int64_t)at * a.D + c, a.D - c, acc, a.scale);
+      if (marks >> (i0 + j) & 1) {
+        const bool away = leaves && i0 + j == kTile - 1;
+        if (entered || away) store_part(a.part + (tile * 2 + !entered) * a.D + c, a.D - c, acc);
+        else store_scaled(out + (int64_t)k[i0 + j] * a.D + c, a.D - c, acc, a.scale);
 #pragma unroll
-      for (int i = 0; i < V; ++i) acc[i] = 0.f;
-      entered = false;
+        for (int i = 0; i < V; ++i) acc[i] = 0.f;
+        entered = false;
+      }
     }
   }
 }
@@ -429,6 +508,7 @@ void embed_workspace(EmbedArgs& a, void* ws) {
   for (int i = 0; i < 2; ++i) take(a.pos[i], a.N * 4);
   take(a.hist, blocks * (int64_t(1) << digit) * 4);
   take(a.totals, (int64_t(1) << digit) * 4);
+  take(a.seen, a.V);
   a.part = reinterpret_cast<float*>(p);
 }
 
@@ -443,17 +523,23 @@ void launch_embed_bwd(const EmbedArgs& a, hipStream_t s) {
   const unsigned blocks = (unsigned)((a.N + rpb - 1) / rpb);
   const int all = key_bits(a.V), passes = (all + kMaxBits - 1) / kMaxBits, bits = (all + passes - 1) / passes;
   int from = -1;
-  for (int p = 0; p < passes; ++p) {
-    const int to = p & 1, bins = 1 << bits;
-    const size_t lds = kSortThreads / 64 * bins * 4;
-    sort_count_kernel<<<blocks, kSortThreads, bins * 4, s>>>(a, from, p * bits, bits, rpb);
-    if ((int)blocks <= kFewBlocks) {
-      sort_place_kernel<true><<<blocks, kSortThreads, lds, s>>>(a, from, to, p * bits, bits, rpb);
-    } else {
-      sort_scan_kernel<<<(bins + kScanCols - 1) / kScanCols, kScanCols * kScanParts, 0, s>>>(a, bits, (int)blocks);
-      sort_place_kernel<false><<<blocks, kSortThreads, lds, s>>>(a, from, to, p * bits, bits, rpb);
+  if (a.N <= kOneRows) {
+    const int one = (all + kOneBits - 1) / kOneBits;
+    sort_one_kernel<<<1, kOneThreads, 0, s>>>(a, all, (all + one - 1) / one);
+    from = 0;
+  } else {
+    for (int p = 0; p < passes; ++p) {
+      const int to = p & 1, bins = 1 << bits;
+      const size_t lds = kSortThreads / 64 * bins * 4;
+      sort_count_kernel<<<blocks, kSortThreads, bins * 4, s>>>(a, from, p * bits, bits, rpb);
+      if ((int)blocks <= kFewBlocks) {
+        sort_place_kernel<true><<<blocks, kSortThreads, lds, s>>>(a, from, to, p * bits, bits, rpb, p + 1 == passes);
+      } else {
+        sort_scan_kernel<<<(bins + kScanCols - 1) / kScanCols, kScanCols * kScanParts, 0, s>>>(a, bits, (int)blocks);
+        sort_place_kernel<false><<<blocks, kSortThreads, lds, s>>>(a, from, to, p * bits, bits, rpb, p + 1 == passes);
+      }
+      from = to;
     }
-    from = to;
   }
   if (a.elem == ELEM_F32) embed_sum_typed<float>(a, from, s);
   else if (a.elem == ELEM_BF16) embed_sum_typed<__bf16>(a, from, s);

@@ -17,7 +17,6 @@ namespace gx::layer {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int64_t kMaxBlocks = 1 << 20;
 
 // --- quantisation ----------------------------------------------------------------
 
@@ -109,7 +108,8 @@ __global__ __launch_bounds__(kThreads) void quantize_kernel(QuantArgs a) {
 template <typename T, int G, int NV, bool SHORT = false>
 void quantize_shaped(const QuantArgs& a, hipStream_t s) {
   const int64_t need = (a.N + kThreads / G - 1) / (kThreads / G);
-  quantize_kernel<T, G, NV, SHORT><<<(unsigned)(need < kMaxBlocks ? need : kMaxBlocks), kThreads, 0, s>>>(a);
+  // (workgroups that take several rows: 16384 x 4096 bf16 34.8 us, 37.9 with one for each four rows)
+  quantize_kernel<T, G, NV, SHORT><<<(unsigned)(need < 2048 ? need : 2048), kThreads, 0, s>>>(a);
 }
 
 template <typename T>

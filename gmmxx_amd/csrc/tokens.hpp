@@ -20,6 +20,7 @@ struct EmbedArgs {
   int32_t* pos[2];
   int32_t* hist;
   int32_t* totals;
+  uint8_t* seen;                         // [V] whether a token has a place
   float* part;
 };
 int64_t embed_workspace_bytes(int64_t N, int64_t V, int D);

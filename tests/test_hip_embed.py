@@ -166,3 +166,21 @@ def test_past_32_bits(hip):
     dtable, = torch.autograd.grad(gmmxx_amd.embed_rows(leaf, index), leaf, dy)
     rows = dtable.any(1).nonzero()[:, 0].tolist()
     assert rows == [0, v // 2, v - 2, v - 1] and torch.equal(dtable[rows], dy[:4])
+
+
+@pytest.mark.parametrize("v", [1, 3, 255, 511, 512, 1023, 2047, 2048, 4095, 65_535, 1 << 20, (1 << 21) - 1, (1 << 22) - 1, 1 << 22])
+@pytest.mark.parametrize("n", [4095, 4096, 4097, 33_000])
+def test_sorts(hip, n, v):
+    """Every width of the sort's digits, with one workgroup, few and many: whole numbers, exact in any order."""
+    print(f"[embed] sort n={n} v={v}", flush=True)
+    g = torch.Generator().manual_seed(v)
+    index = torch.floor((v + 1.0) ** torch.rand(n, generator=g, dtype=torch.float64) - 1.0).long().clamp_(0, v - 1)
+    index[::9] = torch.randint(0, v, (index[::9].numel(),), generator=g)
+    index[4::50] = v
+    index[5::50] = -7
+    index[-1] = v - 1
+    dy = torch.randint(-3, 4, (n, 4), generator=g).float()
+    leaf = torch.zeros((v, 4), device=DEV, requires_grad=True)
+    dtable, = torch.autograd.grad(gmmxx_amd.embed_rows(leaf, index.to(DEV)), leaf, dy.to(DEV))
+    there = (index >= 0) & (index < v)
+    assert torch.equal(dtable.cpu(), torch.zeros((v, 4)).index_add_(0, index[there], dy[there]))
