@@ -183,31 +183,32 @@ __device__ __forceinline__ Row resolved(Lean s) {
   return Row{m, lz + (float)(exact - (double)m), lz - s.u / (s.z * kLog2e)};
 }
 
-// A row by G lanes (or the workgroup's threads, G = kThreads) as Plain; of +inf each weighs 1.
+// Scores lo .. hi - 1 of a row (lo in whole vectors) by G lanes, or the workgroup's threads (G = kThreads), as Plain; of
+// +inf each weighs 1.
 template <typename T, int G, bool SHORT>
-__device__ __forceinline__ Row resolve_slowly(const LogpArgs& a, int64_t n, int lane, float (*red)[3]) {
+__device__ __forceinline__ Plain take_slowly(const LogpArgs& a, int64_t n, int lo, int hi, int lane, float (*red)[3]) {
   constexpr int V = kVec<T>, U = 8;    // vectors in flight
   const T* row = static_cast<const T*>(a.scores) + n * a.lds;
   Plain s;
   float infinite = 0.f;
-  for (int c0 = lane * V; c0 < a.V; c0 += G * V * U) {
+  for (int c0 = lo + lane * V; c0 < hi; c0 += G * V * U) {
     uint4 u[U];
 #pragma unroll
     for (int j = 0; j < U; ++j) {
       const int c = c0 + j * G * V;
-      u[j] = fetch16<SHORT>(row + (c < a.V ? c : 0), c < a.V ? a.V - c : a.V);
+      u[j] = fetch16<SHORT>(row + (c < hi ? c : 0), c < hi ? a.V - c : a.V);
     }
 #pragma unroll
     for (int j = 0; j < U; ++j) {
       const int c = c0 + j * G * V;
-      if (c >= a.V) break;
+      if (c >= hi) break;
       float v[V];
       unpack16<T>(keep16<SHORT, T>(u[j], a.V - c, a.V), v);
 #pragma unroll
       for (int i = 0; i < V; ++i) {
-        const bool inf = c + i < a.V && v[i] == INFINITY;
+        const bool inf = c + i < hi && v[i] == INFINITY;
         infinite += inf ? 1.f : 0.f;
-        v[i] = c + i < a.V && !inf ? v[i] : -INFINITY;
+        v[i] = c + i < hi && !inf ? v[i] : -INFINITY;
       }
       s.add(v);
     }
@@ -230,11 +231,13 @@ __device__ __forceinline__ Row resolve_slowly(const LogpArgs& a, int64_t n, int 
     s.ref = INFINITY;
     s.z = infinite;
   }
-  return resolved(s);
+  return s;
 }
+__device__ __forceinline__ bool only_low(Lean s) { return s.ref == -INFINITY && s.z > 0.f; }
+
 template <typename T, int G, bool SHORT>
 __device__ __forceinline__ Row resolve(const LogpArgs& a, int64_t n, int lane, float (*red)[3], Lean s) {
-  if (s.ref == INFINITY || (s.ref == -INFINITY && s.z > 0.f)) return resolve_slowly<T, G, SHORT>(a, n, lane, red);
+  if (s.ref == INFINITY || only_low(s)) return resolved(take_slowly<T, G, SHORT>(a, n, 0, a.V, lane, red));
   return s.ref == -INFINITY ? Row{-INFINITY, 0.f, 0.f} : resolved(s);
 }
 
@@ -358,21 +361,23 @@ __device__ __forceinline__ uint64_t cut(uint64_t* list, int count, int k, int* s
   return least;
 }
 
-// The k largest of the list in descending order to out[0 .. k - 1], zeros where there are fewer.
+// The k largest of the list in descending order to out[0 .. k - 1], zeros where there are fewer.  The list has room for
+// kAhead more.
+constexpr int kAhead = 16;
 template <int SIZE>
 __device__ __forceinline__ void sorted(uint64_t* list, int count, int k, int* scratch, uint64_t* out) {
   if (count > kThreads && count > k) {
     cut<SIZE>(list, count, k, scratch);
     count = k;
   }
+  if (threadIdx.x < kAhead) list[count + threadIdx.x] = 0;
   __syncthreads();
   if ((int)threadIdx.x < count) {
     const uint64_t mine = list[threadIdx.x];
-    int above = 0, i = 0;
-    for (; i + 16 <= count; i += 16)
+    int above = 0;
+    for (int i = 0; i < count; i += kAhead)
 #pragma unroll
-      for (int q = 0; q < 16; ++q) above += list[i + q] > mine;
-    for (; i < count; ++i) above += list[i] > mine;
+      for (int q = 0; q < kAhead; ++q) above += list[i + q] > mine;
     if (above < k) out[above] = mine;
   }
   if ((int)threadIdx.x >= count && (int)threadIdx.x < k) out[threadIdx.x] = 0;
@@ -433,11 +438,12 @@ struct Vectors {
 };
 
 // A part of a row (x) of each row (y), with k alternatives (or none); one part: the row's results.  The next
-// scores are in flight while those at hand are taken in.
+// scores are in flight while those at hand are taken in.  (Four waves a SIMD: the slow form's code would take registers
+// for two.)
 template <typename T, bool TOP, bool SHORT>
-__global__ __launch_bounds__(kThreads) void logp_part_kernel(LogpArgs a) {
+__global__ __launch_bounds__(kThreads, 4) void logp_part_kernel(LogpArgs a) {
   constexpr int V = kVec<T>, U = kTile / kThreads / V;
-  __shared__ uint64_t list[TOP ? kListSize : 1];
+  __shared__ __align__(16) uint64_t list[TOP ? kListSize + kAhead : 1];
   __shared__ uint64_t out[kLogpMaxK];
   __shared__ float red[kThreads / 64][3];
   __shared__ uint64_t ranks[TOP ? kThreads : 1];
@@ -533,6 +539,11 @@ __global__ __launch_bounds__(kThreads) void logp_part_kernel(LogpArgs a) {
     if constexpr (TOP) sorted<kListSize>(list, count, a.k, scratch, out);
     if (a.splits > 1) {
       const int64_t at = n * a.splits + split;
+      // (a part of low scores alone, as a fully masked row has them, is left as Plain, marked by a negative sum)
+      if (only_low(s)) {
+        const Plain low = take_slowly<T, kThreads, SHORT>(a, n, first, last, threadIdx.x, red);
+        s.ref = low.ref, s.z = -low.z, s.u = low.u;
+      }
       if (threadIdx.x == 0) a.part[at * 3] = s.ref, a.part[at * 3 + 1] = s.z, a.part[at * 3 + 2] = s.u;
       if (TOP && (int)threadIdx.x < a.k) a.part_top[at * a.k + threadIdx.x] = out[threadIdx.x];
     } else {
@@ -548,18 +559,24 @@ __global__ __launch_bounds__(kThreads) void logp_part_kernel(LogpArgs a) {
 constexpr int kMaxSplits = 64;
 template <typename T, bool TOP>
 __global__ __launch_bounds__(kThreads) void logp_join_kernel(LogpArgs a) {
-  __shared__ uint64_t list[TOP ? kMaxSplits * kLogpMaxK : 1];
+  __shared__ __align__(16) uint64_t list[TOP ? kMaxSplits * kLogpMaxK + kAhead : 1];
   __shared__ uint64_t out[kLogpMaxK];
   __shared__ float red[kThreads / 64][3];
   __shared__ int scratch[2 * kThreads / 64], count;
   __shared__ uint64_t lowest;
   for (int64_t n = blockIdx.x; n < a.N; n += gridDim.x) {
     Lean s;
+    Plain low;
     const uint64_t* p = a.part_top + n * a.splits * a.k;
     uint64_t bound = 1;
     if ((int)threadIdx.x < a.splits) {
       const float* q = a.part + (n * a.splits + threadIdx.x) * 3;
       s.ref = q[0], s.z = q[1], s.u = q[2];
+      if (s.z < 0.f) {
+        low.ref = s.ref, low.z = -s.z, low.u = s.u;
+        s = Lean();
+        s.z = 1.f;
+      }
       // every part's list is sorted: no score below a part's last is among the row's k best
       if (TOP) bound = max(bound, p[threadIdx.x * a.k + a.k - 1]);
     }
@@ -580,7 +597,13 @@ __global__ __launch_bounds__(kThreads) void logp_join_kernel(LogpArgs a) {
       if (threadIdx.x == 0) lowest = bound, count = 0;
     }
     s = block_merge(s, red);
-    const Row r = resolve<T, kThreads, false>(a, n, threadIdx.x, red, s);
+    Row r;
+    if (only_low(s)) {
+      __syncthreads();
+      r = resolved(block_merge(low, red));
+    } else {
+      r = resolve<T, kThreads, false>(a, n, threadIdx.x, red, s);
+    }
     if constexpr (TOP) {
       bound = lowest;
 #pragma unroll
