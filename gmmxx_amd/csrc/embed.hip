@@ -229,18 +229,22 @@ __global__ __launch_bounds__(kSortThreads) void sort_place_kernel(EmbedArgs a, i
   }
 }
 
-// The whole sort of up to kOneRows tokens by one workgroup in LDS, at most kOneBits a pass: a training step of few
-// tokens takes one launch for it where it took up to six (each several us of the host's time).
-constexpr int kOneRows = 4096, kOneThreads = 1024, kOneBits = 9;
-__global__ __launch_bounds__(kOneThreads) void sort_one_kernel(EmbedArgs a, int all, int bits) {
+// A part of `rows` tokens sorted by a workgroup in LDS, at most kOneBits a pass.  Up to kOneRows tokens are one part: a
+// training step of few tokens takes one launch for the sort where it took up to six (each several us of the
+// host's time).  Up to kMergeRows, parts of kPart tokens are sorted so and then merged: 4096, 16384 and 32768 tokens of 17
+// bits in 11, 16 and 22 us, where one workgroup takes 15 us for 4096 and digits over all of them 20, 22 and 27.
+constexpr int kOneRows = 2048, kOneThreads = 1024, kOneBits = 9;
+constexpr int kPart = 1024, kMergeRows = 32768;
+__global__ __launch_bounds__(kOneThreads) void sort_one_kernel(EmbedArgs a, int rows, int all, int bits) {
   constexpr int W = kOneThreads / 64, Bins = 1 << kOneBits;
   __shared__ uint32_t key[2][kOneRows];
   __shared__ uint16_t pos[2][kOneRows];
   __shared__ int next[W][Bins], wave_sum[Bins / 64];
-  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, N = (int)a.N;
+  const int base = blockIdx.x * rows, N = min((int)a.N - base, rows);
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
   const int per = (N + W * 64 - 1) / (W * 64) * 64, lo = min(w * per, N), hi = min(lo + per, N);
   for (int i = threadIdx.x; i < N; i += kOneThreads) {
-    key[0][i] = key_at(a, -1, i);
+    key[0][i] = key_at(a, -1, base + i);
     pos[0][i] = (uint16_t)i;
   }
   clear_seen(a, kOneThreads);
@@ -292,10 +296,61 @@ __global__ __launch_bounds__(kOneThreads) void sort_one_kernel(EmbedArgs a, int 
     __syncthreads();
   }
   for (int i = threadIdx.x; i < N; i += kOneThreads) {
-    a.key[0][i] = key[from][i];
-    a.pos[0][i] = pos[from][i];
-    if (key[from][i] < a.V) a.seen[key[from][i]] = 1;
+    a.key[0][base + i] = key[from][i];
+    a.pos[0][base + i] = base + pos[from][i];
+    if (gridDim.x == 1 && key[from][i] < a.V) a.seen[key[from][i]] = 1;
   }
+}
+
+// The sorted parts merged: a token's place is its own in its part and, of every other part, how many come before it
+// (equal ones too where the part does), which binary searches in all parts' tokens in LDS count, four at a time.
+__global__ __launch_bounds__(kThreads) void sort_merge_kernel(EmbedArgs a, int parts) {
+  extern __shared__ __align__(16) uint32_t part_keys[];
+  constexpr int L = kPart / 4 * 4 / kThreads;             // 16 bytes at a time, four parts' in flight
+  for (int t0 = 0; t0 < parts; t0 += 4) {
+    uint4 v[L];
+#pragma unroll
+    for (int j = 0; j < L; ++j) {
+      const int i = (t0 * (kPart / 4) + j * kThreads + (int)threadIdx.x) * 4;
+      v[j] = i < a.N ? *reinterpret_cast<const uint4*>(a.key[0] + i) : make_uint4(~0u, ~0u, ~0u, ~0u);   // (256 bytes)
+      if (i + 1 >= a.N) v[j].y = ~0u;
+      if (i + 2 >= a.N) v[j].z = ~0u;
+      if (i + 3 >= a.N) v[j].w = ~0u;
+    }
+#pragma unroll
+    for (int j = 0; j < L; ++j) {
+      const int i = t0 * (kPart / 4) + j * kThreads + threadIdx.x;
+      if (i < parts * (kPart / 4)) reinterpret_cast<uint4*>(part_keys)[i] = v[j];
+    }
+  }
+  __syncthreads();
+  const int i = blockIdx.x * kThreads + threadIdx.x, mine = i / kPart;
+  if (i >= a.N) return;
+  const uint32_t key = part_keys[i];
+  const int32_t pos = a.pos[0][i];
+  int place = i % kPart;
+  constexpr int U = 4;
+  for (int t0 = 0; t0 < parts; t0 += U) {
+    int at[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) at[u] = 0;
+#pragma unroll
+    for (int step = kPart / 2; step >= 1; step /= 2)
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int t = min(t0 + u, parts - 1);
+        at[u] += part_keys[t * kPart + at[u] + step - 1] < key + (t < mine) ? step : 0;
+      }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int t = min(t0 + u, parts - 1);
+      at[u] += part_keys[t * kPart + at[u]] < key + (t < mine);
+      place += t0 + u < parts && t != mine ? at[u] : 0;
+    }
+  }
+  a.key[1][place] = key;
+  a.pos[1][place] = pos;
+  if (key < a.V) a.seen[key] = 1;
 }
 
 // --- sums ---------------------------------------------------------------------
@@ -523,10 +578,15 @@ void launch_embed_bwd(const EmbedArgs& a, hipStream_t s) {
   const unsigned blocks = (unsigned)((a.N + rpb - 1) / rpb);
   const int all = key_bits(a.V), passes = (all + kMaxBits - 1) / kMaxBits, bits = (all + passes - 1) / passes;
   int from = -1;
+  const int one = (all + kOneBits - 1) / kOneBits, one_bits = (all + one - 1) / one;
   if (a.N <= kOneRows) {
-    const int one = (all + kOneBits - 1) / kOneBits;
-    sort_one_kernel<<<1, kOneThreads, 0, s>>>(a, all, (all + one - 1) / one);
+    sort_one_kernel<<<1, kOneThreads, 0, s>>>(a, kOneRows, all, one_bits);
     from = 0;
+  } else if (a.N <= kMergeRows && passes > 1) {
+    const int parts = (int)((a.N + kPart - 1) / kPart);
+    sort_one_kernel<<<parts, kOneThreads, 0, s>>>(a, kPart, all, one_bits);
+    sort_merge_kernel<<<(unsigned)((a.N + kThreads - 1) / kThreads), kThreads, parts * kPart * 4, s>>>(a, parts);
+    from = 1;
   } else {
     for (int p = 0; p < passes; ++p) {
       const int to = p & 1, bins = 1 << bits;

@@ -169,7 +169,7 @@ def test_past_32_bits(hip):
 
 
 @pytest.mark.parametrize("v", [1, 3, 255, 511, 512, 1023, 2047, 2048, 4095, 65_535, 1 << 20, (1 << 21) - 1, (1 << 22) - 1, 1 << 22])
-@pytest.mark.parametrize("n", [4095, 4096, 4097, 33_000])
+@pytest.mark.parametrize("n", [2047, 2048, 2049, 4097, 20_001, 32_768, 32_769, 34_000])
 def test_sorts(hip, n, v):
     """Every width of the sort's digits, with one workgroup, few and many: whole numbers, exact in any order."""
     print(f"[embed] sort n={n} v={v}", flush=True)
