@@ -14,7 +14,11 @@
 //
 // The sort takes the fewest passes of at most 11 bits; a pass counts digits by block,
 // turns the counts into prefixes over the blocks and places: waves rank 64 tokens at a
-// time by ballots over the digit's bits.
+// time by ballots over the digit's bits.  Few tokens are sorted by one workgroup, or in parts that are merged.
+//
+// 16384 tokens of 65536, 2048 columns bf16: lookup 25 us (rows written once, the frequent ones read from
+// caches: 87 MB at the least, 17 us); sort 15 us, sums 69 us (335 MB, 4.9 TB/s: bytes), parts of
+// runs 8 us.  100003 of 500, 100 columns fp32: 12; 15, 12 and 6 us: waits more than bytes.  One token is a launch: 2.5 us.
 
 #include <type_traits>
 

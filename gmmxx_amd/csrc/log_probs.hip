@@ -13,6 +13,10 @@
 // end, in a fixed order.  Rows are cut into parts where there are too few for the card, and joined by
 // a second kernel.
 //
+// 8192 x 65536 bf16: 250 us (1074 MB, 4.3 TB/s; part of it writes back what the gradient before left in
+// caches), the gradient 400 us (2147 MB, 5.4 TB/s): bytes.  100003 x 500 fp32: 43 and 73 us.  One row of 65536 with
+// 5 alternatives 8 + 4.5 us: the chains of a part and of the join; 130 rows of 32001 with 20, 14 + 5 us.
+//
 // Alternatives are found in the same pass.  A score's rank is a 64-bit number, its value
 // above its complemented index, so no two are equal and ties go to the lower index.  The
 // first scores give a bound that k of them reach; scores that reach the bound go to a list in LDS,

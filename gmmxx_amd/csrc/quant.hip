@@ -6,6 +6,10 @@
 // All in fp32, the sum in exact 32-bit integers (D <= 2^17).  A row of zeros has scale 0; a
 // row that holds a NaN or an infinity has scale NaN, so its products are NaN.  Where a is so
 // small that 127 / a would pass fp32, both are taken times 2^100 first, which is exact.
+//
+// 16384 x 4096 x 8192: 520 to 560 us a product (2.0 to 2.1 POP/s).  What the operands are made of sets the
+// clock: zeros take 357 us, and matrix instructions alone, from registers, give 4.9 POP/s on zeros and 3.5 on random
+// values.  The rows in 8 bits: 35 to 50 us (201 MB).  4 x 4096 x 8192 in one kernel: 9.7 us (33.7 MB, 3.5 TB/s).
 
 #include <math.h>
 
