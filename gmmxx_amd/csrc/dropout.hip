@@ -9,8 +9,8 @@
 // 16-bit types see one mask.  A dropped element is zero whatever x holds.
 //
 // A thread takes 16 bytes of x: one or two counters, whose words are all used.  Bound by bytes: 16384 x 4096
-// bf16 with a residual 71 us (403 MB, 5.7 TB/s), the gradient 55 us (268 MB, 4.9 TB/s); the ten rounds take about
-// 50 instructions for four elements, a third of what the card issues in that time.
+// bf16 with a residual 71 us (403 MB, 5.7 TB/s), the gradient 55 us (268 MB, 4.9 TB/s); eight elements take 195
+// instructions, most of them the rounds', somewhat more than half of what the card issues in that time.
 
 #include "rows.hpp"
 #include "tokens.hpp"
