@@ -423,10 +423,10 @@ int gmmxx_hip_log_probs_backward(int elem, int64_t N, int64_t V, int64_t k, cons
                                  void* stream);
 
 /* N rows of D <= 2^17 elements in 8 bits: with a the largest absolute value of a row,
- * values = round(x (127 / a)) (ties to even) and scales = a / 127, in fp32.  A row of zeros has
- * scale 0, a row with a NaN or an infinity scale NaN and values 0.  Rows of values lie ldv
- * apart, a multiple of 16 that is at least D, from a multiple of 16 on; zeros follow the
- * D values up to the next multiple of 16. */
+ * values = round(x (127 (1 / a))) (ties to even) and scales = a (1 / 127), each operation
+ * rounded to fp32.  A row of zeros has scale 0, a row with a NaN or an infinity scale NaN and
+ * values 0.  Rows of values lie ldv apart, a multiple of 16 that is at least D, from a multiple
+ * of 16 on; zeros follow the D values up to the next multiple of 16. */
 int gmmxx_hip_quantize(int elem, int64_t N, int64_t D, const void* x, int64_t ldx, int8_t* values, int64_t ldv,
                        float* scales, void* stream);
 

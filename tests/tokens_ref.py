@@ -154,9 +154,9 @@ def quantize(x):
     most = np.abs(x).max(1)
     lift = np.where(most < np.float32(2.0 ** -100), np.float32(2.0 ** 100), np.float32(1))
     with np.errstate(divide="ignore"):
-        by = np.where(most > 0, np.float32(127) / (most * lift), np.float32(0))
+        by = np.where(most > 0, np.float32(1) / (most * lift) * np.float32(127), np.float32(0))
     q = np.rint((x * lift[:, None]) * by[:, None])
-    scales = np.where(finite, most / np.float32(127), np.float32(math.nan))
+    scales = np.where(finite, most * (np.float32(1) / np.float32(127)), np.float32(math.nan))
     return torch.from_numpy(q.astype(np.int8)), torch.from_numpy(scales.astype(np.float32))
 
 
