@@ -178,13 +178,13 @@ struct Row { float m, logz, entropy; };
 __device__ __forceinline__ Row resolved(Plain s) {
   if (!(s.ref > -INFINITY)) return Row{-INFINITY, 0.f, 0.f};
   const float logz = logf(s.z);
-  return Row{s.ref, logz, logz - s.u / s.z};
+  return Row{s.ref, logz, fmaxf(logz - s.u / s.z, 0.f)};
 }
 // 2^ref = e^M exactly with M = ref / L: m is M in fp32, and what that rounds off goes to log Z.
 __device__ __forceinline__ Row resolved(Lean s) {
   const double exact = (double)s.ref / (double)kLog2e;
   const float m = (float)exact, lz = logf(s.z);
-  return Row{m, lz + (float)(exact - (double)m), lz - s.u / (s.z * kLog2e)};
+  return Row{m, lz + (float)(exact - (double)m), fmaxf(lz - s.u / (s.z * kLog2e), 0.f)};
 }
 
 // Scores lo .. hi - 1 of a row (lo in whole vectors) by G lanes, or the workgroup's threads (G = kThreads), as Plain; of
@@ -305,6 +305,115 @@ __device__ __forceinline__ float value_of(uint32_t key) {
 }
 __device__ __forceinline__ uint64_t rank_of(uint32_t key, int index) { return (uint64_t)key << 32 | (uint32_t)~index; }
 
+// Short rows: G lanes hold one, NV vectors of its scores each, as integers in their order (vector i of lane l holds the
+// scores from (i G + l) V on).  Each alternative is the largest left, then the lowest index that has it; where a wave
+// has few rows, a round passes over the vectors in which no row has its own.  33000 x 500 fp32 with 10 alternatives 45
+// us, 160000 x 100 with 5 34 us, 8000 x 2000 bf16 with 20 44 us; a workgroup for each row took 308, 1213 and 90.
+// Few rows with many alternatives wait for the rounds (4 x 2000, 20: 17 us) and take a workgroup each (9.6).
+constexpr int kShort = 2048;
+bool short_rows(int64_t N, int V, int k) { return V <= kShort && (V <= 256 || N > 512 || k <= 6); }
+template <int G, typename F>
+__device__ __forceinline__ uint32_t lanes_reduce_key(uint32_t v, F&& op) {
+  return __float_as_uint(lanes_reduce<G>(__uint_as_float(v), [&](float a, float b) {
+    return __uint_as_float(op(__float_as_uint(a), __float_as_uint(b)));
+  }));
+}
+template <typename T, int G, int NV, bool SHORT>
+__global__ __launch_bounds__(kThreads) void logp_rows_top_kernel(LogpArgs a) {
+  constexpr int V = kVec<T>, R = kThreads / G;
+  constexpr bool kSkip = G >= 16;
+  const auto larger = [](uint32_t p, uint32_t q) { return p > q ? p : q; };
+  const auto smaller = [](uint32_t p, uint32_t q) { return p < q ? p : q; };
+  const int lane = threadIdx.x % G;
+  for (int64_t n0 = (int64_t)blockIdx.x * R; n0 < a.N; n0 += (int64_t)gridDim.x * R) {   // (groups exchange together)
+    const bool there = n0 + threadIdx.x / G < a.N;
+    const int64_t n = there ? n0 + threadIdx.x / G : a.N - 1;
+    const T* row = static_cast<const T*>(a.scores) + n * a.lds;
+    uint4 u[NV];
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int c = (i * G + lane) * V;
+      u[i] = fetch16<SHORT>(row + (c < a.V ? c : 0), c < a.V ? a.V - c : a.V);
+    }
+    uint32_t v[NV][V], top[NV], best = 0;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int c = (i * G + lane) * V;
+      float s[V];
+      unpack16<T>(keep16<SHORT, T>(u[i], a.V - c, a.V), s);
+      top[i] = 0;
+#pragma unroll
+      for (int q = 0; q < V; ++q) {
+        v[i][q] = c + q < a.V ? key_of(s[q]) : 0;
+        top[i] = larger(top[i], v[i][q]);
+      }
+      best = larger(best, top[i]);
+    }
+    best = lanes_reduce_key<G>(best, larger);
+    const float m = best ? value_of(best) : -INFINITY;
+    Plain sums;
+    sums.ref = m;
+    if (fabsf(m) < INFINITY) {
+#pragma unroll
+      for (int i = 0; i < NV; ++i)
+#pragma unroll
+        for (int q = 0; q < V; ++q) {
+          float d = value_of(v[i][q]) - m;              // (no candidate: NaN)
+          const float e = exp_below(d);
+          sums.z += e;
+          sums.u = fmaf(e, d, sums.u);
+        }
+    } else {                                            // of +inf each weighs 1
+#pragma unroll
+      for (int i = 0; i < NV; ++i)
+#pragma unroll
+        for (int q = 0; q < V; ++q) sums.z += v[i][q] == best ? 1.f : 0.f;
+    }
+    sums.z = lanes_sum<G>(sums.z);
+    sums.u = lanes_sum<G>(sums.u);
+    const Row r = resolved(sums);
+    if (lane == 0 && there) finish<T>(a, n, r);
+    float value = 0.f;                                  // the alternative that this lane writes
+    int32_t index = 0;
+    int mine = 0;                                       // the last one, as this lane's score 0 would be 0
+    for (int j = 0; j < a.k; ++j) {
+      if (j > 0) {
+        best = 0;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+          if (!kSkip || __any((unsigned)(mine - i * G * V) < (unsigned)V)) {
+            top[i] = 0;
+#pragma unroll
+            for (int q = 0; q < V; ++q) {
+              v[i][q] = mine == i * G * V + q ? 0 : v[i][q];
+              top[i] = larger(top[i], v[i][q]);
+            }
+          }
+          best = larger(best, top[i]);
+        }
+        best = lanes_reduce_key<G>(best, larger);
+      }
+      uint32_t at = 0x7fffffff;
+#pragma unroll
+      for (int i = NV - 1; i >= 0; --i)
+        if (!kSkip || __any(top[i] == best)) {
+#pragma unroll
+          for (int q = V - 1; q >= 0; --q) at = v[i][q] == best ? i * G * V + q : at;
+        }
+      at = lanes_reduce_key<G>(at == 0x7fffffff ? at : at + lane * V, smaller);
+      mine = (int)at - lane * V;
+      if (lane == j % G) {
+        value = best ? log_p(value_of(best), r.m, r.logz) : -INFINITY;
+        index = best ? (int32_t)at : -1;
+      }
+      if ((j % G == G - 1 || j == a.k - 1) && lane <= j % G && there) {
+        a.top[n * a.k + j - j % G + lane] = value;
+        a.top_index[n * a.k + j - j % G + lane] = index;
+      }
+    }
+  }
+}
+
 constexpr int kTile = 4096;            // scores of a workgroup at a time
 constexpr int kListSize = 1024;
 
@@ -419,12 +528,12 @@ __device__ __forceinline__ uint64_t reached(uint64_t mine, int k, uint64_t* rank
 }
 
 // The scores of a row's part from c on, c + V G ..., U vectors of a thread.
-template <typename T, int U, bool SHORT>
+template <typename T, int U>
 struct Vectors {
   static constexpr int V = kVec<T>;
   uint4 u[U];
   // (a whole tile, as most are, takes no thought of the row's end: 9.3 instructions a score where it took 12.5)
-  static __device__ __forceinline__ bool whole(int base, int last) { return !SHORT && base + kThreads * V * U <= last; }
+  static __device__ __forceinline__ bool whole(int base, int last) { return base + kThreads * V * U <= last; }
   __device__ __forceinline__ void fetch(const T* row, int base, int last, int length) {
     if (whole(base, last)) {
 #pragma unroll
@@ -434,14 +543,14 @@ struct Vectors {
 #pragma unroll
     for (int j = 0; j < U; ++j) {
       const int c = base + (j * kThreads + (int)threadIdx.x) * V;
-      u[j] = fetch16<SHORT>(row + (c < last ? c : 0), c < last ? length - c : length);
+      u[j] = fetch16<false>(row + (c < last ? c : 0), c < last ? length - c : length);
     }
   }
   // -inf past the part.
   __device__ __forceinline__ void unpack(int j, int base, int last, int length, float (&v)[V]) const {
     if (whole(base, last)) return unpack16<T>(u[j], v);
     const int c = base + (j * kThreads + (int)threadIdx.x) * V;
-    unpack16<T>(keep16<SHORT, T>(u[j], c < last ? length - c : length, length), v);
+    unpack16<T>(keep16<false, T>(u[j], c < last ? length - c : length, length), v);
     if (c + V > last) {
 #pragma unroll
       for (int i = 0; i < V; ++i) v[i] = c + i < last ? v[i] : -INFINITY;
@@ -452,7 +561,7 @@ struct Vectors {
 // A part of a row (x) of each row (y), with k alternatives (or none); one part: the row's results.  The next
 // scores are in flight while those at hand are taken in.  (Four waves a SIMD: the slow form's code would take registers
 // for two.)
-template <typename T, bool TOP, bool SHORT>
+template <typename T, bool TOP>
 __global__ __launch_bounds__(kThreads, 4) void logp_part_kernel(LogpArgs a) {
   constexpr int V = kVec<T>, U = kTile / kThreads / V;
   __shared__ __align__(16) uint64_t list[TOP ? kListSize + kAhead : 1];
@@ -469,10 +578,10 @@ __global__ __launch_bounds__(kThreads, 4) void logp_part_kernel(LogpArgs a) {
     Lean s;
     uint64_t bound = 1;               // (0: no candidate)
     if (threadIdx.x == 0) count = 0;
-    Vectors<T, U, SHORT> next;
+    Vectors<T, U> next;
     next.fetch(row, first, last, a.V);
     for (int base = first; base < last; base += kTile) {
-      const Vectors<T, U, SHORT> now = next;
+      const Vectors<T, U> now = next;
       if (base + kTile < last) next.fetch(row, base + kTile, last, a.V);
       float v[U][V];
 #pragma unroll
@@ -553,13 +662,13 @@ __global__ __launch_bounds__(kThreads, 4) void logp_part_kernel(LogpArgs a) {
       const int64_t at = n * a.splits + split;
       // (a part of low scores alone, as a fully masked row has them, is left as Plain, marked by a negative sum)
       if (only_low(s)) {
-        const Plain low = take_slowly<T, kThreads, SHORT>(a, n, first, last, threadIdx.x, red);
+        const Plain low = take_slowly<T, kThreads, false>(a, n, first, last, threadIdx.x, red);
         s.ref = low.ref, s.z = -low.z, s.u = low.u;
       }
       if (threadIdx.x == 0) a.part[at * 3] = s.ref, a.part[at * 3 + 1] = s.z, a.part[at * 3 + 2] = s.u;
       if (TOP && (int)threadIdx.x < a.k) a.part_top[at * a.k + threadIdx.x] = out[threadIdx.x];
     } else {
-      const Row r = resolve<T, kThreads, SHORT>(a, n, threadIdx.x, red, s);
+      const Row r = resolve<T, kThreads, false>(a, n, threadIdx.x, red, s);
       if (threadIdx.x == 0) finish<T>(a, n, r);
       if constexpr (TOP) write_top(a, n, out, r);
     }
@@ -775,9 +884,27 @@ void rows_grouped(const LogpArgs& a, hipStream_t s) {
   logp_rows_kernel<T, G, SHORT><<<(unsigned)(need < kMaxBlocks ? need : kMaxBlocks), kThreads, 0, s>>>(a);
 }
 
+template <typename T, int G, int NV, bool SHORT>
+void rows_top(const LogpArgs& a, hipStream_t s) {
+  const int64_t need = (a.N + kThreads / G - 1) / (kThreads / G);
+  logp_rows_top_kernel<T, G, NV, SHORT><<<(unsigned)(need < kMaxBlocks ? need : kMaxBlocks), kThreads, 0, s>>>(a);
+}
+
 template <typename T>
 void logp_typed(const LogpArgs& a, hipStream_t s) {
-  if (a.k == 0 && a.V <= 2048) {
+  if (a.k > 0 && short_rows(a.N, a.V, a.k)) {
+    constexpr int N8 = 8 / kVec<T>;      // vectors of 8 scores
+    if (a.V < kVec<T>) rows_top<T, 4, N8, true>(a, s);
+    else if (a.V <= 32) rows_top<T, 4, N8, false>(a, s);
+    else if (a.V <= 64) rows_top<T, 4, 2 * N8, false>(a, s);
+    else if (a.V <= 128) rows_top<T, 8, 2 * N8, false>(a, s);
+    else if (a.V <= 256) rows_top<T, 8, 4 * N8, false>(a, s);
+    else if (a.V <= 512) rows_top<T, 16, 4 * N8, false>(a, s);
+    else if (a.V <= 1024) rows_top<T, 32, 4 * N8, false>(a, s);
+    else rows_top<T, 64, 4 * N8, false>(a, s);
+    return;
+  }
+  if (a.k == 0 && a.V <= kShort) {
     if (a.V < kVec<T>) rows_grouped<T, 4, true>(a, s);
     else if (a.V <= 128) rows_grouped<T, 4, false>(a, s);
     else if (a.V <= 512) rows_grouped<T, 16, false>(a, s);
@@ -785,9 +912,8 @@ void logp_typed(const LogpArgs& a, hipStream_t s) {
     return;
   }
   const dim3 grid((unsigned)a.splits, (unsigned)(a.N < 65535 ? a.N : 65535));
-  if (a.k == 0) logp_part_kernel<T, false, false><<<grid, kThreads, 0, s>>>(a);      // (V > 2048)
-  else if (a.V < kVec<T>) logp_part_kernel<T, true, true><<<grid, kThreads, 0, s>>>(a);
-  else logp_part_kernel<T, true, false><<<grid, kThreads, 0, s>>>(a);
+  if (a.k == 0) logp_part_kernel<T, false><<<grid, kThreads, 0, s>>>(a);             // (V > kShort)
+  else logp_part_kernel<T, true><<<grid, kThreads, 0, s>>>(a);                        // (V > 256)
   if (a.splits == 1) return;
   const unsigned rows = (unsigned)(a.N < kMaxBlocks ? a.N : kMaxBlocks);
   if (a.k == 0) logp_join_kernel<T, false><<<rows, kThreads, 0, s>>>(a);
@@ -820,7 +946,7 @@ int64_t align256(int64_t v) { return (v + 255) / 256 * 256; }
 
 // Parts of a row: none with enough rows for the card, else parts of 4096 scores or more.
 int logp_splits(int64_t N, int V, int k) {
-  if (k == 0 && V <= 2048) return 1;
+  if (V <= kShort) return 1;
   const int64_t blocks = k ? 512 : 1024;
   int64_t parts = (blocks + N - 1) / (N > 0 ? N : 1);
   const int64_t most = (V + 4095) / 4096;

@@ -235,3 +235,20 @@ def test_far_scores(hip, v, k, dtype):
     s[8], s[9, 5], s[10], s[11, 1::2] = big, -big, -big, -2.0 ** 100
     t[:] = torch.tensor([v // 3, 0, v // 2, v // 3, 1, v // 4, v // 4, 2, 3, 5, 0, 1], device=DEV)
     check(s, t, k)
+
+
+@pytest.mark.parametrize("dtype", (F32, F16), ids=str)
+@pytest.mark.parametrize("n", [300, 600])
+@pytest.mark.parametrize("v", [2, 5, 32, 33, 64, 65, 128, 129, 256, 257, 512, 513, 1024, 1025, 2048, 2049])
+def test_short_rows_with_alternatives(hip, n, v, dtype):
+    """Every group of lanes, more rows than a workgroup's, ties and masks among them."""
+    g = torch.Generator().manual_seed(v)
+    s = (torch.randint(-6, 7, (n, v), generator=g) / 2.0).to(dtype)
+    s[torch.rand((n, v), generator=g) < 0.3] = -INF
+    s[7], s[8] = -INF, torch.finfo(dtype).min
+    s[9, v // 2] = INF
+    s[10, ::2] = float("nan")
+    t = torch.randint(0, v, (n,), generator=g)
+    t[::13] = -1
+    for k in sorted({1, min(v, 7), min(v, 33), min(v, 64)}):
+        check(s.to(DEV), t.to(DEV), k)
