@@ -66,6 +66,24 @@ def test_counts(hip, n, v, k):
     check(*make(n, v, BF16, seed=n), k)
 
 
+@pytest.mark.parametrize("n", [4095, 4097])
+@pytest.mark.parametrize("v", [2049, 4099, 32768, 32769])
+@pytest.mark.parametrize("dtype", (F32, BF16), ids=str)
+def test_many_long_rows(hip, n, v, dtype):
+    """Both sides of the counts and lengths from which a wave takes a row; masked rows and far scores among them.
+    A lane adds 128 vectors of fp32 at most, 8 in a vector and 6 levels: 142 additions, the bound counts 154."""
+    print(f"[log_probs] n={n} v={v} {dtype}", flush=True)
+    s, t = make(61, v, dtype)
+    s, t = s.repeat(n // 61 + 1, 1)[:n], t.repeat(n // 61 + 1)[:n]
+    s[7], s[8], s[9] = -INF, torch.finfo(dtype).min, float("nan")
+    s[10, v - 1], s[11, :v - 1], s[12] = 2.0 ** 101, -INF, torch.finfo(dtype).max
+    got = gmmxx_amd.log_probs(s, t)
+    at = torch.cat([torch.arange(30), torch.arange(n - 30, n)]).to(DEV)
+    want = ref.log_probs(s[at], t[at])
+    experts_ref.close(got.chosen[at], *want["chosen"], "chosen")
+    experts_ref.close(got.entropy[at], *want["entropy"], "entropy")
+
+
 @pytest.mark.parametrize("v", [6, 700, 3000, 40_000])
 @pytest.mark.parametrize("k", [0, 4])
 @pytest.mark.parametrize("dtype", experts_ref.DTYPES, ids=str)
