@@ -20,6 +20,7 @@
 // caches: 87 MB at the least, 17 us); sort 15 us, sums 69 us (335 MB, 4.9 TB/s: bytes), parts of
 // runs 8 us.  100003 of 500, 100 columns fp32: 12; 15, 12 and 6 us: waits more than bytes.  One token is a launch: 2.5 us.
 
+#include <algorithm>
 #include <type_traits>
 
 #include "rows.hpp"
@@ -239,12 +240,15 @@ __global__ __launch_bounds__(kSortThreads) void sort_place_kernel(EmbedArgs a, i
 // bits in 11, 16 and 22 us, where one workgroup takes 15 us for 4096 and digits over all of them 20, 22 and 27.
 constexpr int kOneRows = 2048, kOneThreads = 1024, kOneBits = 9;
 constexpr int kPart = 1024, kMergeRows = 32768;
+// Rows whose marks few workgroups clear: of more, the sort by parts has workgroups that do nothing else (2000 tokens of
+// 2^24 rows 16 us against 119, 5000 of them 19 against 35, 1000 of a million 13 against 16).
+constexpr int kOneClear = 1 << 18;
 __global__ __launch_bounds__(kOneThreads) void sort_one_kernel(EmbedArgs a, int rows, int all, int bits) {
   constexpr int W = kOneThreads / 64, Bins = 1 << kOneBits;
   __shared__ uint32_t key[2][kOneRows];
   __shared__ uint16_t pos[2][kOneRows];
   __shared__ int next[W][Bins], wave_sum[Bins / 64];
-  const int base = blockIdx.x * rows, N = min((int)a.N - base, rows);
+  const int base = blockIdx.x * rows, N = max(min((int)a.N - base, rows), 0);   // (the last workgroups only clear)
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
   const int per = (N + W * 64 - 1) / (W * 64) * 64, lo = min(w * per, N), hi = min(lo + per, N);
   for (int i = threadIdx.x; i < N; i += kOneThreads) {
@@ -583,12 +587,13 @@ void launch_embed_bwd(const EmbedArgs& a, hipStream_t s) {
   const int all = key_bits(a.V), passes = (all + kMaxBits - 1) / kMaxBits, bits = (all + passes - 1) / passes;
   int from = -1;
   const int one = (all + kOneBits - 1) / kOneBits, one_bits = (all + one - 1) / one;
-  if (a.N <= kOneRows) {
+  if (a.N <= kOneRows && a.V <= kOneClear) {
     sort_one_kernel<<<1, kOneThreads, 0, s>>>(a, kOneRows, all, one_bits);
     from = 0;
   } else if (a.N <= kMergeRows && passes > 1) {
     const int parts = (int)((a.N + kPart - 1) / kPart);
-    sort_one_kernel<<<parts, kOneThreads, 0, s>>>(a, kPart, all, one_bits);
+    const int clear = (int)std::min<int64_t>(a.V / (kOneClear / 4), 256);
+    sort_one_kernel<<<std::max(parts, clear), kOneThreads, 0, s>>>(a, kPart, all, one_bits);
     sort_merge_kernel<<<(unsigned)((a.N + kThreads - 1) / kThreads), kThreads, parts * kPart * 4, s>>>(a, parts);
     from = 1;
   } else {

@@ -65,6 +65,14 @@ def test_tables(hip, v, kind):
     check(*make(3001, v, 12, F32, seed=v, kind=kind), scale=2.0)
 
 
+@pytest.mark.parametrize("v", [(1 << 18) - 1, 1 << 18, (1 << 18) + 1, 700_001])
+@pytest.mark.parametrize("n", [1, 1024, 1025, 2048, 2049])
+def test_few_tokens_of_large_tables(hip, n, v):
+    """Both sides of the size from which workgroups do nothing but clear marks."""
+    print(f"[embed] n={n} v={v}", flush=True)
+    check(*make(n, v, 5, F32, seed=n, kind="outside"))
+
+
 def test_largest_table(hip):
     """Tokens of 24 bits."""
     v = 1 << 24
