@@ -369,7 +369,7 @@ void tiled(const QuantMatmulArgs& a, hipStream_t s) {
 // --- products: few rows ------------------------------------------------------------
 
 // 16 NT columns a workgroup, by 16 x 16 x 64 MFMA with the matrix's rows first; its four waves take every fourth 64 of
-// the reduction, for MT tiles of 16 rows of x.
+// the reduction, for MT tiles of 16 rows of x (and the next 16 MT along y).
 constexpr int kFewRows = 32;
 
 // 16 bytes of the matrix's rows at reduction element k, zeros from K on.
@@ -407,14 +407,15 @@ __global__ __launch_bounds__(kThreads) void quant_few_kernel(QuantMatmulArgs a) 
   const int64_t f0 = (int64_t)blockIdx.x * (16 * NT);
   const int K = a.D, last = (K + 15) / 16 * 16 - 16;
   const int r = lane & 15, kc = (lane >> 4) * 16;
-  const int64_t row = 16 * (wave % MT) + r, col = f0 + 16 * (wave / MT % NT) + 4 * (lane >> 4);
+  const int64_t n0 = (int64_t)blockIdx.y * (16 * MT);
+  const int64_t row = n0 + 16 * (wave % MT) + r, col = f0 + 16 * (wave / MT % NT) + 4 * (lane >> 4);
   const Factors<O> factors(a, col);
   const float sx = a.xs[row < a.N ? row : a.N - 1];
   const int8_t *w[NT], *x[MT];
 #pragma unroll
   for (int n = 0; n < NT; ++n) w[n] = a.w + (f0 + 16 * n + r < a.F ? f0 + 16 * n + r : a.F - 1) * a.ldw;
 #pragma unroll
-  for (int m = 0; m < MT; ++m) x[m] = a.x + (16 * m + r < a.N ? 16 * m + r : a.N - 1) * a.ldx;
+  for (int m = 0; m < MT; ++m) x[m] = a.x + (n0 + 16 * m + r < a.N ? n0 + 16 * m + r : a.N - 1) * a.ldx;
   i32x4 acc[NT][MT] = {};
   for (int k0 = wave * 64; k0 < K; k0 += W * 64 * U) {
     i32x4 p[U][NT], q[U][MT];
@@ -555,10 +556,16 @@ void few_rows_out(const QuantArgs& x, const QuantMatmulArgs& a, int G, hipStream
 
 template <typename O>
 void matmul_typed(const QuantMatmulArgs& a, hipStream_t s) {
-  if (a.N <= kFewRows) {
+  // (Of more rows too, by groups of 32, where that gives no more workgroups than the card holds at once: their waves share
+  // the reduction, which a tile goes through alone.  64 x 8192 x 2048 14 us against 19 by tiles, 256 x 8000 x 100 14 against
+  // 18, 64 x 1024 x 2048 4.5 against 7; 128 x 8192 x 2048, twice as many, 25 against 19.)
+  const int64_t groups = (a.F + 15) / 16 * ((a.N + kFewRows - 1) / kFewRows);
+  if (a.N <= kFewRows || groups <= 256) {
     // 32 columns a workgroup halve what is read of x where there are enough of them: 32 x 4096 x 8192 11.2 and 14.8 us,
     // 32 x 1024 x 2048 5.2 and 4.5.
-    const auto grid = [&](int n) { return (unsigned)((a.F + 16 * n - 1) / (16 * n)); };
+    const auto grid = [&](int n) {
+      return dim3((unsigned)((a.F + 16 * n - 1) / (16 * n)), (unsigned)((a.N + kFewRows - 1) / kFewRows));
+    };
     if (a.N <= 16) quant_few_kernel<O, 1, 1><<<grid(1), kThreads, 0, s>>>(a);
     else if (a.F < 4096) quant_few_kernel<O, 2, 1><<<grid(1), kThreads, 0, s>>>(a);
     else quant_few_kernel<O, 2, 2><<<grid(2), kThreads, 0, s>>>(a);

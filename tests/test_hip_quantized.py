@@ -99,6 +99,31 @@ def test_columns(hip, n, f):
     check(n, 96, f, F16, bias=f % 2 == 0, seed=f)
 
 
+@pytest.mark.parametrize("n,f", [(40, 2100), (200, 1100)])
+@pytest.mark.parametrize("d", [1, 15, 16, 17, 64, 100, 127, 128, 129, 257, 383, 1000, 1025])
+def test_depths_of_tiles(hip, n, f, d):
+    """More groups of 32 rows and 16 columns than the card holds at once."""
+    print(f"[int8] n={n} d={d} f={f}", flush=True)
+    check(n, d, f, BF16, seed=d)
+
+
+@pytest.mark.parametrize("dtype", experts_ref.DTYPES, ids=str)
+@pytest.mark.parametrize("n", [33, 64, 65, 96, 1000, 4095, 8190, 8193])
+@pytest.mark.parametrize("f", [1, 16, 17])
+def test_groups_of_rows(hip, n, f, dtype):
+    """256 groups of 32 rows and 16 columns, one more, and fewer."""
+    print(f"[int8] n={n} f={f} {dtype}", flush=True)
+    check(n, 70, f, dtype, bias=n % 2 == 0, seed=n)
+
+
+def test_longest_sums_of_tiles(hip):
+    d = 131_072
+    x = Quantized(torch.full((200, d), 127, dtype=torch.int8, device=DEV), torch.ones(200, device=DEV))
+    w = Quantized(torch.full((1100, d), -127, dtype=torch.int8, device=DEV), torch.ones(1100, device=DEV))
+    # (-127^2 2^17 needs 14 bits: fp32 holds it)
+    assert (gmmxx_amd.quantized_matmul(x, w) == -127.0 ** 2 * d).all()
+
+
 @pytest.mark.parametrize("dtype", experts_ref.DTYPES, ids=str)
 @pytest.mark.parametrize("n,d,f", [(4096, 128, 4096), (4099, 300, 4100), (5000, 1000, 3500), (2048, 513, 16_384)])
 def test_large_tiles(hip, n, d, f, dtype):
@@ -171,6 +196,21 @@ def test_layouts_of_values(hip, n):
     rows = x[:1].expand(n, d)
     assert torch.equal(gmmxx_amd.quantized_matmul(Quantized(rows, sx[:1].expand(n)), Quantized(w, sw)),
                        want[:1].expand(n, 40))
+
+
+def test_layouts_of_values_in_tiles(hip):
+    n, d, f = 90, 75, 1600
+    x, w = whole(n, d), whole(f, d, seed=1)
+    sx, sw = rand(n, seed=2).abs(), rand(f, seed=3).abs()
+    want = gmmxx_amd.quantized_matmul(Quantized(x, sx), Quantized(w, sw))
+    experts_ref.close(want, *ref.quantized_matmul(x, sx, w, sw, None, F32), "contiguous")
+    for ld, first in ((80, 0), (128, 16), (77, 0), (96, 5)):
+        views = []
+        for t in (x, w):
+            room = torch.full((t.shape[0] * ld + first + 64,), 99, dtype=torch.int8, device=DEV)
+            views.append(room[first:first + t.shape[0] * ld].reshape(t.shape[0], ld)[:, :d])
+            views[-1].copy_(t)
+        assert torch.equal(gmmxx_amd.quantized_matmul(Quantized(views[0], sx), Quantized(views[1], sw)), want)
 
 
 def test_no_rows(hip):
