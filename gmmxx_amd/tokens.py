@@ -201,8 +201,9 @@ def quantize_rows(x: torch.Tensor) -> Quantized:
     """The rows of a matrix in 8 bits, with a scale each.
 
     With a the largest absolute value of a row: ``values = round(x * (127 * (1 / a)))`` (ties to
-    even), ``scales = a * (1 / 127)``, each operation rounded to float32.  ``x`` is (rows, D) with D <= 131072.  A row of zeros has
-    scale 0; a row with a NaN or an infinity has scale NaN, and so have its products.  For a product's
+    even), ``scales = a * (1 / 127)``, each operation rounded to float32.  ``x`` is (rows, D) with
+    D <= 131072.  A row of zeros has scale 0; a row with a NaN or an infinity has scale NaN, and so
+    have its products.  For a product's
     matrix, whose columns have the scales, take the rows of its transpose.  The rows of
     ``values`` are laid out in whole 128 bytes, as ``quantized_matmul`` reads them.  Has no gradient."""
     _quantizable(x, "x")
