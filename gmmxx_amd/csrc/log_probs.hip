@@ -79,9 +79,11 @@ struct Plain {
 
 // The same in half the instructions: sums of 2^l and 2^l l with l = s L - ref, L = log2(e) in fp32, where ref
 // need not be the largest s L, only near it.  Where a vector's sum passes 2^10, ref is raised to
-// its largest.  A ref that is not finite at the end (no score, or scores past 2^100) says that the row is to be
-// taken in as Plain.
-constexpr float kFar = 0x1p100f;
+// its largest, rounded: the largest score's own l is what the rounding left, at most 1/2 where |ref| < kNear, and 64
+// where |s| < kFar: 2^22 sums of 2^64 still fit.  Below -kFar scores that differ do so by 64 at least, so
+// what is no larger weighs nothing beside other scores and is left out.  A row whose ref ends past kNear, or that
+// holds only scores left out, is taken in as Plain (see slowly).
+constexpr float kNear = 0x1p24f, kFar = 0x1p30f;
 struct Lean {
   float ref = -INFINITY, z = 0.f, u = 0.f;
   __device__ __forceinline__ void raise(float to) {
@@ -238,10 +240,13 @@ __device__ __forceinline__ Plain take_slowly(const LogpArgs& a, int64_t n, int l
   return s;
 }
 __device__ __forceinline__ bool only_low(Lean s) { return s.ref == -INFINITY && s.z > 0.f; }
+__device__ __forceinline__ bool slowly(Lean s) {
+  return s.ref == -INFINITY ? s.z > 0.f : !(fabsf(s.ref) < kNear);
+}
 
 template <typename T, int G, bool SHORT>
 __device__ __forceinline__ Row resolve(const LogpArgs& a, int64_t n, int lane, float (*red)[3], Lean s) {
-  if (s.ref == INFINITY || only_low(s)) return resolved(take_slowly<T, G, SHORT>(a, n, 0, a.V, lane, red));
+  if (slowly(s)) return resolved(take_slowly<T, G, SHORT>(a, n, 0, a.V, lane, red));
   return s.ref == -INFINITY ? Row{-INFINITY, 0.f, 0.f} : resolved(s);
 }
 
@@ -828,7 +833,7 @@ __global__ __launch_bounds__(kThreads) void logp_bwd_kernel(LogpArgs a, int tx_,
     const Factors f = factors_of(a, r, dtop);
     const int t = a.dchosen ? (int)token_at(a, r) : -1;
     const float dc = t >= 0 ? a.dchosen[r] : 0.f;
-    const bool quick = fabsf(f.m) < kFar || f.m == -INFINITY;
+    const bool quick = fabsf(f.m) < 0x1p100f || f.m == -INFINITY;
     const Quick q(f);
     if (there) {
       for (int base = first; base < last; base += span) {

@@ -270,3 +270,47 @@ def test_short_rows_with_alternatives(hip, n, v, dtype):
     t[::13] = -1
     for k in sorted({1, min(v, 7), min(v, 33), min(v, 64)}):
         check(s.to(DEV), t.to(DEV), k)
+
+
+FAR = [-1e30, -1e20, -1e12, -1e10, -3e9, -1.2e9, -1e9, -5e8, -3.1e7, -1.5e7, 1.5e7, 3.1e7, 5e8, 1e9, 1.2e9, 3e9, 1e10, 1e12, 1e20,
+       1e30]
+
+
+def far_rows(v, dtype):
+    """For each far value rows of it alone, of numbers around it, of ordinary scores of which it takes the place of a third, or of
+    most of those in front, and a row of which it is the only candidate."""
+    g = torch.Generator().manual_seed(v)
+    rows = []
+    for x in FAR:
+        some = 3.0 * torch.randn((5, v), generator=g)
+        some[0] = x
+        some[1] = x + some[1] * abs(x) * 2.0 ** -23
+        some[2][torch.rand(v, generator=g) < 0.3] = x
+        some[3, :v - v // 4] = x
+        some[4], some[4, v // 2] = -INF, x
+        rows.append(some)
+    s = torch.cat(rows).to(dtype)
+    t = torch.randint(0, v, (s.shape[0],), generator=g)
+    t[4::5] = v // 2
+    return s.to(DEV), t.to(DEV)
+
+
+@pytest.mark.parametrize("v,k", [(3, 0), (9, 0), (9, 3), (100, 0), (600, 0), (600, 3), (600, 9), (2000, 0), (5000, 0), (5000, 3),
+                                 (40_000, 0), (40_000, 3)])
+@pytest.mark.parametrize("dtype", (F32, BF16), ids=str)
+def test_values_of_far_scores(hip, v, k, dtype):
+    """Scores of sizes at which log2(e) times them is rounded by more than exponents hold, as fill values often are."""
+    print(f"[log_probs] far values v={v} k={k} {dtype}", flush=True)
+    s, t = far_rows(v, dtype)
+    compare(gmmxx_amd.log_probs(s, t, top_k=k), ref.log_probs(s, t, k))
+
+
+@pytest.mark.parametrize("dtype", (F32, BF16), ids=str)
+def test_values_of_far_scores_in_many_rows(hip, dtype):
+    s, t = far_rows(2500, dtype)
+    n = s.shape[0]
+    got = gmmxx_amd.log_probs(s.repeat(42, 1), t.repeat(42))
+    want = ref.log_probs(s, t)
+    for part in (slice(0, n), slice(41 * n, 42 * n)):
+        experts_ref.close(got.chosen[part], *want["chosen"], "chosen")
+        experts_ref.close(got.entropy[part], *want["entropy"], "entropy")
