@@ -774,8 +774,8 @@ __device__ __forceinline__ float slope(const Factors& f, float s) {
   return s > -INFINITY ? p * fmaf(f.h, lp + f.entropy, f.c) : 0.f;
 }
 
-// The same in fewer instructions, where |m| < 2^100: with l = s L - k, L = log2(e) in fp32 and k = m L + log2 Z rounded
-// to fp32, p = 2^(l - off) by what k's rounding left, off, and so ds = 2^l (c' + h' l).
+// The same in fewer instructions, where |m| < kNear: with l = s L - k, L = log2(e) in fp32 and k = m L + log2 Z rounded
+// to fp32, p = 2^(l - off) by what k's rounding left, off (at most 2 there), and so ds = 2^l (c' + h' l).
 struct Quick {
   float k, c, h;
   __device__ __forceinline__ explicit Quick(const Factors& f) {
@@ -833,7 +833,7 @@ __global__ __launch_bounds__(kThreads) void logp_bwd_kernel(LogpArgs a, int tx_,
     const Factors f = factors_of(a, r, dtop);
     const int t = a.dchosen ? (int)token_at(a, r) : -1;
     const float dc = t >= 0 ? a.dchosen[r] : 0.f;
-    const bool quick = fabsf(f.m) < 0x1p100f || f.m == -INFINITY;
+    const bool quick = fabsf(f.m) < kNear || f.m == -INFINITY;
     const Quick q(f);
     if (there) {
       for (int base = first; base < last; base += span) {

@@ -314,3 +314,10 @@ def test_values_of_far_scores_in_many_rows(hip, dtype):
     for part in (slice(0, n), slice(41 * n, 42 * n)):
         experts_ref.close(got.chosen[part], *want["chosen"], "chosen")
         experts_ref.close(got.entropy[part], *want["entropy"], "entropy")
+
+
+@pytest.mark.parametrize("v,k", [(3, 0), (9, 0), (9, 3), (600, 0), (600, 3), (600, 9), (5000, 0), (5000, 3), (40_000, 0), (40_000, 3)])
+@pytest.mark.parametrize("dtype", (F32, BF16), ids=str)
+def test_gradients_of_far_scores(hip, v, k, dtype):
+    print(f"[log_probs] far gradients v={v} k={k} {dtype}", flush=True)
+    check(*far_rows(v, dtype), k)
