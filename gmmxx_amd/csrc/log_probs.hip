@@ -4,13 +4,15 @@
 // A row's candidates are its scores that are neither -inf nor NaN.  With m the largest,
 // d = s - m, Z = Σ e^d and U = Σ e^d d over the candidates:
 //   log p_t = d_t - log Z,   H = -Σ p log p = log Z - U / Z
-// (both terms of H are non-negative: nothing cancels).  Of several +inf each has
+// Both terms of H are non-negative then.  Sums beside a reference below m (see Lean) make log Z and -U / Z larger and
+// smaller by what it lacks, at most 2.1: of rows with p near 1, log p and H, near 0, are good to some 1e-7, not to
+// digits of their own (64 to 40000 normal scores and one with p = 0.98 or 0.9996: 3e-7 to 8e-7 at most).  Of several +inf each has
 // p = 1 / their number.  The gradient from g (chosen), h (entropy) and q (alternatives) is
 //   ds_j = g [j = t] + Σ_i q_i [j = top_i] - p_j (g + Σ_i q_i + h (log p_j + H)).
 //
-// One pass over the scores: a thread keeps its own sums beside a reference near its largest score, brought to a
-// larger one where that comes up (once a 16-byte vector at most), and the threads' are merged at the
-// end, in a fixed order.  Rows are cut into parts where there are too few for the card, and joined by
+// One pass over the scores: a thread keeps its own sums beside a reference, at first the largest of the first scores of
+// its wave (or group of lanes), brought to a larger one where scores pass it by much (once a 16-byte vector at most), and
+// the threads' are merged at the end, in a fixed order.  Rows are cut into parts where there are too few for the card, and joined by
 // a second kernel.
 //
 // 8192 x 65536 bf16: 235 us (1074 MB, 4.6 TB/s; part of it writes back what the gradient before left in
@@ -78,8 +80,8 @@ struct Plain {
 };
 
 // The same in half the instructions: sums of 2^l and 2^l l with l = s L - ref, L = log2(e) in fp32, where ref
-// need not be the largest s L, only near it.  Where a vector's sum passes 2^10, ref is raised to
-// its largest, rounded: the largest score's own l is what the rounding left, at most 1/2 where |ref| < kNear, and 64
+// need not be the largest s L, only near it.  Where a vector's sum passes the number of its scores, which one of 3.02 (fp32:
+// 2.02) above ref does, and none without one above it, ref is raised to its largest, rounded: the largest score's own l is what the rounding left, at most 1/2 where |ref| < kNear, and 64
 // where |s| < kFar: 2^22 sums of 2^64 still fit.  Below -kFar scores that differ do so by 64 at least, so
 // what is no larger weighs nothing beside other scores and is left out.  A row whose ref ends past kNear, or that
 // holds only scores left out, is taken in as Plain (see slowly).
@@ -93,6 +95,10 @@ struct Lean {
     u = f == 0.f ? 0.f : f * fmaf(z, by, u);
     z *= f;
     ref = to;
+  }
+  // `top`: the largest of some of the scores to come.
+  __device__ __forceinline__ void begin(float top) {
+    if (top > -kFar) ref = top < kFar ? top * kLog2e : INFINITY;
   }
   template <int V>
   __device__ __forceinline__ void sums(const float (&s)[V], float& zv, float& uv) const {
@@ -109,7 +115,7 @@ struct Lean {
   __device__ __forceinline__ void add(const float (&s)[V]) {
     float zv, uv;
     sums(s, zv, uv);
-    if (!(zv <= 1024.f)) {
+    if (!(zv <= 1.01f * V)) {                         // (1.01: what ref's rounding leaves of equal scores)
       float top = -INFINITY;
 #pragma unroll
       for (int i = 0; i < V; ++i) top = fmaxf(top, s[i]);
@@ -172,7 +178,7 @@ __device__ __forceinline__ int64_t token_at(const LogpArgs& a, int64_t n) {
 
 // log p of a score v: m and log Z need not be the largest score's, only belong together.
 __device__ __forceinline__ float log_p(float v, float m, float logz) {
-  return v > -INFINITY ? (v == m ? -logz : (v - m) - logz) : -INFINITY;
+  return v > -INFINITY ? fminf(v == m ? -logz : (v - m) - logz, 0.f) : -INFINITY;
 }
 
 struct Row { float m, logz, entropy; };
@@ -273,13 +279,24 @@ __global__ __launch_bounds__(kThreads) void logp_rows_kernel(LogpArgs a) {
   for (int64_t n = (int64_t)blockIdx.x * R + threadIdx.x / G; n < a.N; n += (int64_t)gridDim.x * R) {
     const T* row = static_cast<const T*>(a.scores) + n * a.lds;
     Lean s;
-    for (int c0 = lane * V; c0 < a.V; c0 += G * V * U) {
+#pragma unroll 1                       // (a first round of its own would take registers: 65536 x 4096 bf16 107 us)
+    for (int base = 0; base < a.V; base += G * V * U) {
+      const int c0 = base + lane * V;
       uint4 u[U];
 #pragma unroll
       for (int j = 0; j < U; ++j) {
         const int c = c0 + j * G * V;
         u[j] = fetch16<SHORT>(row + (c < a.V ? c : 0), c < a.V ? a.V - c : a.V);
       }
+      if constexpr (!SHORT)          // (what fetch16 gives are scores of the row, in place or not)
+        if (base == 0) {
+          // all lanes begin at the largest of their first scores, which few later ones pass by much
+          float v[V], top = -INFINITY;
+          unpack16<T>(u[0], v);
+#pragma unroll
+          for (int i = 0; i < V; ++i) top = fmaxf(top, v[i]);
+          s.begin(lanes_reduce<G>(top, [](float p, float q) { return fmaxf(p, q); }));
+        }
 #pragma unroll
       for (int j = 0; j < U; ++j) {
         const int c = c0 + j * G * V;
@@ -585,21 +602,24 @@ __global__ __launch_bounds__(kThreads, 4) void logp_part_kernel(LogpArgs a) {
     if (threadIdx.x == 0) count = 0;
     Vectors<T, U> next;
     next.fetch(row, first, last, a.V);
+#pragma unroll 1
     for (int base = first; base < last; base += kTile) {
       const Vectors<T, U> now = next;
       if (base + kTile < last) next.fetch(row, base + kTile, last, a.V);
-      float v[U][V];
+      float v[U][V], most = -INFINITY;        // (also where all of a thread's are NaN)
 #pragma unroll
-      for (int j = 0; j < U; ++j) {
-        now.unpack(j, base, last, a.V, v[j]);
-        s.add(v[j]);
-      }
-      if constexpr (TOP) {
-        float most = -INFINITY;        // (also where all of a thread's are NaN)
+      for (int j = 0; j < U; ++j) now.unpack(j, base, last, a.V, v[j]);
+      if (TOP || base == first) {
 #pragma unroll
         for (int j = 0; j < U; ++j)
 #pragma unroll
           for (int i = 0; i < V; ++i) most = fmaxf(most, v[j][i]);
+      }
+      // (a wave begins at the largest of its first scores, which few later ones pass by much)
+      if (base == first) s.begin(lanes_reduce<64>(most, [](float p, float q) { return fmaxf(p, q); }));
+#pragma unroll
+      for (int j = 0; j < U; ++j) s.add(v[j]);
+      if constexpr (TOP) {
         if (base == first) {
           int at = 0;                  // the first place of a thread's largest
 #pragma unroll

@@ -321,3 +321,36 @@ def test_values_of_far_scores_in_many_rows(hip, dtype):
 def test_gradients_of_far_scores(hip, v, k, dtype):
     print(f"[log_probs] far gradients v={v} k={k} {dtype}", flush=True)
     check(*far_rows(v, dtype), k)
+
+
+@pytest.mark.parametrize("n,v,lanes,k", [(2000, 64, 4, 0), (2000, 512, 16, 0), (2000, 2000, 64, 0), (4100, 4096, 256, 0),
+                                         (2000, 5000, 256, 0), (2000, 5000, 256, 1), (2000, 9000, 1024, 0), (2000, 9000, 1024, 1)])
+@pytest.mark.parametrize("dtype", (F32, BF16), ids=str)
+def test_confident_rows(hip, n, v, lanes, k, dtype):
+    """Two candidates, 3.1 to 9.8 powers of two apart, the likelier in a vector that the same lane takes later, p from 0.89
+    to 0.999.  The sums are beside the likelier then, whose 2^l is 1 within 2 U; the other's, at most 0.117, is good to 8 U,
+    and their sum is rounded by U: log Z is good to 4 U, and so is log p (of at most 0.12, which is rounded by less than U).
+    The entropy is log Z less a term of at most 0.25, whose own sum is good to 9 U of itself and whose divisor to 6 U: 4 U."""
+    step = lanes * (16 // dtype.itemsize)
+    g = torch.Generator().manual_seed(v)
+    low = 8.0 * torch.rand(n, generator=g) - 4.0
+    s = torch.full((n, v), -INF)
+    s[:, 1], s[:, step + 2] = low, low + 2.2 + 4.5 * torch.rand(n, generator=g)
+    s, t = s.to(dtype).to(DEV), torch.full((n,), step + 2, device=DEV)
+    got, want = gmmxx_amd.log_probs(s, t, top_k=k), ref.log_probs(s, t, k)
+    chosen, entropy = want["chosen"][0], want["entropy"][0]
+    u = experts_ref.U
+    experts_ref.close(got.chosen, chosen, torch.full_like(chosen, 5 * u), "chosen")
+    experts_ref.close(got.entropy, entropy, torch.full_like(entropy, 9 * u), "entropy")
+
+
+@pytest.mark.parametrize("v", [5, 64, 500, 2000, 5000, 40_000])
+@pytest.mark.parametrize("dtype", experts_ref.DTYPES, ids=str)
+def test_no_probability_past_one(hip, v, dtype):
+    n = 1000
+    s, t = make(n, v, dtype, spread=1.0)
+    t = t.clamp(min=0)
+    s.scatter_(1, t[:, None], 14.0 + 6.0 * torch.rand((n, 1), generator=torch.Generator().manual_seed(1)).to(dtype).to(DEV))
+    for k in (0, 2):
+        r = gmmxx_amd.log_probs(s, t, top_k=k)
+        assert (r.chosen <= 0).all() and (r.top <= 0).all() and (r.entropy >= 0).all()
