@@ -794,7 +794,7 @@ __device__ __forceinline__ float slope(const Factors& f, float s) {
   return s > -INFINITY ? p * fmaf(f.h, lp + f.entropy, f.c) : 0.f;
 }
 
-// The same in fewer instructions, where |m| < kNear: with l = s L - k, L = log2(e) in fp32 and k = m L + log2 Z rounded
+// The same in fewer instructions, where |m| < kNear and the row's gradients are finite: with l = s L - k, L = log2(e) in fp32 and k = m L + log2 Z rounded
 // to fp32, p = 2^(l - off) by what k's rounding left, off (at most 2 there), and so ds = 2^l (c' + h' l).
 struct Quick {
   float k, c, h;
@@ -810,6 +810,8 @@ struct Quick {
     c = fmaf(f.h, f.entropy - off * kLn2, f.c) * back;
     h = f.h * kLn2 * back;
   }
+  // (what is no candidate is multiplied by 2^-160, which is 0, and has no other look at it)
+  __device__ __forceinline__ bool finite() const { return fmaf(fabsf(h), 160.f, fabsf(c)) < INFINITY; }
   __device__ __forceinline__ float slope(float s) const {
     const float l = fmaxf(fmaf(s, kLog2e, -k), -160.f);
     return fast_exp2(l) * fmaf(h, l, c);
@@ -853,8 +855,8 @@ __global__ __launch_bounds__(kThreads) void logp_bwd_kernel(LogpArgs a, int tx_,
     const Factors f = factors_of(a, r, dtop);
     const int t = a.dchosen ? (int)token_at(a, r) : -1;
     const float dc = t >= 0 ? a.dchosen[r] : 0.f;
-    const bool quick = fabsf(f.m) < kNear || f.m == -INFINITY;
     const Quick q(f);
+    const bool quick = (fabsf(f.m) < kNear || f.m == -INFINITY) && q.finite();
     if (there) {
       for (int base = first; base < last; base += span) {
         uint4 u[U];

@@ -354,3 +354,33 @@ def test_no_probability_past_one(hip, v, dtype):
     for k in (0, 2):
         r = gmmxx_amd.log_probs(s, t, top_k=k)
         assert (r.chosen <= 0).all() and (r.top <= 0).all() and (r.entropy >= 0).all()
+
+
+@pytest.mark.parametrize("v,k", [(3, 0), (9, 0), (9, 3), (600, 0), (600, 3), (5000, 0), (5000, 3), (40_000, 0), (40_000, 3)])
+@pytest.mark.parametrize("dtype", experts_ref.DTYPES, ids=str)
+def test_gradients_that_are_not_finite(hip, v, k, dtype):
+    """They reach the row's candidates and nothing else."""
+    print(f"[log_probs] gradients not finite v={v} k={k} {dtype}", flush=True)
+    n, nan = 12, float("nan")
+    s, t = make(n, v, dtype)
+    g = torch.Generator().manual_seed(2)
+    s[torch.rand((n, v), generator=g).to(DEV) < 0.3] = -INF
+    s[torch.rand((n, v), generator=g).to(DEV) < 0.2] = nan
+    s[:, v // 2] = 1.0
+    s[9] = -INF
+    t[:] = v // 2
+    dc, dh, dt = (torch.randn(sh, generator=g) for sh in ((n,), (n,), (n, k)))
+    dc[0], dc[1], dc[2], dc[9] = nan, INF, -INF, nan
+    dh[3], dh[4], dh[5], dh[6] = nan, INF, -INF, 3e38
+    if k:
+        dt[7, 0], dt[8, 0] = nan, INF
+    leaf = s.detach().requires_grad_()
+    r = gmmxx_amd.log_probs(leaf, t, top_k=k)
+    some = 3 if k else 2
+    ds, = torch.autograd.grad((r.chosen, r.entropy, r.top)[:some], leaf, [x.to(DEV) for x in (dc, dh, dt)[:some]])
+    assert not ds[~(s > -INF)].any()
+    fine = [10, 11]
+    want = ref.log_probs(s[fine], t[fine], k, dc[fine], dh[fine], dt[fine] if k else None)
+    experts_ref.close(ds[fine], *want["dscores"], "dscores")
+    for row in range(6):
+        assert not torch.isfinite(ds[row, v // 2])
