@@ -3,7 +3,8 @@
 //   a = max |x|,  r = 127 (1 / a),  q = round(x r) (ties to even),  scale = a (1 / 127)
 //   out[n][f] = (Σ_d qx[n][d] qw[f][d]) xs[n] ws[f] + bias[f]
 //
-// All in fp32, each operation rounded, the sum in exact 32-bit integers (D <= 2^17).  A row of zeros has scale 0; a
+// All in fp32, each operation rounded, the sum in exact 32-bit integers (D <= 2^17).  The scales' product is formed
+// first; where it may pass fp32's range on either side (see usual), the result is formed in 64 bits and rounded.  A row of zeros has scale 0; a
 // row that holds a NaN or an infinity has scale NaN, so its products are NaN.  Where a is so
 // small that r would pass fp32, both are taken times 2^100 first, which is exact.
 //
@@ -126,6 +127,16 @@ void quantize_typed(const QuantArgs& a, hipStream_t s) {
   else if (nvec <= 512) quantize_shaped<T, 64, 8>(a, s);
   else if (nvec <= 2048) quantize_shaped<T, 256, 8>(a, s);
   else quantize_shaped<T, 256, 0>(a, s);
+}
+
+// --- a sum as a result -------------------------------------------------------------
+
+// Scales of 0, NaN or between 2^-60 and 2^60: the product of two such has fp32's precision, times a whole number too.
+__device__ __forceinline__ bool usual(float s) { return !(fabsf(s) > 0x1p60f) && !(s != 0.f && fabsf(s) < 0x1p-60f); }
+
+__device__ __forceinline__ float scaled(int sum, float x, float w, float b) { return (float)sum * (x * w) + b; }
+__device__ __forceinline__ float scaled_any(int sum, float x, float w, float b) {
+  return usual(x) && usual(w) ? scaled(sum, x, w, b) : (float)((double)sum * ((double)x * (double)w) + (double)b);
 }
 
 // --- products: tiles -------------------------------------------------------------
@@ -273,8 +284,8 @@ struct Tile {
 
 // A wave's results, 64 columns by 32 TQ rows, times the rows' and the columns' scales, as whole 128-byte lines: through the
 // wave's piece of LDS, from which 8 (16 for fp32) lanes take a row's 64 columns.  sw, bias and sx are the
-// columns' and rows' own, in LDS; `cols` and `rows` of them exist.
-template <typename O, int TQ>
+// columns' and rows' own, in LDS; `cols` and `rows` of them exist.  ANY: scales of any size.
+template <bool ANY, typename O, int TQ>
 __device__ __forceinline__ void store_products(uint8_t* piece, const i32x16 (&acc)[2][TQ], int lane, const float* sw,
                                                const float* bias, const float* sx, O* out, int64_t ld, int rows, int cols) {
   constexpr int Bytes = 64 * sizeof(O), Chunks = Bytes / 16;
@@ -294,7 +305,10 @@ __device__ __forceinline__ void store_products(uint8_t* piece, const i32x16 (&ac
           const float x = sx[32 * (j0 + j) + (lane & 31)];
           vec o;
 #pragma unroll
-          for (int c = 0; c < 4; ++c) o[c] = (O)((float)acc[i][j0 + j][4 * v + c] * (x * w[c]) + b[c]);
+          for (int c = 0; c < 4; ++c) {
+            const int sum = acc[i][j0 + j][4 * v + c];
+            o[c] = (O)(ANY ? scaled_any(sum, x, w[c], b[c]) : scaled(sum, x, w[c], b[c]));
+          }
           const int r = 32 * j + (lane & 31), byte = n * (int)sizeof(O);
           *reinterpret_cast<vec*>(piece + r * Bytes + (((byte >> 4) ^ (r & 7)) << 4) + (byte & 15)) = o;
         }
@@ -353,8 +367,11 @@ __global__ __launch_bounds__(64 * WP * WQ) void quant_tiles_kernel(QuantMatmulAr
     else fetch_direct(x, qoff[n - C::LP] + k, stage + BP * DEEP + (n - C::LP) * (C::Waves * 1024));
   };
   auto store = [&](uint8_t* piece) {
-    store_products<O>(piece, acc, lane, sw + wp, bias + wp, sx + wq,
-                      static_cast<O*>(a.out) + (q0 + wq) * a.F + p0 + wp, a.F, rows - wq, cols - wp);
+    O* out = static_cast<O*>(a.out) + (q0 + wq) * a.F + p0 + wp;
+    bool odd = !usual(sw[wp + lane]);                   // (64 columns and BQ / WQ rows are this wave's)
+    for (int r = lane; r < BQ / WQ; r += 64) odd |= !usual(sx[wq + r]);
+    if (__any(odd)) store_products<true>(piece, acc, lane, sw + wp, bias + wp, sx + wq, out, a.F, rows - wq, cols - wp);
+    else store_products<false>(piece, acc, lane, sw + wp, bias + wp, sx + wq, out, a.F, rows - wq, cols - wp);
   };
   C::run(K, load, wave, lane, acc, store);
 }
@@ -394,7 +411,7 @@ struct Factors {
     if (n >= a.N) return;
 #pragma unroll
     for (int c = 0; c < 4; ++c)
-      if (f0 + c < a.F) static_cast<O*>(a.out)[n * a.F + f0 + c] = (O)((float)t[c] * (sx * ws[c]) + b[c]);
+      if (f0 + c < a.F) static_cast<O*>(a.out)[n * a.F + f0 + c] = (O)scaled_any(t[c], sx, ws[c], b[c]);
   }
 };
 

@@ -13,7 +13,7 @@ the scores over the tokens that it answers with, and the large product of servin
 Every function runs on the caller's current stream, never synchronises, and is
 differentiable (once) by torch's autograd but for the 8-bit products, which are for serving.
 Elements are float32, bfloat16 or float16; sums and statistics are float32 (of 8-bit values:
-exact integers) and results are rounded once.  Results are the same from run to run.
+exact integers) and results are rounded to their type at the end.  Results are the same from run to run.
 Forward-mode derivatives, traces and tensors that hold no values of their own are refused
 with ``NotImplementedError``, as in ``gmmxx_amd.experts``.
 """
@@ -221,8 +221,10 @@ def quantized_matmul(x: Union[torch.Tensor, Quantized], weight: Quantized, bias:
     ``Quantized`` of (F, D), F <= 2^22, one row for each column of the result (``quantize_rows`` lays it
     out; values in rows that are not whole, aligned 16 bytes are copied at every call).
     ``bias`` is (F,) of the result's dtype, which is x's, float32 where x is ``Quantized``, or
-    ``dtype``.  Sums are exact; the result is rounded once.  Has no gradient: operands that
-    require one are refused outside ``torch.no_grad()``."""
+    ``dtype``.  Sums are exact.  Each is rounded to float32, so is the product of its two scales, so
+    is theirs with the bias added, and so to ``dtype`` is the result; with a scale below 2^-60 or above 2^60 in size
+    it is formed in 64 bits instead, so no size of the scales loses it.  Has no gradient:
+    operands that require one are refused outside ``torch.no_grad()``."""
     if not isinstance(weight, Quantized):
         raise TypeError("weight must be a Quantized (see quantize_rows)")
     if isinstance(x, Quantized):

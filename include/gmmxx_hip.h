@@ -431,7 +431,9 @@ int gmmxx_hip_quantize(int elem, int64_t N, int64_t D, const void* x, int64_t ld
                        float* scales, void* stream);
 
 /* out[n][f] = (sum over d of x[n][d] w[f][d]) xscales[n] wscales[f] + bias[f] (bias NULL: none;
- * of `elem`, as out).  The sum is exact.  Rows lie multiples of 16 bytes (at most 2^23) apart
+ * of `elem`, as out).  The sum is exact.  It is rounded to fp32, and so are the scales' product and theirs with
+ * the bias added; with a scale below 2^-60 or above 2^60 in size (0 apart) the result is formed in 64
+ * bits and then rounded to fp32.  Rows lie multiples of 16 bytes (at most 2^23) apart
  * from a multiple of 16 on, and may be read up to the next multiple of 16 after their D values,
  * whatever is there. */
 int gmmxx_hip_quantized_matmul(int elem, int64_t N, int64_t F, int64_t D, const int8_t* x, int64_t ldx,

@@ -274,3 +274,62 @@ def test_rows_of_zeros_and_not_finite(hip, n):
     wide = torch.zeros((n, 411), dtype=F16, device=DEV)
     wide[:, 7:307] = rand(n, 300, dtype=F16)
     assert torch.equal(gmmxx_amd.quantized_matmul(wide[:, 7:307], q), gmmxx_amd.quantized_matmul(rand(n, 300, dtype=F16), q))
+
+
+@pytest.mark.parametrize("dtype", experts_ref.DTYPES, ids=str)
+@pytest.mark.parametrize("n,f", [(5, 60), (60, 70), (90, 1600), (300, 4100)])
+def test_scales_whose_product_passes_fp32(hip, n, f, dtype):
+    """Scales of every size: what counts is the whole product.  Beside scales whose product has fp32's precision a result is
+    rounded three times before the bias (the sum, the scales' product, the product); the others are as good."""
+    print(f"[int8] scales n={n} f={f} {dtype}", flush=True)
+    x, w = whole(n, 96), whole(f, 96, seed=1)
+    x[::7], x[3::7] = 0, 1                        # sums of 0, of which a scale makes nothing else
+    sx, sw = rand(n, seed=2).abs() + 0.1, rand(f, seed=3).abs() + 0.1
+    for i, p in enumerate((100.0, -70.0, 40.0, -120.0, 120.0, -148.0, 124.0)):
+        sx[i % n::11] *= 2.0 ** p
+    for i, p in enumerate((-75.0, 40.0, -100.0, 120.0, 100.0, -20.0, -140.0)):
+        sw[i::13] *= 2.0 ** p
+    b = rand(f, seed=4, dtype=dtype)
+    for bias in (None, b):
+        y = gmmxx_amd.quantized_matmul(Quantized(x, sx), Quantized(w, sw), bias, dtype=dtype)
+        want, _ = ref.quantized_matmul(x, sx, w, sw, bias, dtype)
+        prod = (x.cpu().double() @ w.cpu().double().t()) * sx.cpu().double()[:, None] * sw.cpu().double()
+        bound = 3 * U * prod.abs() + U * want.abs() + 2.0 ** -149 + ref.rounded(dtype, want)
+        # (no result lies so near the border of infinity that fp32's error decides)
+        out = prod if bias is None else prod + bias.cpu().double()
+        border = torch.finfo(dtype).max * (1 + experts_ref.unit(dtype) / 2)
+        assert ((out.abs() / border - 1).abs() > 5 * U).all()
+        experts_ref.close(y, want, bound.nan_to_num(0.0, 0.0, 0.0), f"{n} x {f}")
+
+
+def test_scales_of_other_rows_change_nothing(hip):
+    """A row's results are those that it has alone beside scales of any size."""
+    for n, f in ((20, 60), (90, 1600)):
+        x, w = whole(n, 96), whole(f, 96, seed=1)
+        sx, sw = rand(n, seed=2).abs() + 0.1, rand(f, seed=3).abs() + 0.1
+        b = rand(f, seed=4)
+        want = gmmxx_amd.quantized_matmul(Quantized(x, sx), Quantized(w, sw), b)
+        sx[::3] *= 2.0 ** 100
+        sw[5::9] *= 2.0 ** -120
+        y = gmmxx_amd.quantized_matmul(Quantized(x, sx), Quantized(w, sw), b)
+        rows, cols = torch.arange(n) % 3 != 0, torch.arange(f) % 9 != 5
+        assert torch.equal(y.cpu()[rows][:, cols], want.cpu()[rows][:, cols])
+
+
+@pytest.mark.parametrize("n", [1, 30, 100])
+def test_rows_of_any_size(hip, n):
+    """Rows and matrices of small and of large numbers, brought into 8 bits on the way."""
+    x, w, b = rand(n, 300), rand(70, 300, seed=1), rand(70, seed=3)
+    x[::2] *= 2.0 ** 110
+    x[1::2] *= 2.0 ** -110
+    w[::2] *= 2.0 ** 30
+    w[1::2] *= 2.0 ** -60
+    x[n // 2] = 0.0
+    q = gmmxx_amd.quantize_rows(w)
+    qx, sx = ref.quantize(x)
+    want, _ = ref.quantized_matmul(qx, sx, q.values, q.scales, b, F32)
+    prod = (qx.double() @ q.values.cpu().double().t()) * sx.double()[:, None] * q.scales.cpu().double()
+    y = gmmxx_amd.quantized_matmul(x, q, b)
+    experts_ref.close(y, want, (3 * U * prod.abs() + U * want.abs() + 2.0 ** -149 + ref.rounded(F32, want)).nan_to_num(0.0, 0.0, 0.0),
+                      "rows")
+    assert torch.equal(y[n // 2], b)
