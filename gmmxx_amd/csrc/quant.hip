@@ -3,7 +3,8 @@
 //   a = max |x|,  r = 127 (1 / a),  q = round(x r) (ties to even),  scale = a (1 / 127)
 //   out[n][f] = (Σ_d qx[n][d] qw[f][d]) xs[n] ws[f] + bias[f]
 //
-// All in fp32, each operation rounded, the sum in exact 32-bit integers (D <= 2^17).  The scales' product is formed
+// All in fp32, each operation rounded, the sum in exact 32-bit integers (D <= 2^17; the one sum that passes them, 2^31, is
+// told from the others, see kPast).  The scales' product is formed
 // first; where it may pass fp32's range on either side (see usual), the result is formed in 64 bits and rounded.  A row of zeros has scale 0; a
 // row that holds a NaN or an infinity has scale NaN, so its products are NaN.  Where a is so
 // small that r would pass fp32, both are taken times 2^100 first, which is exact.
@@ -134,9 +135,16 @@ void quantize_typed(const QuantArgs& a, hipStream_t s) {
 // Scales of 0, NaN or between 2^-60 and 2^60: the product of two such has fp32's precision, times a whole number too.
 __device__ __forceinline__ bool usual(float s) { return !(fabsf(s) > 0x1p60f) && !(s != 0.f && fabsf(s) < 0x1p-60f); }
 
+// The 32 bits of -2^31 are a sum of 2^31: of 2^17 products all of (-128)^2; no sum is below -2^17 128 127.
+constexpr int kPast = -0x7fffffff - 1;
+typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+__device__ __forceinline__ i32x4 added(i32x4 a, i32x4 b) { return (i32x4)((u32x4)a + (u32x4)b); }   // (past 2^31 too)
+__device__ __forceinline__ bool may_pass(int D) { return D == kQuantMaxD; }
+
 __device__ __forceinline__ float scaled(int sum, float x, float w, float b) { return (float)sum * (x * w) + b; }
 __device__ __forceinline__ float scaled_any(int sum, float x, float w, float b) {
-  return usual(x) && usual(w) ? scaled(sum, x, w, b) : (float)((double)sum * ((double)x * (double)w) + (double)b);
+  if (!usual(x) || !usual(w)) return (float)((sum == kPast ? 0x1p31 : (double)sum) * ((double)x * (double)w) + (double)b);
+  return sum == kPast ? 0x1p31f * (x * w) + b : scaled(sum, x, w, b);
 }
 
 // --- products: tiles -------------------------------------------------------------
@@ -284,7 +292,7 @@ struct Tile {
 
 // A wave's results, 64 columns by 32 TQ rows, times the rows' and the columns' scales, as whole 128-byte lines: through the
 // wave's piece of LDS, from which 8 (16 for fp32) lanes take a row's 64 columns.  sw, bias and sx are the
-// columns' and rows' own, in LDS; `cols` and `rows` of them exist.  ANY: scales of any size.
+// columns' and rows' own, in LDS; `cols` and `rows` of them exist.  ANY: scales and sums of any size.
 template <bool ANY, typename O, int TQ>
 __device__ __forceinline__ void store_products(uint8_t* piece, const i32x16 (&acc)[2][TQ], int lane, const float* sw,
                                                const float* bias, const float* sx, O* out, int64_t ld, int rows, int cols) {
@@ -368,7 +376,7 @@ __global__ __launch_bounds__(64 * WP * WQ) void quant_tiles_kernel(QuantMatmulAr
   };
   auto store = [&](uint8_t* piece) {
     O* out = static_cast<O*>(a.out) + (q0 + wq) * a.F + p0 + wp;
-    bool odd = !usual(sw[wp + lane]);                   // (64 columns and BQ / WQ rows are this wave's)
+    bool odd = may_pass(K) || !usual(sw[wp + lane]);    // (64 columns and BQ / WQ rows are this wave's)
     for (int r = lane; r < BQ / WQ; r += 64) odd |= !usual(sx[wq + r]);
     if (__any(odd)) store_products<true>(piece, acc, lane, sw + wp, bias + wp, sx + wq, out, a.F, rows - wq, cols - wp);
     else store_products<false>(piece, acc, lane, sw + wp, bias + wp, sx + wq, out, a.F, rows - wq, cols - wp);
@@ -465,7 +473,7 @@ __global__ __launch_bounds__(kThreads) void quant_few_kernel(QuantMatmulArgs a) 
   if (wave < NT * MT) {
     i32x4 t = sums[0][wave][lane];
 #pragma unroll
-    for (int q = 1; q < W; ++q) t += sums[q][wave][lane];
+    for (int q = 1; q < W; ++q) t = added(t, sums[q][wave][lane]);
     factors.store(a, t, sx, row, col);
   }
 }
@@ -543,7 +551,7 @@ __global__ __launch_bounds__(kThreads) void quant_few_rows_kernel(QuantArgs x, Q
   __syncthreads();
   if (wave == 0) {
 #pragma unroll
-    for (int i = 1; i < W; ++i) acc += sums[i][lane];
+    for (int i = 1; i < W; ++i) acc = added(acc, sums[i][lane]);
     factors.store(a, acc, sx, r, col);
   }
 }

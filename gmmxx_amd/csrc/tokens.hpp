@@ -66,7 +66,7 @@ int64_t logp_top_offset(int64_t N, int splits);      // of `part_top` in the wor
 void launch_logp(const LogpArgs& a, hipStream_t s);
 void launch_logp_bwd(const LogpArgs& a, hipStream_t s);
 
-constexpr int kQuantMaxD = 1 << 17;      // the sum of D products of two values up to 127 fits 32 bits
+constexpr int kQuantMaxD = 1 << 17;      // sums of D products of two values from -128 to 127 lie above -2^31 and up to 2^31
 constexpr int kQuantPad = 128;           // rows of 8-bit values are padded to whole cache lines
 struct QuantArgs {
   const void* x; int64_t ldx;            // N rows of D elements

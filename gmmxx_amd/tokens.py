@@ -29,7 +29,7 @@ from .experts import _ELEMS, _MAX_POSITIONS, MAX_WIDTH, _failed, _native, _opera
 MAX_TOKENS = 1 << 24        # rows of an embedding's table
 MAX_SCORES = 1 << 22        # scores in a row
 MAX_ALTERNATIVES = 64
-MAX_QUANTIZED = 1 << 17     # the longest sum of 8-bit products that 32 bits hold
+MAX_QUANTIZED = 1 << 17     # the longest sum of 8-bit products that 32 bits tell from every other
 _FP32_MAX = torch.finfo(torch.float32).max
 
 

@@ -333,3 +333,19 @@ def test_rows_of_any_size(hip, n):
     experts_ref.close(y, want, (3 * U * prod.abs() + U * want.abs() + 2.0 ** -149 + ref.rounded(F32, want)).nan_to_num(0.0, 0.0, 0.0),
                       "rows")
     assert torch.equal(y[n // 2], b)
+
+
+@pytest.mark.parametrize("n,f", [(1, 20), (30, 20), (200, 20), (20, 4100), (200, 1100), (300, 9000)])
+@pytest.mark.parametrize("d", [131_072, 131_071])
+def test_longest_sums_of_the_lowest_value(hip, n, d, f):
+    """-128 on both sides, as a user's values may have it: a sum of 2^31 at the longest."""
+    print(f"[int8] -128 n={n} d={d} f={f}", flush=True)
+    x = Quantized(torch.full((n, d), -128, dtype=torch.int8, device=DEV), torch.ones(n, device=DEV))
+    w = torch.full((f, d), -128, dtype=torch.int8, device=DEV)
+    w[1::2] = 127
+    b = torch.full((f,), 5.0, device=DEV)
+    y = gmmxx_amd.quantized_matmul(x, Quantized(w, torch.full((f,), 0.5, device=DEV)), b)
+    # (the sum, its product and the sum with the bias are rounded)
+    want = torch.tensor([8192.0 * d, -8128.0 * d], dtype=torch.float64) + 5.0
+    for i in range(2):
+        assert ((y[:, i::2].double() - want[i]).abs() <= 3 * U * want[i].abs()).all()
