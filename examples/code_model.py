@@ -34,7 +34,6 @@ class CodeModel(torch.nn.Module):
         self.maps = weight(experts, width, width, scale=width ** -0.5)
         self.head = weight(tokens, width, scale=width ** -0.5)
         self.steps = torch.zeros(1, dtype=torch.int64, device=device)       # the dropout's seed
-        self.served = None
 
     def hidden(self, tokens):
         h = gmmxx_amd.embed_rows(self.table, tokens, scale=self.scale)
@@ -53,11 +52,15 @@ class CodeModel(torch.nn.Module):
         return -(p.chosen.sum() + entropy * p.entropy.sum()) / counted
 
     @torch.no_grad()
-    def answer(self, tokens, top_k=3):
-        """The likeliest next tokens and their log probabilities."""
-        if self.served is None:
-            self.served = gmmxx_amd.quantize_rows(self.head)
-        scores = gmmxx_amd.quantized_matmul(self.hidden(tokens), self.served)
+    def quantized_head(self):
+        """The head as it is now, for ``answer``."""
+        return gmmxx_amd.quantize_rows(self.head)
+
+    @torch.no_grad()
+    def answer(self, tokens, top_k=3, head=None):
+        """The likeliest next tokens and their log probabilities.  ``head``: a trained model's ``quantized_head()``,
+        made once for many answers; without it the head is brought into 8 bits here."""
+        scores = gmmxx_amd.quantized_matmul(self.hidden(tokens), self.quantized_head() if head is None else head)
         return gmmxx_amd.log_probs(scores, torch.full_like(tokens, -1), top_k=top_k)
 
 
@@ -95,7 +98,8 @@ def run(rows=20_000, clusters=20, steps=150, dtype=torch.bfloat16, device="cuda:
 def main():
     losses, model, codes = run()
     print(f"loss {losses[0]:.3f} -> {losses[-1]:.3f} in {len(losses)} steps")
-    answer = model.answer(codes[:1])
+    head = model.quantized_head()
+    answer = model.answer(codes[:1], head=head)
     print(f"after {int(codes[0])}:", ", ".join(f"{int(t)} ({float(p):.2f})" for t, p in
                                                zip(answer.top_index[0], answer.top[0])))
 

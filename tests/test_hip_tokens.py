@@ -190,3 +190,22 @@ def test_example(hip):
     assert one.top.shape == (1, 3) and many.top_index.shape == (40, 3)
     assert ((many.top_index >= 0) & (many.top_index < 9)).all() and not many.chosen.any()
     assert (many.top[:, :-1] >= many.top[:, 1:]).all()
+
+
+def test_example_answers_with_its_present_head(hip):
+    path = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "examples")
+    sys.path.insert(0, path)
+    try:
+        import code_model
+    finally:
+        sys.path.remove(path)
+    _, model, codes = code_model.run(rows=2000, clusters=9, steps=2)
+    before = model.answer(codes[:50])
+    with torch.no_grad():
+        model.head.copy_(model.head.flip(0))                 # as training further or loading does
+    after = model.answer(codes[:50])
+    # (the same scores at the mirrored tokens; their probabilities' sum is added in another order)
+    assert torch.equal(after.top_index, 8 - before.top_index)
+    head = model.quantized_head()
+    given = model.answer(codes[:50], head=head)
+    assert all(torch.equal(a, b) for a, b in zip(given, after))
