@@ -15,9 +15,10 @@
 // the threads' are merged at the end, in a fixed order.  Rows are cut into parts where there are too few for the card, and joined by
 // a second kernel.
 //
-// 8192 x 65536 bf16: 235 us (1074 MB, 4.6 TB/s; part of it writes back what the gradient before left in
-// caches), the gradient 400 us (2147 MB, 5.4 TB/s): bytes.  100003 x 500 fp32: 43 and 73 us.  One row of 65536 with
-// 5 alternatives 8 + 4.5 us: the chains of a part and of the join; 130 rows of 32001 with 20, 14 + 5 us.
+// 8192 x 65536 bf16: 185 us call after call (1074 MB, 5.8 TB/s, some of it from caches), 228 behind a gradient whose writes
+// are still in the caches, and the gradient 396 us (2147 MB, 5.4 TB/s): bytes.  100003 x 500 fp32: 44 and 73 us.  One row
+// of 65536 with 5 alternatives 8.5 + 4.5 us: the chains of a part and of the join; 130 rows of 32001 with 20, 15 + 5
+// us, 21 + 5 with rows of the type's lowest value alone, which are read twice.
 //
 // Alternatives are found in the same pass.  A score's rank is a 64-bit number, its value
 // above its complemented index, so no two are equal and ties go to the lower index.  The
@@ -912,9 +913,15 @@ void rows_grouped(const LogpArgs& a, hipStream_t s) {
 }
 
 // Without alternatives a wave takes a whole row also where rows enough fill the card: it waits for no other and has no
-// barrier.  65536 x 4096 bf16 90 us against a workgroup's 225, 30000 x 3001 fp32 61 against 119, 4096 x 4096 bf16 10.8
-// against 15.9, 10000 x 32001 bf16 117 against 132; at 8192 x 65536 a workgroup is ahead, 185 against 212.
-bool rows_by_wave(int64_t N, int V) { return V <= kShort || (V <= 32768 && N >= 4096); }
+// barrier.  us a call by waves and by workgroups, for 128, 1000, 2500, 4096 and 10000 rows of V scores:
+//    3001 bf16  7.4  7.7   7.6  7.8   7.7 10.8    8.3 15.7   16  34      fp32  7.4  7.3   7.7  7.6   8.4 11.9    11  17   22  37
+//    9001       9.8 10.0   9.3 14.1  14.0 16.6   17   24     33  50           13   10    14   16    19   21      26  30   65  72
+//   12288      12   10    11   14    17   16     20   22     41  45           17   10    17   18    23   22      33  32   89  81
+//   32001      22   10    25   20    37   31     46   46    120 133           35   10    39   27    58   52      93  92  222 210
+//   32768      22   10    25   19    37   30     52   44    131 114           34   10    39   26    65   55     101  94  238 215
+// At 8192 x 65536 bf16 a workgroup is ahead, 185 against 212.  The type has no part in the rule, since the
+// workspace's size, which callers ask for without one, goes by it too.
+bool rows_by_wave(int64_t N, int V) { return V <= kShort || (V <= 9216 && N >= 1000) || (V <= 32768 && N >= 4096); }
 
 template <typename T, int G, int NV, bool SHORT>
 void rows_top(const LogpArgs& a, hipStream_t s) {

@@ -384,3 +384,20 @@ def test_gradients_that_are_not_finite(hip, v, k, dtype):
     experts_ref.close(ds[fine], *want["dscores"], "dscores")
     for row in range(6):
         assert not torch.isfinite(ds[row, v // 2])
+
+
+@pytest.mark.parametrize("n", [999, 1000])
+@pytest.mark.parametrize("v", [2049, 9216, 9217])
+@pytest.mark.parametrize("dtype", (F32, BF16), ids=str)
+def test_long_rows_by_count(hip, n, v, dtype):
+    """Both sides of the count from which a wave takes a row of these lengths."""
+    print(f"[log_probs] n={n} v={v} {dtype}", flush=True)
+    s, t = make(43, v, dtype)
+    s, t = s.repeat(n // 43 + 1, 1)[:n], t.repeat(n // 43 + 1)[:n]
+    s[7], s[8], s[9] = -INF, torch.finfo(dtype).min, float("nan")
+    s[10, v - 1], s[11, :v - 1], s[12] = 3e12, -INF, -1e10
+    got = gmmxx_amd.log_probs(s, t)
+    at = torch.cat([torch.arange(20), torch.arange(n - 20, n)]).to(DEV)
+    want = ref.log_probs(s[at], t[at])
+    experts_ref.close(got.chosen[at], *want["chosen"], "chosen")
+    experts_ref.close(got.entropy[at], *want["entropy"], "entropy")
