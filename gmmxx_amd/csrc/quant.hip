@@ -133,7 +133,10 @@ void quantize_typed(const QuantArgs& a, hipStream_t s) {
 // --- a sum as a result -------------------------------------------------------------
 
 // Scales of 0, NaN or between 2^-60 and 2^60: the product of two such has fp32's precision, times a whole number too.
-__device__ __forceinline__ bool usual(float s) { return !(fabsf(s) > 0x1p60f) && !(s != 0.f && fabsf(s) < 0x1p-60f); }
+// (& and |: without branches, 4 x 4096 x 8192 11.3 us a call, with them 11.5)
+__device__ __forceinline__ bool usual(float s) {
+  return !(fabsf(s) > 0x1p60f) & !((s != 0.f) & (fabsf(s) < 0x1p-60f));
+}
 
 // The 32 bits of -2^31 are a sum of 2^31: of 2^17 products all of (-128)^2; no sum is below -2^17 128 127.
 constexpr int kPast = -0x7fffffff - 1;
@@ -376,9 +379,9 @@ __global__ __launch_bounds__(64 * WP * WQ) void quant_tiles_kernel(QuantMatmulAr
   };
   auto store = [&](uint8_t* piece) {
     O* out = static_cast<O*>(a.out) + (q0 + wq) * a.F + p0 + wp;
-    bool odd = may_pass(K) || !usual(sw[wp + lane]);    // (64 columns and BQ / WQ rows are this wave's)
+    bool odd = may_pass(K) | !usual(sw[wp + lane]);     // (64 columns and BQ / WQ rows are this wave's)
     for (int r = lane; r < BQ / WQ; r += 64) odd |= !usual(sx[wq + r]);
-    if (__any(odd)) store_products<true>(piece, acc, lane, sw + wp, bias + wp, sx + wq, out, a.F, rows - wq, cols - wp);
+    if (__builtin_expect(__any(odd), 0)) store_products<true>(piece, acc, lane, sw + wp, bias + wp, sx + wq, out, a.F, rows - wq, cols - wp);
     else store_products<false>(piece, acc, lane, sw + wp, bias + wp, sx + wq, out, a.F, rows - wq, cols - wp);
   };
   C::run(K, load, wave, lane, acc, store);
@@ -417,9 +420,18 @@ struct Factors {
   }
   __device__ __forceinline__ void store(const QuantMatmulArgs& a, i32x4 t, float sx, int64_t n, int64_t f0) const {
     if (n >= a.N) return;
+    O o[4];
+    const bool odd = may_pass(a.D) | !(usual(sx) & usual(ws[0]) & usual(ws[1]) & usual(ws[2]) & usual(ws[3]));
+    if (__builtin_expect(__any(odd), 0)) {
+#pragma unroll
+      for (int c = 0; c < 4; ++c) o[c] = (O)scaled_any(t[c], sx, ws[c], b[c]);
+    } else {
+#pragma unroll
+      for (int c = 0; c < 4; ++c) o[c] = (O)scaled(t[c], sx, ws[c], b[c]);
+    }
 #pragma unroll
     for (int c = 0; c < 4; ++c)
-      if (f0 + c < a.F) static_cast<O*>(a.out)[n * a.F + f0 + c] = (O)scaled_any(t[c], sx, ws[c], b[c]);
+      if (f0 + c < a.F) static_cast<O*>(a.out)[n * a.F + f0 + c] = o[c];
   }
 };
 
