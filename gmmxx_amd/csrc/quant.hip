@@ -9,9 +9,9 @@
 // row that holds a NaN or an infinity has scale NaN, so its products are NaN.  Where a is so
 // small that r would pass fp32, both are taken times 2^100 first, which is exact.
 //
-// 16384 x 4096 x 8192: 520 to 560 us a product (2.0 to 2.1 POP/s).  What the operands are made of sets the
+// 16384 x 4096 x 8192: 485 to 585 us a product (1.9 to 2.3 POP/s), the longer the warmer the card.  What the operands are made of sets the
 // clock: zeros take 357 us, and matrix instructions alone, from registers, give 4.9 POP/s on zeros and 3.5 on random
-// values.  The rows in 8 bits: 35 to 50 us (201 MB).  4 x 4096 x 8192 in one kernel: 9.7 us (33.7 MB, 3.5 TB/s).
+// values.  The rows in 8 bits: 35 to 50 us (201 MB).  4 x 4096 x 8192 in one kernel: 10 us (33.7 MB, 3.4 TB/s).
 
 #include <math.h>
 
