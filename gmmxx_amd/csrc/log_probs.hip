@@ -6,14 +6,14 @@
 //   log p_t = d_t - log Z,   H = -Σ p log p = log Z - U / Z
 // Both terms of H are non-negative then.  Sums beside a reference below m (see Lean) make log Z and -U / Z larger and
 // smaller by what it lacks, at most 2.1: of rows with p near 1, log p and H, near 0, are good to some 1e-7, not to
-// digits of their own (64 to 40000 normal scores and one with p = 0.98 or 0.9996: 3e-7 to 8e-7 at most).  Of several +inf each has
-// p = 1 / their number.  The gradient from g (chosen), h (entropy) and q (alternatives) is
+// digits of their own (64 to 40000 normal scores and one with p = 0.98 or 0.9996: 3e-7 to 8e-7 at most).
+// Of several +inf each has p = 1 / their number.  The gradient from g (chosen), h (entropy) and q (alternatives) is
 //   ds_j = g [j = t] + Σ_i q_i [j = top_i] - p_j (g + Σ_i q_i + h (log p_j + H)).
 //
 // One pass over the scores: a thread keeps its own sums beside a reference, at first the largest of the first scores of
 // its wave (or group of lanes), brought to a larger one where scores pass it by much (once a 16-byte vector at most), and
-// the threads' are merged at the end, in a fixed order.  Rows are cut into parts where there are too few for the card, and joined by
-// a second kernel.
+// the threads' are merged at the end, in a fixed order.  Rows are cut into parts where there are too few for the card,
+// and joined by a second kernel.
 //
 // 8192 x 65536 bf16: 185 us call after call (1074 MB, 5.8 TB/s, some of it from caches), 228 behind a gradient whose writes
 // are still in the caches, and the gradient 396 us (2147 MB, 5.4 TB/s): bytes.  100003 x 500 fp32: 44 and 73 us.  One row
@@ -81,11 +81,12 @@ struct Plain {
 };
 
 // The same in half the instructions: sums of 2^l and 2^l l with l = s L - ref, L = log2(e) in fp32, where ref
-// need not be the largest s L, only near it.  Where a vector's sum passes the number of its scores, which one of 3.02 (fp32:
-// 2.02) above ref does, and none without one above it, ref is raised to its largest, rounded: the largest score's own l is what the rounding left, at most 1/2 where |ref| < kNear, and 64
-// where |s| < kFar: 2^22 sums of 2^64 still fit.  Below -kFar scores that differ do so by 64 at least, so
-// what is no larger weighs nothing beside other scores and is left out.  A row whose ref ends past kNear, or that
-// holds only scores left out, is taken in as Plain (see slowly).
+// need not be the largest s L, only near it.  Where a vector's sum passes the number of its scores, which one of 3.02
+// (fp32: 2.02) above ref does, and none without one above it, ref is raised to its largest, rounded: the largest
+// score's own l is what the rounding left, at most 1/2 where |ref| < kNear, and 64 where |s| < kFar: 2^22 sums of 2^64
+// still fit.  Below -kFar scores that differ do so by 64 at least, so what is no larger weighs nothing beside other
+// scores and is left out.  A row whose ref ends past kNear, or that holds only scores left out, is taken in as Plain
+// (see slowly).
 constexpr float kNear = 0x1p24f, kFar = 0x1p30f;
 struct Lean {
   float ref = -INFINITY, z = 0.f, u = 0.f;
@@ -280,7 +281,7 @@ __global__ __launch_bounds__(kThreads) void logp_rows_kernel(LogpArgs a) {
   for (int64_t n = (int64_t)blockIdx.x * R + threadIdx.x / G; n < a.N; n += (int64_t)gridDim.x * R) {
     const T* row = static_cast<const T*>(a.scores) + n * a.lds;
     Lean s;
-#pragma unroll 1                       // (a first round of its own would take registers: 65536 x 4096 bf16 107 us)
+#pragma unroll 1                       // (a first pass peeled off takes registers: 65536 x 4096 bf16 107 us, not 93)
     for (int base = 0; base < a.V; base += G * V * U) {
       const int c0 = base + lane * V;
       uint4 u[U];
@@ -795,8 +796,9 @@ __device__ __forceinline__ float slope(const Factors& f, float s) {
   return s > -INFINITY ? p * fmaf(f.h, lp + f.entropy, f.c) : 0.f;
 }
 
-// The same in fewer instructions, where |m| < kNear and the row's gradients are finite: with l = s L - k, L = log2(e) in fp32 and k = m L + log2 Z rounded
-// to fp32, p = 2^(l - off) by what k's rounding left, off (at most 2 there), and so ds = 2^l (c' + h' l).
+// The same in fewer instructions, where |m| < kNear and the row's gradients are finite: with l = s L - k, L = log2(e) in
+// fp32 and k = m L + log2 Z rounded to fp32, p = 2^(l - off) by what k's rounding left, off (at most 2 there), and so
+// ds = 2^l (c' + h' l).
 struct Quick {
   float k, c, h;
   __device__ __forceinline__ explicit Quick(const Factors& f) {
